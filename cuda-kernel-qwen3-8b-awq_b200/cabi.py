@@ -15,6 +15,8 @@ CSRC = os.path.join(_HERE, "csrc")
 QW3_OK, QW3_ERR_ARG, QW3_ERR_CUDA, QW3_ERR_IO, QW3_ERR_RANGE = 0, 1, 2, 3, 4
 QW3_ERR_TIMEOUT, QW3_ERR_DEVICE, QW3_ERR_NOMEM, QW3_ERR_STATE = 5, 6, 7, 8
 EPI_STORE, EPI_RESIDUAL, EPI_GELU, EPI_ROPE_KV, EPI_ARGMAX = range(5)
+F16, BF16 = range(2)
+ROPE_HALVES, ROPE_PAIRS = range(2)
 MAX_STAGES = 8
 
 # Every symbol include/qw3_cabi.h declares.
@@ -26,6 +28,7 @@ EXPORTS = [
     "qw3_set_batched_prefill",
     "qw3_set_chained_decode",
     "qw3_kv_upload", "qw3_layer_decode", "qw3_stage_export", "qw3_stage_connect", "qw3_stage_layers",
+    "qw3_page_slots", "qw3_rope_kv4_append", "qw3_kv4_read", "qw3_attn_kv4_decode",
     "qw3_fused_plan", "qw3_fused_repack_host", "qw3_stage_hidden", "qw3_tp_export", "qw3_tp_connect",
 ]
 
@@ -51,6 +54,30 @@ class Config(C.Structure):
                 ("rank", C.c_int32), ("world", C.c_int32), ("use_graph", C.c_int32), ("use_pdl", C.c_int32),
                 ("keep_logits", C.c_int32), ("persistent", C.c_int32), ("tensor_parallel", C.c_int32),
                 ("attn_split_min", C.c_int32), ("cluster", C.c_int32)]
+
+
+class Kv4Pool(C.Structure):
+    _fields_ = [("d_pages", C.c_void_p), ("n_pages", C.c_int64), ("page_stride", C.c_int64), ("page_size", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32)]
+
+
+class PageArgs(C.Structure):
+    _fields_ = [("d_ctx_len", C.c_void_p), ("d_new_len", C.c_void_p), ("n_req", C.c_int32), ("page_size", C.c_int32),
+                ("d_block_table", C.c_void_p), ("table_stride", C.c_int64), ("max_blocks", C.c_int32), ("free_capacity", C.c_int32),
+                ("d_free", C.c_void_p), ("d_n_free", C.c_void_p), ("d_n_free_out", C.c_void_p), ("d_cu", C.c_void_p),
+                ("d_kv_len", C.c_void_p), ("d_pos", C.c_void_p), ("d_slot", C.c_void_p), ("max_tokens", C.c_int32)]
+
+
+class Kv4AppendArgs(C.Structure):
+    _fields_ = [("d_qkv", C.c_void_p), ("qkv_stride", C.c_int64), ("tokens", C.c_int64), ("heads", C.c_int32), ("layout", C.c_int32),
+                ("rot_dim", C.c_int32), ("reserved", C.c_int32), ("d_slot", C.c_void_p), ("d_pos", C.c_void_p), ("d_cos", C.c_void_p),
+                ("d_sin", C.c_void_p), ("max_pos", C.c_int64), ("d_q_out", C.c_void_p), ("d_k_out", C.c_void_p)]
+
+
+class AttnKv4Args(C.Structure):
+    _fields_ = [("d_q", C.c_void_p), ("q_stride", C.c_int64), ("n_req", C.c_int32), ("heads", C.c_int32), ("d_block_table", C.c_void_p),
+                ("table_stride", C.c_int64), ("max_blocks", C.c_int32), ("scale", C.c_float), ("d_kv_len", C.c_void_p),
+                ("d_out", C.c_void_p)]
 
 
 def build(force=False, verbose=False):
@@ -102,6 +129,10 @@ def lib():
         "qw3_handoff_wait": [vp, i32, i64, i32, vp, vp],
         "qw3_embed_gather_w4": [vp, vp, vp, i64, i64, i64, vp, i32, vp, vp],
         "qw3_argmax_f16": [vp, i64, vp, vp, vp],
+        "qw3_page_slots": [C.POINTER(PageArgs), vp, vp],
+        "qw3_rope_kv4_append": [C.POINTER(Kv4Pool), C.POINTER(Kv4AppendArgs), vp, vp],
+        "qw3_kv4_read": [C.POINTER(Kv4Pool), vp, i64, vp, vp, vp, vp],
+        "qw3_attn_kv4_decode": [C.POINTER(Kv4Pool), C.POINTER(AttnKv4Args), vp, vp],
         "qw3_config_default": [C.POINTER(Config)],
         "qw3_create": [C.c_char_p, C.POINTER(Config), C.POINTER(vp)],
         "qw3_destroy": [vp],

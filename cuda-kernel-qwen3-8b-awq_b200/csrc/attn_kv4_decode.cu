@@ -1,0 +1,526 @@
+// Attention of single tokens over the paged 4-bit cache (attentionKernel, Inference.cu:182-266, intended math; heads grouped over KV heads).
+//
+//   score_j = c (sk_j sum_d code_jd q_d + mk_j sum_d q_d),  out = sum_j p_j (sv_j code_j + mv_j) / sum_j p_j,  c = scale * log2(e)
+//
+// The codes go into the tensor cores as they are: a nibble in the low bits of a half is the subnormal code * 2^-24 (or * 2^-20 four bits
+// further up), so a mask is all the unpacking there is, products are exact, and scales are applied to fp32 sums.  V's scale is folded into the
+// exponent: u_j = score_j + log2(sv_j), P_j = 2^(u_j - max u + 8) enters the second product as fp16 (the largest is between 2^8 and 2^15, so
+// the 11 bits reach 22 powers of two below it, whatever the scales are), and the sums of p and p mv take P_j / sv_j in fp32.
+// The two terms of the output are far larger than their sum (codes are not centred), and the tensor cores cut off what an accumulator
+// cannot hold: after four chunks at most the products go to fp32 sums in shared memory, rounded to nearest (a list of 40 K
+// tokens: error 2.0e-3 of the output's size without that, 2.1e-4 with it).
+//
+// A warp works on 32 tokens at a time, two tiles of 16 that bulk copies bring into its own ring of two: S^T = K Q^T (16 tokens x 8 heads
+// of the group), then O^T += V^T P^T, with mma.sync m16n8k16.  At 136 bytes a token and KV head the kernel is bound by HBM; one m16n8k16 a
+// token and KV head is a third of what the warp-level path can issue meanwhile, and its operands need no pass through tensor memory.
+// The 32-token chunks of all (KV head, request) pairs form one list that is cut into equal parts, one a CTA, whatever the lengths are; the four
+// warps of a CTA take its chunks in turn and join their states in shared memory, and pairs that are cut by the border of a CTA are joined
+// from the workspace by the last CTA to arrive, in order of the parts: results do not depend on timing.
+#include "kv4.cuh"
+
+namespace qw3 {
+
+constexpr int KD_WARPS = 4, KD_THREADS = 32 * KD_WARPS, KD_STAGES = 2, KD_CTAS = 4;   // CTAs an SM
+constexpr int KD_CHUNK = 32, KD_STAGE_BYTES = 2 * KV4_TILE_BYTES;
+constexpr int KD_FLUSH = 4;            // chunks whose products are summed in an accumulator
+constexpr int KD_MIN_CHUNKS = 8;       // chunks a CTA takes at least
+constexpr int KD_PART = 1024 + 32;     // floats of a partial state: outputs, then (maximum, sum of p, sum of p mv) of eight heads
+constexpr int KD_MAX_GRID = 1024;
+static_assert(2 * (size_t)KD_MAX_GRID * KD_PART <= WS_PARTIALS && KD_MAX_GRID <= WS_MAX_TILES, "workspace");
+
+struct KdSmem {
+    uint8_t ring[KD_WARPS][KD_STAGES][KD_STAGE_BYTES];
+    float4 o[KD_WARPS][8][32];        // sums of a warp, in the order of its fragments
+    float stat[KD_WARPS][8][3];
+    uint64_t bar[KD_WARPS][KD_STAGES];
+    int valid[KD_WARPS][KD_STAGES];   // tokens of the two tiles, 16 bits each
+    int last;
+};
+
+__device__ __forceinline__ float kd_ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float kd_lg2(float x) {
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float kd_rcp(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t kd_transpose(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+__device__ __forceinline__ void kd_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+struct KdParams {
+    Qw3Kv4Pool pool;
+    Qw3AttnKv4Args a;
+    int group, q_tiles, heads_t;   // heads a KV head, tiles of eight of them, (KV head, tile) pairs
+    long long most_tokens;         // that a row of the table can hold
+    float c;
+    float* part;
+    int* count;
+    int* err;
+};
+
+// A place in the list of chunks: pair `ht`, request `b`, chunk `c` of the request's `n`.
+struct KdPlace {
+    int ht, b, c, n;
+};
+
+template <class T>
+__global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(const KdParams p) {
+    extern __shared__ __align__(128) uint8_t kd_smem[];
+    KdSmem& sm = *reinterpret_cast<KdSmem*>(kd_smem);
+    using R = RowType<T>;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int B = p.a.n_req, tiles_page = p.pool.page_size / 16;
+    pdl_launch_dependents();
+    if (lane == 0) {
+        for (int s = 0; s < KD_STAGES; ++s) mbar_init(smem_u32(&sm.bar[warp][s]), 1);
+        mbar_fence_init();
+    }
+    __syncthreads();
+    pdl_wait();
+
+    const auto length = [&](int b) {
+        const int n = p.a.d_kv_len[b];
+        return n < 0 ? 0 : (long long)n > p.most_tokens ? (int)p.most_tokens : n;
+    };
+    // requests without tokens: rows of zeros
+    for (int b = blockIdx.x; b < B; b += gridDim.x) {
+        const int n = p.a.d_kv_len[b];
+        if (tid == 0 && (n < 0 || (long long)n > p.most_tokens)) kv4_error(p.err, KV4_ERR_DECODE_LEN);
+        if (length(b) == 0)
+            for (int i = tid; i < p.a.heads * 16; i += KD_THREADS) reinterpret_cast<uint4*>(static_cast<T*>(p.a.d_out) + (size_t)b * p.a.heads * 128)[i] = make_uint4(0, 0, 0, 0);
+    }
+    // this CTA's part of the list
+    long long per_head = 0;
+    for (int b = lane; b < B; b += 32) per_head += (length(b) + KD_CHUNK - 1) / KD_CHUNK;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, d);
+    const long long total = per_head * p.heads_t;
+    const long long wanted = total / KD_MIN_CHUNKS;
+    const int grid = (int)(wanted < 1 ? 1 : wanted < (long long)gridDim.x ? wanted : (long long)gridDim.x);
+    if (total == 0 || (int)blockIdx.x >= grid) return;
+    const long long x0 = total * blockIdx.x / grid, x1 = total * (blockIdx.x + 1) / grid;
+    const int n_mine = (int)(x1 - x0);   // a list of 2^31 chunks would be 10 TB
+    KdPlace place;
+    {
+        place.ht = (int)(x0 / per_head);
+        long long y = x0 - place.ht * per_head;
+        for (int b0 = 0;; b0 += 32) {
+            const int n = b0 + lane < B ? (length(b0 + lane) + KD_CHUNK - 1) / KD_CHUNK : 0;
+            int s = n;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int a = __shfl_up_sync(0xffffffffu, s, d);
+                if (lane >= d) s += a;
+            }
+            const int all = __shfl_sync(0xffffffffu, s, 31);
+            if (y < all) {
+                const int l = __ffs(__ballot_sync(0xffffffffu, y < s)) - 1;
+                place.b = b0 + l;
+                place.n = __shfl_sync(0xffffffffu, n, l);
+                place.c = (int)y - __shfl_sync(0xffffffffu, s - n, l);
+                break;
+            }
+            y -= all;
+        }
+    }
+    const auto next_request = [&](KdPlace& q) {   // the next one that has chunks
+        do {
+            if (++q.b == B) {
+                q.b = 0;
+                if (++q.ht == p.heads_t) {   // never, unless the lengths change under the kernel: then it ends all the same, inside its buffers
+                    q.ht = p.heads_t - 1;
+                    q.n = 0x7fffffff;
+                    return;
+                }
+            }
+            q.n = (length(q.b) + KD_CHUNK - 1) / KD_CHUNK;
+        } while (q.n == 0);
+    };
+
+    // copies: chunk number `k` of this warp is number warp + 4 k of the CTA; the page of the next one is looked up one ahead
+    KdPlace ahead = place;
+    int ahead_at = 0, issued = 0;       // of the CTA's chunks, of this warp's
+    int tokens = 0;                     // lanes 0 and 1: of the tile to be copied
+    const uint8_t* src = nullptr;
+    const auto look_up = [&](int at) {
+        if (at >= n_mine) return;
+        int left = at - ahead_at;
+        ahead_at = at;
+        while (left >= ahead.n - ahead.c) {
+            left -= ahead.n - ahead.c;
+            ahead.c = 0;
+            next_request(ahead);
+        }
+        ahead.c += left;
+        if (lane < 2) {
+            const int tile = 2 * ahead.c + lane;
+            const int n = length(ahead.b) - 16 * tile;
+            tokens = n < 0 ? 0 : n < 16 ? n : 16;
+            if (tokens > 0) {
+                const int in = tile / tiles_page, page = p.a.d_block_table[ahead.b * p.a.table_stride + in];
+                if (page < 0 || page >= p.pool.n_pages) {
+                    kv4_error(p.err, KV4_ERR_DECODE_PAGE);
+                    tokens = 0;
+                } else {
+                    src = static_cast<const uint8_t*>(p.pool.d_pages) + page * p.pool.page_stride +
+                          ((long long)(ahead.ht / p.q_tiles) * tiles_page + (tile - in * tiles_page)) * KV4_TILE_BYTES;
+                }
+            }
+        }
+    };
+    const auto issue = [&]() {   // the chunk that was looked up; then looks up the one after
+        const int s = issued % KD_STAGES;
+        const uint32_t bar = smem_u32(&sm.bar[warp][s]);
+        const int n0 = __shfl_sync(0xffffffffu, tokens, 0), n1 = __shfl_sync(0xffffffffu, tokens, 1);
+        if (lane == 0) {
+            sm.valid[warp][s] = n0 | n1 << 16;
+            mbar_expect_tx(bar, (uint32_t)KV4_TILE_BYTES * ((n0 > 0) + (n1 > 0)));
+        }
+        __syncwarp();
+        if (lane < 2 && tokens > 0) kd_copy(smem_u32(&sm.ring[warp][s][lane * KV4_TILE_BYTES]), src, KV4_TILE_BYTES, bar);
+        ++issued;
+        look_up(warp + KD_WARPS * issued);
+    };
+    const int my_chunks = (n_mine - warp + KD_WARPS - 1) / KD_WARPS;
+    look_up(warp);
+    for (int s = 0; s < KD_STAGES && issued < my_chunks; ++s) issue();
+
+    const int row0 = g ^ ((g >> 1) & 1);   // token of a tile that index g of a fragment stands for (and + 8): neighbours in t are of either parity,
+                                           // which halves the bank conflicts of the V rows
+    bool ok = true;
+    int done = 0, used = 0;   // chunks of the CTA's that are behind, of this warp's
+    while (done < n_mine) {
+        const int part_end = min(n_mine, done + place.n - place.c);
+        const int kvh = place.ht / p.q_tiles, q_tile = place.ht - kvh * p.q_tiles;
+        const int nq = min(8, p.group - 8 * q_tile), head0 = kvh * p.group + 8 * q_tile;
+
+        // q of the eight heads: fp16 fragments in the order of the nibbles (bf16: times a power of two of the head's own), and sums
+        uint32_t qf[4][4];   // word j of a row: low nibbles k 0..7, 8..15, high nibbles the same
+        float f0, f1, qs0, qs1;
+        {
+            uint4 w[4];
+            const uint4* src_q = reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.d_q) + place.b * p.a.q_stride + (size_t)(head0 + g) * 128 + 32 * t);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = g < nq ? src_q[j] : make_uint4(0, 0, 0, 0);
+            float sum = 0.0f, big = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = R::unpack(u[e]);
+                    sum += f.x + f.y;
+                    big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+                }
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            float f = p.c;
+            if (sizeof(T) == 2 && R::FLOOR < 1e-9f) {   // bf16: the largest value of the head goes to [2^14, 2^15)
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                const int ex = (int)(__float_as_uint(big) >> 23);   // biased; 255 for Inf
+                int shift = ex == 0 || ex == 255 ? 0 : 127 + 14 - ex;
+                shift = min(shift, 100);
+                const float up = __uint_as_float((uint32_t)(127 + shift) << 23);
+                f *= __uint_as_float((uint32_t)(127 - shift) << 23);
+                sum *= up;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t* u = &w[j].x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 v = R::unpack(u[e]);
+                        u[e] = RowType<__half>::pack(v.x * up, v.y * up);
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                qf[j][0] = __byte_perm(w[j].x, w[j].z, 0x5410);
+                qf[j][1] = __byte_perm(w[j].y, w[j].w, 0x5410);
+                qf[j][2] = __byte_perm(w[j].x, w[j].z, 0x7632);
+                qf[j][3] = __byte_perm(w[j].y, w[j].w, 0x7632);
+            }
+            f0 = __shfl_sync(0xffffffffu, f, 8 * t);
+            f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+            qs0 = __shfl_sync(0xffffffffu, sum, 8 * t);
+            qs1 = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+        }
+
+        int unflushed = 0;   // chunks in the accumulators
+        const auto flush = [&](float (&o)[8][4], float r0, float r1) {   // (sums + accumulators) times a factor a head
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float4* const at = &sm.o[warp][i][lane];
+                const float4 a = *at;
+                *at = make_float4((a.x + o[i][0]) * r0, (a.y + o[i][1]) * r1, (a.z + o[i][2]) * r0, (a.w + o[i][3]) * r1);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+            }
+            unflushed = 0;
+        };
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sm.o[warp][i][lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float o[8][4], mu0 = -INFINITY, mu1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, m0 = 0.0f, m1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+
+        for (; warp + KD_WARPS * used < part_end; ++used) {
+            const int s = used % KD_STAGES;
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.bar[warp][s]), (uint32_t)(used / KD_STAGES) & 1u));
+            if (!ok) continue;   // reported below
+            const int both = sm.valid[warp][s];
+            const uint8_t* const stage = sm.ring[warp][s];
+            float u[2][4];       // score, then u: tokens row0, row0 + 8 x heads 2t, 2t + 1
+            float inv[2][2], mv[2][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int n = both >> (16 * e) & 0xffff;
+                const uint8_t* const tile = stage + e * KV4_TILE_BYTES;
+                const uint4 ka = *reinterpret_cast<const uint4*>(tile + row0 * 64 + 16 * t), kb = *reinterpret_cast<const uint4*>(tile + row0 * 64 + 512 + 16 * t);
+                const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+                float lo[4] = {0.0f, 0.0f, 0.0f, 0.0f}, hi[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t a8 = wa[j] >> 8, b8 = wb[j] >> 8;
+                    mma_16816(lo, wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu, qf[j][0], qf[j][1]);
+                    mma_16816(hi, wa[j] & 0x00f000f0u, wb[j] & 0x00f000f0u, a8 & 0x00f000f0u, b8 & 0x00f000f0u, qf[j][2], qf[j][3]);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {   // token row0 + 8 h
+                    const bool in = row0 + 8 * h < n;
+                    const uint32_t kp = *reinterpret_cast<const uint32_t*>(tile + KV4_KP + 4 * row0 + 32 * h);
+                    const uint32_t vp = *reinterpret_cast<const uint32_t*>(tile + KV4_VP + 4 * row0 + 32 * h);
+                    const float2 ks = R::unpack(kp), vs = R::unpack(vp);
+                    const float sk = ks.x * 16777216.0f, lg = kd_lg2(vs.x);
+                    const float s0 = fmaf(sk, fmaf(hi[2 * h], 0.0625f, lo[2 * h]), ks.y * qs0), s1 = fmaf(sk, fmaf(hi[2 * h + 1], 0.0625f, lo[2 * h + 1]), ks.y * qs1);
+                    u[e][2 * h] = in ? fmaf(f0, s0, lg) : -INFINITY;
+                    u[e][2 * h + 1] = in ? fmaf(f1, s1, lg) : -INFINITY;
+                    inv[e][h] = in ? kd_rcp(vs.x) : 0.0f;
+                    mv[e][h] = in ? vs.y : 0.0f;
+                }
+            }
+            float x0m = fmaxf(fmaxf(u[0][0], u[0][2]), fmaxf(u[1][0], u[1][2])), x1m = fmaxf(fmaxf(u[0][1], u[0][3]), fmaxf(u[1][1], u[1][3]));
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) {
+                x0m = fmaxf(x0m, __shfl_xor_sync(0xffffffffu, x0m, d));
+                x1m = fmaxf(x1m, __shfl_xor_sync(0xffffffffu, x1m, d));
+            }
+            if (__any_sync(0xffffffffu, x0m > mu0 + 7.0f || x1m > mu1 + 7.0f)) {   // rare after the first chunks
+                const float n0 = fmaxf(mu0, x0m), n1 = fmaxf(mu1, x1m);
+                const float r0 = mu0 == -INFINITY ? 0.0f : kd_ex2(mu0 - n0), r1 = mu1 == -INFINITY ? 0.0f : kd_ex2(mu1 - n1);
+                mu0 = n0;
+                mu1 = n1;
+                l0 *= r0; m0 *= r0;
+                l1 *= r1; m1 *= r1;
+                flush(o, r0, r1);
+            }
+            if (unflushed == KD_FLUSH) flush(o, 1.0f, 1.0f);
+            ++unflushed;
+            const float z0 = mu0 == -INFINITY ? 0.0f : mu0 - 8.0f, z1 = mu1 == -INFINITY ? 0.0f : mu1 - 8.0f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint8_t* const tile = stage + e * KV4_TILE_BYTES + KV4_V;
+                uint32_t pf[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float p0 = kd_ex2(u[e][2 * h] - z0), p1 = kd_ex2(u[e][2 * h + 1] - z1);
+                    const uint32_t pp = RowType<__half>::pack(p0, p1);
+                    // all sums take the rounded P, so that its error meets the value and not its far larger terms; below fp16's normal
+                    // numbers, where the products no longer matter but p itself may (a tiny scale), the unrounded one
+                    const float2 pr = RowType<__half>::unpack(pp);
+                    const float w0 = (p0 >= 6.103515625e-5f ? pr.x : p0) * inv[e][h], w1 = (p1 >= 6.103515625e-5f ? pr.y : p1) * inv[e][h];
+                    l0 += w0;
+                    l1 += w1;
+                    m0 = fmaf(w0, mv[e][h], m0);
+                    m1 = fmaf(w1, mv[e][h], m1);
+                    pf[h] = kd_transpose(pp);
+                }
+                const int ra = 2 * t + (t & 1), rb = 2 * t + (~t & 1);   // tokens of indexes 2t and 2t + 1
+                const uint2 a0 = *reinterpret_cast<const uint2*>(tile + ra * 64 + 8 * g), b0 = *reinterpret_cast<const uint2*>(tile + rb * 64 + 8 * g);
+                const uint2 a1 = *reinterpret_cast<const uint2*>(tile + ra * 64 + 512 + 8 * g), b1 = *reinterpret_cast<const uint2*>(tile + rb * 64 + 512 + 8 * g);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {   // dims 16 g + 4 i .. + 3
+                    const int sel = i & 1 ? 0x7632 : 0x5410;
+                    const uint32_t x = i < 2 ? __byte_perm(a0.x, b0.x, sel) : __byte_perm(a0.y, b0.y, sel);
+                    const uint32_t y = i < 2 ? __byte_perm(a1.x, b1.x, sel) : __byte_perm(a1.y, b1.y, sel);
+                    const uint32_t x8 = x >> 8, y8 = y >> 8;
+                    mma_16816(o[2 * i], x & 0x000f000fu, x8 & 0x000f000fu, y & 0x000f000fu, y8 & 0x000f000fu, pf[0], pf[1]);
+                    mma_16816(o[2 * i + 1], x & 0x00f000f0u, x8 & 0x00f000f0u, y & 0x00f000f0u, y8 & 0x00f000f0u, pf[0], pf[1]);
+                }
+            }
+            __syncwarp();
+            if (issued < my_chunks) issue();
+        }
+
+        // the states of the four warps, then of the CTAs that share the pair
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+            m0 += __shfl_xor_sync(0xffffffffu, m0, d);
+            m1 += __shfl_xor_sync(0xffffffffu, m1, d);
+        }
+        if (!ok) l0 = l1 = NAN;
+        if (g == 0) {
+            float* const st = sm.stat[warp][2 * t];
+            st[0] = mu0; st[1] = l0; st[2] = m0;
+            st[3] = mu1; st[4] = l1; st[5] = m1;
+        }
+        flush(o, 1.0f, 1.0f);
+        __syncthreads();
+        // thread (i, lane): dims 16 g + 4 i .. + 3 of heads 2t and 2t + 1
+        const int i = warp;
+        float top[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, m[2] = {0.0f, 0.0f};
+        float4 lo = make_float4(0, 0, 0, 0), hi = make_float4(0, 0, 0, 0);
+        const auto add = [&](int h, float mu, float sl, float smv) {   // joins a state's sums of head 2t + h; returns its factor
+            const float f = mu == -INFINITY ? 0.0f : kd_ex2(mu - top[h]);
+            // a state without tokens adds nothing, one that gave up adds its NaN
+            l[h] += mu == -INFINITY ? (sl != sl ? sl : 0.0f) : sl * f;
+            m[h] += mu == -INFINITY ? 0.0f : smv * f;
+            return f;
+        };
+        const auto accumulate = [&](float4& to, const float4& from, float fa, float fb) {
+            to.x = fmaf(from.x, fa, to.x);
+            to.y = fmaf(from.y, fb, to.y);
+            to.z = fmaf(from.z, fa, to.z);
+            to.w = fmaf(from.w, fb, to.w);
+        };
+#pragma unroll
+        for (int w = 0; w < KD_WARPS; ++w)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) top[h] = fmaxf(top[h], sm.stat[w][2 * t + h][0]);
+#pragma unroll
+        for (int w = 0; w < KD_WARPS; ++w) {
+            const float* const st = sm.stat[w][2 * t];
+            const float fa = add(0, st[0], st[1], st[2]), fb = add(1, st[3], st[4], st[5]);
+            accumulate(lo, sm.o[w][2 * i][lane], fa, fb);
+            accumulate(hi, sm.o[w][2 * i + 1][lane], fa, fb);
+        }
+        const long long start = x0 + done - place.c, end = start + place.n;   // the pair's chunks in the list
+        const int first = owner_of(start, grid, total), parts = owner_of(end - 1, grid, total) - first + 1;
+        bool write = true;
+        if (parts > 1) {
+            const auto slot = [&](int k) { return p.part + (size_t)(k == 0 ? 2 * first + 1 : 2 * (first + k)) * KD_PART; };
+            float* const mine = slot((int)blockIdx.x - first);
+            reinterpret_cast<float4*>(mine)[(2 * i) * 32 + lane] = lo;
+            reinterpret_cast<float4*>(mine)[(2 * i + 1) * 32 + lane] = hi;
+            if (i == 0 && g == 0) {
+                float* const st = mine + 1024 + 6 * t;
+                st[0] = top[0]; st[1] = l[0]; st[2] = m[0];
+                st[3] = top[1]; st[4] = l[1]; st[5] = m[1];
+            }
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                const int before = atomicAdd(p.count + first, 1);
+                sm.last = before == parts - 1;
+                if (sm.last) p.count[first] = 0;
+            }
+            __syncthreads();
+            write = sm.last != 0;
+            if (write) {
+                __threadfence();
+                top[0] = top[1] = -INFINITY;
+                l[0] = l[1] = m[0] = m[1] = 0.0f;
+                lo = hi = make_float4(0, 0, 0, 0);
+                for (int k = 0; k < parts; ++k) {
+                    const float* const st = slot(k) + 1024 + 6 * t;
+                    top[0] = fmaxf(top[0], __ldcg(st));
+                    top[1] = fmaxf(top[1], __ldcg(st + 3));
+                }
+#pragma unroll 4
+                for (int k = 0; k < parts; ++k) {
+                    const float* const from = slot(k);
+                    const float* const st = from + 1024 + 6 * t;
+                    const float4 a = __ldcg(reinterpret_cast<const float4*>(from) + (2 * i) * 32 + lane), b = __ldcg(reinterpret_cast<const float4*>(from) + (2 * i + 1) * 32 + lane);
+                    const float fa = add(0, __ldcg(st), __ldcg(st + 1), __ldcg(st + 2)), fb = add(1, __ldcg(st + 3), __ldcg(st + 4), __ldcg(st + 5));
+                    accumulate(lo, a, fa, fb);
+                    accumulate(hi, b, fa, fb);
+                }
+            }
+        }
+        if (write) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (2 * t + h >= nq) continue;
+                const float r = 1.0f / l[h], a = 16777216.0f, b = 1048576.0f;   // what the nibbles' places stand for
+                const float v0 = fmaf(h ? lo.y : lo.x, a, m[h]) * r, v1 = fmaf(h ? hi.y : hi.x, b, m[h]) * r;
+                const float v2 = fmaf(h ? lo.w : lo.z, a, m[h]) * r, v3 = fmaf(h ? hi.w : hi.z, b, m[h]) * r;
+                T* const dst = static_cast<T*>(p.a.d_out) + ((size_t)place.b * p.a.heads + head0 + 2 * t + h) * 128 + 16 * g + 4 * i;
+                const bool any = l[h] != 0.0f;   // no page of the request was inside the pool
+                *reinterpret_cast<uint2*>(dst) = any ? make_uint2(R::pack(v0, v1), R::pack(v2, v3)) : make_uint2(0, 0);
+            }
+        }
+        done = part_end;
+        if (done < n_mine) {
+            place.c = 0;
+            next_request(place);
+            __syncthreads();   // sm.o and sm.stat are read
+        }
+    }
+    if (!ok) {   // a copy that did not land in time: the ones in flight are waited for
+        if (lane == 0) atomicCAS(p.err, 0, 0x30031);
+        for (int k = 0; k < KD_STAGES && k < issued; ++k)
+            mbar_wait(smem_u32(&sm.bar[warp][(issued - 1 - k) % KD_STAGES]), (uint32_t)((issued - 1 - k) / KD_STAGES) & 1u);
+    }
+}
+
+}  // namespace qw3
+
+using namespace qw3;
+
+extern "C" int qw3_attn_kv4_decode(const Qw3Kv4Pool* pool, const Qw3AttnKv4Args* a, qw3_ws_t ws, void* stream) {
+    const char* who = "qw3_attn_kv4_decode";
+    QW3_REQUIRE(a, "%s: null argument", who);
+    int rc = kv4_check(who, pool, ws);
+    if (rc != QW3_OK) return rc;
+    QW3_REQUIRE(a->n_req >= 0, "%s: n_req out of range", who);
+    if (a->n_req == 0) return QW3_OK;
+    QW3_REQUIRE(a->d_q && a->d_block_table && a->d_kv_len && a->d_out, "%s: null pointer", who);
+    QW3_REQUIRE(a->heads > 0 && a->heads <= 4096 && a->heads % pool->kv_heads == 0, "%s: heads must be a multiple of kv_heads", who);
+    QW3_REQUIRE(a->q_stride >= (int64_t)a->heads * 128 && a->q_stride % 8 == 0 && a->q_stride < ((int64_t)1 << 31), "%s: q_stride must be a multiple of 8 and hold the heads", who);
+    QW3_REQUIRE(a->max_blocks > 0 && a->table_stride >= a->max_blocks, "%s: block table out of range", who);
+    QW3_REQUIRE(((reinterpret_cast<uintptr_t>(a->d_q) | reinterpret_cast<uintptr_t>(a->d_out)) & 15) == 0, "%s: q and out must be 16-byte aligned", who);
+    QW3_REQUIRE(a->scale == a->scale && a->scale - a->scale == 0.0f, "%s: scale must be finite", who);
+    const Workspace* w = ws_struct(ws);
+    KdParams p;
+    p.pool = *pool;
+    p.a = *a;
+    p.group = a->heads / pool->kv_heads;
+    p.q_tiles = (p.group + 7) / 8;
+    p.heads_t = pool->kv_heads * p.q_tiles;
+    p.most_tokens = (long long)a->max_blocks * pool->page_size;
+    if (p.most_tokens > 0x7fffffff - 64) p.most_tokens = 0x7fffffff - 64;
+    p.c = (float)((a->scale == 0.0f ? 0.08838834764831845 : (double)a->scale) * 1.4426950408889634);
+    p.part = w->partials;
+    p.count = w->counters;
+    p.err = w->err;
+    // CTAs that the longest rows of the table could keep busy
+    const double most = (double)a->n_req * p.heads_t * (double)((p.most_tokens + KD_CHUNK - 1) / KD_CHUNK) / KD_MIN_CHUNKS;
+    int grid = w->sm_count * KD_CTAS;
+    if (grid > KD_MAX_GRID) grid = KD_MAX_GRID;
+    if (most < grid) grid = most < 1.0 ? 1 : (int)most;
+    const auto kernel = pool->dtype == QW3_F16 ? attn_kv4_decode_kernel<__half> : attn_kv4_decode_kernel<__nv_bfloat16>;
+    QW3_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(KdSmem)));
+    QW3_CUDA(kv4_launch(kernel, dim3(grid), dim3(KD_THREADS), sizeof(KdSmem), static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, p));
+    return QW3_OK;
+}

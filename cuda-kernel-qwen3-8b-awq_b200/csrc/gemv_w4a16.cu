@@ -625,6 +625,10 @@ int qw3_ws_check(qw3_ws_t ws, void* stream) {
         if (base) QW3_CUDA(cudaMemsetAsync(base + workspace_zero_from(), 0, workspace_bytes() - workspace_zero_from(), st));
         else QW3_CUDA(cudaMemsetAsync(ws->h.ws.err, 0, 4, st));
         QW3_CUDA(cudaStreamSynchronize(st));
+        if (err >= 0xE0000 && err <= 0xEffff) {   // KV4_ERR_*, kv4.cuh
+            set_last_error("an index or length outside its buffers (device error word = 0x%x)", err);
+            return QW3_ERR_RANGE;
+        }
         set_last_error("a bounded device-side wait gave up (device error word = 0x%x)", err);
         return QW3_ERR_TIMEOUT;
     }

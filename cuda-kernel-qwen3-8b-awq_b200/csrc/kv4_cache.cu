@@ -1,0 +1,366 @@
+// Paged 4-bit KV cache: pages handed out to requests that grow, rows rotated, quantised and stored, rows read back.
+#include <cooperative_groups.h>
+
+#include "kv4.cuh"
+
+namespace qw3 {
+
+// ---- block tables and slots ------------------------------------------------------------------------------------------------------
+// One cluster.  Every CTA sums the lengths of all requests for itself (two prefix sums, of new tokens and of new pages, kept in shared
+// memory), the cluster meets once, so that outputs may be the inputs' own buffers, and then its threads fill the lists: a thread takes
+// four tokens in a row and finds their request by bisection.  Bound by latency: two dependent rounds of global loads.
+constexpr int PS_THREADS = 512;
+constexpr int PS_MAX_REQ = 16384;
+
+__global__ void __launch_bounds__(PS_THREADS) page_slots_kernel(const Qw3PageArgs p, int* err) {
+    extern __shared__ int ps_smem[];
+    __shared__ long long warp_sum[2][PS_THREADS / 32];
+    const int n = p.n_req, P = p.page_size;
+    int* const cu = ps_smem;            // [n + 1] tokens before a request
+    int* const off = cu + n + 1;        // [n + 1] pages before a request
+    int* const ctx = off + n + 1;       // [n]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    const int n_free = *p.d_n_free;
+    const int each = (n + PS_THREADS - 1) / PS_THREADS, b0 = min(tid * each, n), b1 = min(b0 + each, n);
+    long long tokens = 0, pages = 0;
+    int bad = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int c = p.d_ctx_len[b], x = p.d_new_len[b];
+        ctx[b] = c;
+        if (c < 0 || x < 0) {
+            bad = max(bad, 1);
+        } else {
+            const long long need = ((long long)c + x + P - 1) / P;
+            if (need > p.max_blocks) bad = max(bad, 2);
+            pages += need - ((long long)c + P - 1) / P;
+            tokens += x;
+        }
+    }
+    long long t = tokens, g = pages;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const long long a = __shfl_up_sync(0xffffffffu, t, d), b = __shfl_up_sync(0xffffffffu, g, d);
+        if (lane >= d) { t += a; g += b; }
+    }
+    if (lane == 31) { warp_sum[0][warp] = t; warp_sum[1][warp] = g; }
+    const int any1 = __syncthreads_or(bad == 1), any2 = __syncthreads_or(bad == 2);
+    long long total = 0, total_pages = 0;
+    for (int w = 0; w < PS_THREADS / 32; ++w) {
+        if (w == warp) { t += total; g += total_pages; }
+        total += warp_sum[0][w];
+        total_pages += warp_sum[1][w];
+    }
+    int code = 0;
+    if (any1) code = KV4_ERR_LENGTH;
+    else if (any2) code = KV4_ERR_TABLE;
+    else if (n_free < 0 || n_free > p.free_capacity || total_pages > n_free) code = KV4_ERR_PAGES;
+    else if (total > p.max_tokens) code = KV4_ERR_TOKENS;
+    // below, sums fit 32 bits (max_tokens and n_free do)
+    if (code == 0) {
+        t -= tokens;
+        g -= pages;
+        for (int b = b0; b < b1; ++b) {
+            const int c = ctx[b], x = p.d_new_len[b];
+            cu[b] = (int)t;
+            off[b] = (int)g;
+            t += x;
+            g += (c + x + P - 1) / P - (c + P - 1) / P;
+        }
+    }
+    if (tid == 0) { cu[n] = (int)total; off[n] = (int)total_pages; }
+    // all CTAs have read the lengths and the number of free pages
+    if (gridDim.x > 1) cooperative_groups::this_cluster().sync();
+    else __syncthreads();
+
+    const int first = blockIdx.x * PS_THREADS + tid, step = gridDim.x * PS_THREADS;
+    const auto find = [n](const int* starts, int i) {   // the last request that starts at or before i
+        int lo = 0, hi = n;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (starts[mid] <= i) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    if (code != 0) {
+        if (first == 0) {
+            kv4_error(err, code);
+            *p.d_n_free_out = n_free;
+        }
+        for (int b = first; b <= n; b += step) {
+            p.d_cu[b] = 0;
+            if (b < n) p.d_kv_len[b] = ctx[b];
+        }
+        for (int i = first; i < p.max_tokens; i += step) { p.d_pos[i] = 0; p.d_slot[i] = -1; }
+        return;
+    }
+    if (first == 0) *p.d_n_free_out = n_free - (int)total_pages;
+    for (int b = first; b <= n; b += step) {
+        p.d_cu[b] = cu[b];
+        if (b < n) p.d_kv_len[b] = ctx[b] + cu[b + 1] - cu[b];
+    }
+    for (int i = first; i < (int)total_pages; i += step) {
+        const int b = find(off, i);
+        p.d_block_table[b * p.table_stride + (ctx[b] + P - 1) / P + i - off[b]] = p.d_free[n_free - 1 - i];
+    }
+    for (int i4 = first * 4; i4 < p.max_tokens; i4 += step * 4) {
+        int b = i4 < (int)total ? find(cu, i4) : n - 1;
+        for (int i = i4; i < min(i4 + 4, p.max_tokens); ++i) {
+            int pos = 0, slot = -1;
+            if (i < (int)total) {
+                while (cu[b + 1] <= i) ++b;
+                const int c = ctx[b];
+                pos = c + i - cu[b];
+                const int block = pos / P, fresh = block - (c + P - 1) / P;
+                const int page = fresh >= 0 ? p.d_free[n_free - 1 - (off[b] + fresh)] : p.d_block_table[b * p.table_stride + block];
+                if (page < 0 || page >= 0x7fffffff / P) kv4_error(err, KV4_ERR_FREE_ID);
+                else slot = page * P + pos % P;
+            }
+            p.d_pos[i] = pos;
+            p.d_slot[i] = slot;
+        }
+    }
+}
+
+// ---- rotation, quantisation, store -----------------------------------------------------------------------------------------------
+// A half-warp takes a row of 128 dims, eight to a lane; a CTA takes one token, whose cosines and sines its lanes keep for all heads.
+// Products and sums of the rotation are rounded one by one (no contraction), so that a row's codes do not depend on the compiler.
+// K is quantised from the fp32 rotated row, not from its rounding.
+constexpr int AP_THREADS = 256, AP_GROUPS = AP_THREADS / 16;
+
+template <class T, bool PAIRS>
+__global__ void __launch_bounds__(AP_THREADS)
+rope_kv4_append_kernel(const Qw3Kv4Pool pool, const Qw3Kv4AppendArgs p, int* err) {
+    using R = RowType<T>;
+    const int tid = threadIdx.x, group = tid >> 4, l = tid & 15;
+    const int token = blockIdx.x, kv = pool.kv_heads, P = pool.page_size, rot = p.rot_dim;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int slot = p.d_slot[token];
+    const int pos = rot > 0 ? p.d_pos[token] : 0;
+    if (rot > 0 && (pos < 0 || pos >= p.max_pos)) {
+        if (tid == 0) kv4_error(err, KV4_ERR_APPEND_POS);
+        return;
+    }
+    const int page = slot >= 0 ? slot / P : -1, in_page = slot - page * P;
+    if (page >= pool.n_pages && tid == 0) kv4_error(err, KV4_ERR_APPEND_SLOT);
+    const bool store = page >= 0 && page < pool.n_pages;
+    uint8_t* const tile0 = static_cast<uint8_t*>(pool.d_pages) + (store ? page * pool.page_stride + (in_page >> 4) * KV4_TILE_BYTES : 0);
+    const int r = in_page & 15;
+
+    float cs[8], sn[8];
+    const bool turns = 8 * l < rot;
+    // halves: lane l holds dims 8l .. 8l+7 of one half, lane `mate` their partners; pairs: four pairs in the lane
+    const bool upper = !PAIRS && 16 * l >= rot;
+    const int mate = PAIRS ? l : upper ? l - rot / 16 : l + rot / 16;
+    if (turns) {
+        const size_t at = (size_t)pos * (rot / 2) + (PAIRS ? 4 * l : 8 * (upper ? mate : l));
+        for (int e = 0; e < (PAIRS ? 4 : 8); e += 4) {
+            const float4 c = *reinterpret_cast<const float4*>(p.d_cos + at + e), s = *reinterpret_cast<const float4*>(p.d_sin + at + e);
+            cs[e] = c.x; cs[e + 1] = c.y; cs[e + 2] = c.z; cs[e + 3] = c.w;
+            sn[e] = s.x; sn[e + 1] = s.y; sn[e + 2] = s.z; sn[e + 3] = s.w;
+        }
+    }
+    const T* const row = static_cast<const T*>(p.d_qkv) + (size_t)token * p.qkv_stride + 8 * l;
+    const int rows = p.heads + 2 * kv, last = (rows + AP_GROUPS - 1) / AP_GROUPS * AP_GROUPS;   // whole rounds: the shuffles need every lane
+    for (int j = group; j < last; j += AP_GROUPS) {
+        const uint4 w = j < rows ? *reinterpret_cast<const uint4*>(row + (size_t)j * 128) : make_uint4(0, 0, 0, 0);
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = R::unpack(ws[e]);
+            x[2 * e] = f.x;
+            x[2 * e + 1] = f.y;
+        }
+        const bool is_q = j < p.heads, is_k = !is_q && j < p.heads + kv;
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = PAIRS ? 0.0f : __shfl_sync(0xffffffffu, x[e], mate, 16);
+        if ((is_q || is_k) && turns) {
+            if (PAIRS) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float a = x[2 * e], b = x[2 * e + 1];
+                    x[2 * e] = __fsub_rn(__fmul_rn(a, cs[e]), __fmul_rn(b, sn[e]));
+                    x[2 * e + 1] = __fadd_rn(__fmul_rn(b, cs[e]), __fmul_rn(a, sn[e]));
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float own = __fmul_rn(x[e], cs[e]), other = __fmul_rn(y[e], sn[e]);
+                    x[e] = upper ? __fadd_rn(own, other) : __fsub_rn(own, other);
+                }
+            }
+        }
+        if (j < rows && (is_q || (is_k && p.d_k_out != nullptr))) {
+            T* const dst = is_q ? static_cast<T*>(p.d_q_out) + ((size_t)token * p.heads + j) * 128
+                                : static_cast<T*>(p.d_k_out) + ((size_t)token * kv + j - p.heads) * 128;
+            *reinterpret_cast<uint4*>(dst + 8 * l) = make_uint4(R::pack(x[0], x[1]), R::pack(x[2], x[3]), R::pack(x[4], x[5]), R::pack(x[6], x[7]));
+        }
+        float lo = x[0], hi = x[0];
+        bool finite = true;   // a difference that is not 0 is of Inf or NaN
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            lo = fminf(lo, x[e]);
+            hi = fmaxf(hi, x[e]);
+            finite = finite && x[e] - x[e] == 0.0f;
+        }
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+        }
+        const uint32_t alive = __ballot_sync(0xffffffffu, finite) >> (tid & 16) & 0xffffu;
+        if (is_q || j >= rows || !store) continue;
+        // minimum and scale as they are stored: the codes are those of the rounded pair
+        const uint32_t m_bits = R::pack(lo, lo) & 0xffffu;
+        const float m = R::unpack(m_bits).x;
+        float s = R::unpack(R::pack(__fdiv_rn(__fsub_rn(hi, m), 15.0f), 0.0f)).x;
+        const bool whole = alive == 0xffffu && s <= R::CEIL;
+        s = fmaxf(s, R::FLOOR);
+        uint32_t codes = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float c = rintf(__fdiv_rn(__fsub_rn(x[e], m), s));
+            codes |= (uint32_t)(int)fminf(fmaxf(c, 0.0f), 15.0f) << (4 * e);
+        }
+        // a row with Inf or NaN reads back as NaN
+        const uint32_t pair = (R::pack(s, 0.0f) & 0xffffu) | (m_bits << 16);
+        uint8_t* const tile = tile0 + (size_t)(j - p.heads - (is_k ? 0 : kv)) * (P / 16) * KV4_TILE_BYTES;
+        *reinterpret_cast<uint32_t*>(tile + (is_k ? 0 : KV4_V) + r * 64 + 4 * l) = whole ? codes : 0u;
+        if (l == 0) *reinterpret_cast<uint32_t*>(tile + (is_k ? KV4_KP : KV4_VP) + r * 4) = whole ? pair : (R::pack(1.0f, 0.0f) & 0xffffu) | 0x7fff0000u;
+    }
+}
+
+// ---- rows read back --------------------------------------------------------------------------------------------------------------
+// A half-warp takes a row: four bytes of codes in, sixteen out, a lane.  A slot below zero gives a row of zeros.
+constexpr int RD_THREADS = 256, RD_GROUPS = RD_THREADS / 16;
+
+template <class T>
+__global__ void __launch_bounds__(RD_THREADS)
+kv4_read_kernel(const Qw3Kv4Pool pool, const int32_t* __restrict__ d_slot, int64_t tokens, T* __restrict__ k_out, T* __restrict__ v_out, int* err) {
+    using R = RowType<T>;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int l = threadIdx.x & 15, kv = pool.kv_heads, P = pool.page_size;
+    const int64_t rows = tokens * kv;
+    for (int64_t i = (int64_t)blockIdx.x * RD_GROUPS + (threadIdx.x >> 4); i < rows; i += (int64_t)gridDim.x * RD_GROUPS) {
+        const int64_t token = i / kv;
+        const int head = (int)(i - token * kv), slot = d_slot[token];
+        const int page = slot >= 0 ? slot / P : -1, in_page = slot - page * P;
+        if (page >= pool.n_pages && l == 0) kv4_error(err, KV4_ERR_READ_SLOT);
+        const bool there = page >= 0 && page < pool.n_pages;
+        const uint8_t* const tile = static_cast<const uint8_t*>(pool.d_pages) + (there ? page * pool.page_stride + ((int64_t)head * (P / 16) + (in_page >> 4)) * KV4_TILE_BYTES : 0);
+        const int r = in_page & 15;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            uint32_t codes = 0, pair = 0;
+            if (there) {
+                codes = *reinterpret_cast<const uint32_t*>(tile + (v ? KV4_V : 0) + r * 64 + 4 * l);
+                pair = *reinterpret_cast<const uint32_t*>(tile + (v ? KV4_VP : KV4_KP) + r * 4);
+            }
+            const float2 sm = R::unpack(pair);
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)   // code * scale is exact in fp32
+                w[e] = R::pack(fmaf((float)(codes >> (8 * e) & 15u), sm.x, sm.y), fmaf((float)(codes >> (8 * e + 4) & 15u), sm.x, sm.y));
+            *reinterpret_cast<uint4*>((v ? v_out : k_out) + (size_t)i * 128 + 8 * l) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+// ---- checks ----------------------------------------------------------------------------------------------------------------------
+int ws_on_device(const char* who, qw3_ws_t ws) {
+    QW3_REQUIRE(ws, "%s: null workspace", who);
+    int dev = -1;
+    QW3_CUDA(cudaGetDevice(&dev));
+    QW3_REQUIRE(dev == ws_struct(ws)->device, "%s: the workspace belongs to device %d, the current device is %d", who, ws_struct(ws)->device, dev);
+    return QW3_OK;
+}
+
+int kv4_check(const char* who, const Qw3Kv4Pool* pool, qw3_ws_t ws) {
+    QW3_REQUIRE(pool && pool->d_pages && ws, "%s: null pool, pages or workspace", who);
+    QW3_REQUIRE(pool->head_dim == 128, "%s: head_dim must be 128", who);
+    QW3_REQUIRE(pool->dtype == QW3_F16 || pool->dtype == QW3_BF16, "%s: dtype must be QW3_F16 or QW3_BF16", who);
+    QW3_REQUIRE(pool->page_size >= 16 && pool->page_size <= 1024 && pool->page_size % 16 == 0, "%s: page_size must be a multiple of 16, 16 to 1024", who);
+    QW3_REQUIRE(pool->kv_heads > 0 && pool->kv_heads <= 1024, "%s: kv_heads out of range", who);
+    QW3_REQUIRE(pool->n_pages > 0 && pool->n_pages <= 0x7fffffff / pool->page_size, "%s: n_pages out of range (slots have 31 bits)", who);
+    QW3_REQUIRE(pool->page_stride >= (int64_t)pool->kv_heads * pool->page_size * 136 && pool->page_stride % 16 == 0 && pool->page_stride < ((int64_t)1 << 40),
+                "%s: page_stride must be a multiple of 16 and hold kv_heads * page_size * 136 bytes", who);
+    QW3_REQUIRE((reinterpret_cast<uintptr_t>(pool->d_pages) & 15) == 0, "%s: pages must be 16-byte aligned", who);
+    return ws_on_device(who, ws);
+}
+
+static bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }
+
+}  // namespace qw3
+
+using namespace qw3;
+
+extern "C" {
+
+int qw3_page_slots(const Qw3PageArgs* a, qw3_ws_t ws, void* stream) {
+    const char* who = "qw3_page_slots";
+    QW3_REQUIRE(a && ws, "%s: null argument", who);
+    QW3_REQUIRE(a->d_ctx_len && a->d_new_len && a->d_block_table && a->d_free && a->d_n_free && a->d_n_free_out && a->d_cu && a->d_kv_len, "%s: null pointer", who);
+    QW3_REQUIRE(a->max_tokens >= 0 && (a->max_tokens == 0 || (a->d_pos && a->d_slot)), "%s: null pointer or max_tokens out of range", who);
+    QW3_REQUIRE(a->max_tokens <= 0x7fffffff - 65536, "%s: max_tokens out of range", who);
+    QW3_REQUIRE(a->n_req > 0 && a->n_req <= PS_MAX_REQ, "%s: n_req must be 1 to %d", who, PS_MAX_REQ);
+    QW3_REQUIRE(a->page_size >= 16 && a->page_size <= 1024 && a->page_size % 16 == 0, "%s: page_size must be a multiple of 16, 16 to 1024", who);
+    QW3_REQUIRE(a->max_blocks > 0 && a->max_blocks <= (0x7fffffff - 1024) / a->page_size && a->table_stride >= a->max_blocks, "%s: block table out of range", who);
+    QW3_REQUIRE(a->free_capacity >= 0, "%s: free_capacity out of range", who);
+    int rc = ws_on_device(who, ws);
+    if (rc != QW3_OK) return rc;
+    const size_t smem = (size_t)(3 * a->n_req + 2) * 4;
+    if (smem > 48 * 1024) QW3_CUDA(cudaFuncSetAttribute(page_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * PS_MAX_REQ + 2) * 4));
+    const int cluster = a->max_tokens > 4 * PS_THREADS ? 8 : 1;
+    QW3_CUDA(kv4_launch(page_slots_kernel, dim3(cluster), dim3(PS_THREADS), smem, static_cast<cudaStream_t>(stream), ws_pdl(ws), cluster, *a, ws_struct(ws)->err));
+    return QW3_OK;
+}
+
+int qw3_rope_kv4_append(const Qw3Kv4Pool* pool, const Qw3Kv4AppendArgs* a, qw3_ws_t ws, void* stream) {
+    const char* who = "qw3_rope_kv4_append";
+    QW3_REQUIRE(a, "%s: null argument", who);
+    int rc = kv4_check(who, pool, ws);
+    if (rc != QW3_OK) return rc;
+    QW3_REQUIRE(a->tokens >= 0 && a->tokens <= 0x7fffffff, "%s: tokens out of range", who);
+    QW3_REQUIRE(a->heads > 0 && a->heads <= 4096, "%s: heads out of range", who);
+    QW3_REQUIRE(a->rot_dim >= 0 && a->rot_dim <= 128 && a->rot_dim % 16 == 0, "%s: rot_dim must be a multiple of 16, 0 to 128", who);
+    QW3_REQUIRE(a->layout == QW3_ROPE_HALVES || a->layout == QW3_ROPE_PAIRS, "%s: unknown layout", who);
+    if (a->tokens == 0) return QW3_OK;
+    QW3_REQUIRE(a->d_qkv && a->d_q_out && a->d_slot, "%s: null pointer", who);
+    QW3_REQUIRE(a->rot_dim == 0 || (a->d_pos && a->d_cos && a->d_sin && a->max_pos > 0), "%s: positions and tables are needed to rotate", who);
+    QW3_REQUIRE(a->qkv_stride >= (int64_t)(a->heads + 2 * pool->kv_heads) * 128 && a->qkv_stride % 8 == 0 && a->qkv_stride < ((int64_t)1 << 31),
+                "%s: qkv_stride must be a multiple of 8 and hold heads + 2 kv_heads rows", who);
+    QW3_REQUIRE(aligned16(a->d_qkv) && aligned16(a->d_q_out) && aligned16(a->d_k_out) && aligned16(a->d_cos) && aligned16(a->d_sin),
+                "%s: rows and tables must be 16-byte aligned", who);
+    const auto kernel = pool->dtype == QW3_F16 ? (a->layout == QW3_ROPE_PAIRS ? rope_kv4_append_kernel<__half, true> : rope_kv4_append_kernel<__half, false>)
+                                               : (a->layout == QW3_ROPE_PAIRS ? rope_kv4_append_kernel<__nv_bfloat16, true> : rope_kv4_append_kernel<__nv_bfloat16, false>);
+    QW3_CUDA(kv4_launch(kernel, dim3((unsigned)a->tokens), dim3(AP_THREADS), 0, static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, *pool, *a, ws_struct(ws)->err));
+    return QW3_OK;
+}
+
+int qw3_kv4_read(const Qw3Kv4Pool* pool, const int32_t* d_slot, int64_t tokens, void* d_k_out, void* d_v_out, qw3_ws_t ws, void* stream) {
+    const char* who = "qw3_kv4_read";
+    int rc = kv4_check(who, pool, ws);
+    if (rc != QW3_OK) return rc;
+    QW3_REQUIRE(tokens >= 0 && tokens <= 0x7fffffff, "%s: tokens out of range", who);
+    if (tokens == 0) return QW3_OK;
+    QW3_REQUIRE(d_slot && d_k_out && d_v_out, "%s: null pointer", who);
+    QW3_REQUIRE(aligned16(d_k_out) && aligned16(d_v_out), "%s: rows must be 16-byte aligned", who);
+    const int64_t ctas = (tokens * pool->kv_heads + RD_GROUPS - 1) / RD_GROUPS, most = (int64_t)ws_struct(ws)->sm_count * 8;
+    const dim3 grid((unsigned)(ctas < most ? ctas : most));
+    if (pool->dtype == QW3_F16)
+        QW3_CUDA(kv4_launch(kv4_read_kernel<__half>, grid, dim3(RD_THREADS), 0, static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, *pool, d_slot, tokens,
+                        static_cast<__half*>(d_k_out), static_cast<__half*>(d_v_out), ws_struct(ws)->err));
+    else
+        QW3_CUDA(kv4_launch(kv4_read_kernel<__nv_bfloat16>, grid, dim3(RD_THREADS), 0, static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, *pool, d_slot, tokens,
+                        static_cast<__nv_bfloat16*>(d_k_out), static_cast<__nv_bfloat16*>(d_v_out), ws_struct(ws)->err));
+    return QW3_OK;
+}
+
+}  // extern "C"

@@ -127,3 +127,145 @@ def argmax_f16(logits, ws):
     tok = torch.zeros(1, dtype=torch.int32, device=logits.device)
     cabi.check(cabi.lib().qw3_argmax_f16(_ptr(logits), logits.numel(), _ptr(tok), ws.h, _stream()), "qw3_argmax_f16")
     return tok
+
+
+# ---- paged 4-bit KV cache: many requests, heads grouped over KV heads, fp16 or bf16 rows ----------------------------------------
+# Tensors may live on any CUDA device (all of a call, and its workspace, on the same one); the call goes to that device's current
+# stream.  What the device finds out of range is left out and reported by Workspace.check().
+
+_DTYPES = {torch.float16: cabi.F16, torch.bfloat16: cabi.BF16}
+
+
+def _want(cond, message):
+    if not cond:
+        raise ValueError(message)
+
+
+def _rows128(t, heads, what, device, dtype):
+    """Rows of `heads` x 128 values, the heads of a token together: [tokens][heads][128], or [tokens][heads * 128] where heads is given."""
+    _want(t.device == device and t.dtype == dtype, f"{what}: {dtype} on {device} expected")
+    if t.dim() == 3:
+        _want(t.shape[2] == 128 and t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == 128), f"{what}: [tokens][heads][128] expected, the heads of a token together")
+        n = t.shape[1]
+    else:
+        _want(t.dim() == 2 and t.shape[1] % 128 == 0 and t.stride(1) == 1, f"{what}: [tokens][heads * 128] expected")
+        n = t.shape[1] // 128
+    _want(heads is None or n == heads, f"{what}: {heads} heads expected, not {n}")
+    return n, (t.stride(0) if t.shape[0] > 1 else n * 128)
+
+
+def _ints(t, shape, what, device):
+    _want(t.device == device and t.dtype == torch.int32 and t.is_contiguous() and tuple(t.shape) == shape, f"{what}: contiguous int32 {list(shape)} on {device} expected")
+
+
+def _table(t, rows, device):
+    _want(t.device == device and t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] == rows and t.shape[1] > 0 and (t.shape[1] == 1 or t.stride(1) == 1),
+          f"block_table: int32 [{rows}][blocks] on {device} expected")
+    return t.stride(0) if rows > 1 else t.shape[1]
+
+
+def _on(device, name, *args):
+    """Calls entry point `name` on the device's current stream."""
+    _want(device.type == "cuda", f"{name}: CUDA tensors expected")
+    if device.index == torch.cuda.current_device():
+        cabi.check(getattr(cabi.lib(), name)(*args, _stream()), name)
+    else:
+        with torch.cuda.device(device):
+            cabi.check(getattr(cabi.lib(), name)(*args, _stream()), name)
+
+
+class Kv4Cache:
+    """A pool of pages of 4-bit K and V rows of one layer.  pages: uint8 [n_pages][page_bytes] (rows may be further apart, as where the
+    pages of several layers are interleaved), page_bytes = kv_heads * page_size * 136."""
+
+    def __init__(self, pages, page_size, kv_heads, dtype):
+        _want(pages.dtype == torch.uint8 and pages.dim() == 2 and pages.shape[0] > 0 and pages.stride(1) == 1, "pages: uint8 [n_pages][bytes] expected")
+        _want(dtype in _DTYPES, "dtype: torch.float16 or torch.bfloat16 expected")
+        _want(page_size >= 16 and page_size % 16 == 0 and kv_heads > 0, "page_size: a multiple of 16 expected, and kv_heads above 0")
+        _want(pages.shape[1] >= kv_heads * page_size * 136, f"pages: {kv_heads * page_size * 136} bytes a page expected")
+        self.pages, self.page_size, self.kv_heads, self.dtype = pages, page_size, kv_heads, dtype
+        stride = pages.stride(0) if pages.shape[0] > 1 else kv_heads * page_size * 136
+        self.pool = cabi.Kv4Pool(pages.data_ptr(), pages.shape[0], stride, page_size, kv_heads, 128, _DTYPES[dtype])
+
+    @classmethod
+    def alloc(cls, n_pages, page_size, kv_heads, dtype=torch.float16, device="cuda"):
+        return cls(torch.zeros(n_pages, kv_heads * page_size * 136, dtype=torch.uint8, device=device), page_size, kv_heads, dtype)
+
+
+def page_slots(ctx_len, new_len, page_size, block_table, free_pages, n_free, max_tokens, ws, kv_len=None, n_free_out=None):
+    """Pages for new_len[b] more tokens of each request, taken from the top of the stack free_pages[: n_free].  Updates block_table; returns
+    (cu, pos, slots, kv_len, n_free_out): new tokens before each request, position and slot of each new token (0 and -1 behind the last),
+    the new lengths and what is left of the stack.  kv_len=ctx_len and n_free_out=n_free update those in place."""
+    dev = ctx_len.device
+    n = ctx_len.numel()
+    _ints(ctx_len, (n,), "ctx_len", dev)
+    _ints(new_len, (n,), "new_len", dev)
+    _want(free_pages.dim() == 1, "free_pages: one dimension expected")
+    _ints(free_pages, (free_pages.numel(),), "free_pages", dev)
+    _ints(n_free, (1,), "n_free", dev)
+    stride = _table(block_table, n, dev)
+    _want(0 <= max_tokens < 2 ** 31, "max_tokens: out of range")
+    out = torch.empty(n + 1 + 2 * max_tokens, dtype=torch.int32, device=dev)
+    cu, pos, slots = out[:n + 1], out[n + 1:n + 1 + max_tokens], out[n + 1 + max_tokens:]
+    kv_len = torch.empty_like(ctx_len) if kv_len is None else kv_len
+    n_free_out = torch.empty_like(n_free) if n_free_out is None else n_free_out
+    _ints(kv_len, (n,), "kv_len", dev)
+    _ints(n_free_out, (1,), "n_free_out", dev)
+    a = cabi.PageArgs(ctx_len.data_ptr(), new_len.data_ptr(), n, page_size, block_table.data_ptr(), stride, block_table.shape[1], free_pages.numel(),
+                      free_pages.data_ptr(), n_free.data_ptr(), n_free_out.data_ptr(), cu.data_ptr(), kv_len.data_ptr(), pos.data_ptr(), slots.data_ptr(),
+                      max_tokens)
+    _on(dev, "qw3_page_slots", C.byref(a), ws.h)
+    return cu, pos, slots, kv_len, n_free_out
+
+
+def rope_kv4_append(qkv, cache, slots, pos, cos, sin, heads, ws, pairs=False):
+    """Rotates q and k of the rows qkv = [tokens][(heads + 2 kv_heads) * 128] by the angles of cos, sin = fp32 [max_pos][rot_dim / 2] (None: not
+    at all) at pos, and stores k and v in 4 bits in their slots (below 0: not stored).  Returns the rotated q [tokens][heads][128] and
+    k [tokens][kv_heads][128].  pairs: dims 2i and 2i + 1 turn together, as in rope_kv_append; else i and i + rot_dim / 2."""
+    dev, kv = qkv.device, cache.kv_heads
+    _want(cache.pages.device == dev, "qkv and the cache's pages: one device expected")
+    _, stride = _rows128(qkv, heads + 2 * kv, "qkv", dev, cache.dtype)
+    tokens = qkv.shape[0]
+    _ints(slots, (tokens,), "slots", dev)
+    rot = 0
+    if cos is not None:
+        _ints(pos, (tokens,), "pos", dev)
+        for t, what in ((cos, "cos"), (sin, "sin")):
+            _want(t is not None and t.device == dev and t.dtype == torch.float32 and t.dim() == 2 and t.is_contiguous() and t.shape == cos.shape and t.shape[0] > 0,
+                  f"{what}: contiguous float32 [max_pos][rot_dim / 2] on {dev} expected")
+        rot = 2 * cos.shape[1]
+    q = torch.empty(tokens, heads, 128, dtype=cache.dtype, device=dev)
+    k = torch.empty(tokens, kv, 128, dtype=cache.dtype, device=dev)
+    a = cabi.Kv4AppendArgs(qkv.data_ptr(), stride, tokens, heads, cabi.ROPE_PAIRS if pairs else cabi.ROPE_HALVES, rot, 0, slots.data_ptr(),
+                           pos.data_ptr() if rot else None, cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, cos.shape[0] if rot else 0,
+                           q.data_ptr(), k.data_ptr())
+    _on(dev, "qw3_rope_kv4_append", C.byref(cache.pool), C.byref(a), ws.h)
+    return q, k
+
+
+def kv4_read(cache, slots, ws):
+    """The rows of the slots as dense K and V, [tokens][kv_heads][128] each; zeros for a slot below 0."""
+    dev = cache.pages.device
+    _want(slots.dim() == 1, "slots: one dimension expected")
+    tokens = slots.numel()
+    _ints(slots, (tokens,), "slots", dev)
+    k = torch.empty(tokens, cache.kv_heads, 128, dtype=cache.dtype, device=dev)
+    v = torch.empty_like(k)
+    _on(dev, "qw3_kv4_read", C.byref(cache.pool), slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr(), ws.h)
+    return k, v
+
+
+def attn_kv4_decode(q, cache, block_table, kv_len, ws, scale=None):
+    """Attention of one token a request, q = [requests][heads][128] after rotation, over the request's kv_len tokens in the cache; a row of
+    zeros where there are none.  scale: of the scores, 1 / sqrt(128) by default."""
+    dev = q.device
+    _want(cache.pages.device == dev, "q and the cache's pages: one device expected")
+    _want(scale is None or scale != 0, "scale: 0 is not a scale")
+    heads, stride = _rows128(q, None, "q", dev, cache.dtype)
+    n = q.shape[0]
+    _ints(kv_len, (n,), "kv_len", dev)
+    table_stride = _table(block_table, n, dev)
+    out = torch.empty(n, heads, 128, dtype=cache.dtype, device=dev)
+    a = cabi.AttnKv4Args(q.data_ptr(), stride, n, heads, block_table.data_ptr(), table_stride, block_table.shape[1], scale or 0.0, kv_len.data_ptr(), out.data_ptr())
+    _on(dev, "qw3_attn_kv4_decode", C.byref(cache.pool), C.byref(a), ws.h)
+    return out

@@ -68,7 +68,8 @@ int qw3_ws_destroy(qw3_ws_t ws);
 /* enable != 0: the kernels launched with this workspace use programmatic dependent launch, so that
  * a kernel's weight prefetch overlaps the tail of the kernel before it in the stream. */
 int qw3_ws_set_pdl(qw3_ws_t ws, int enable);
-/* Reads (and clears) the device error word: QW3_OK or QW3_ERR_TIMEOUT.  Synchronises `stream`. */
+/* Reads (and clears) the device error word: QW3_OK, QW3_ERR_TIMEOUT, or QW3_ERR_RANGE where an operator of the paged cache met an index or
+ * a length outside its buffers.  Synchronises `stream`. */
 int qw3_ws_check(qw3_ws_t ws, void* stream);
 
 enum Qw3Epilogue {
@@ -173,6 +174,101 @@ int qw3_attn_prefill_status(void* stream);
  * at their barrier once and give up.  Every row of d_ctx comes back as a result or as NaN. */
 int qw3_attn_prefill_poll_once(const void* d_qkv, const void* d_k_cache, const void* d_v_cache, int32_t heads, int32_t head_dim,
                                int64_t max_pos, int32_t pos0, int32_t rows, void* d_ctx, void* stream);
+
+/* ---- Serving a batch: paged 4-bit KV cache -------------------------------------------------------------------------------
+ * The reference keeps one fp16 cache of one sequence (Inference.cu:404-407).  These operators keep the caches of many requests in
+ * pages of one pool, 4.25 bits a value, with heads grouped over KV heads.  Rows are fp16 or bf16; head_dim is 128.
+ *
+ * A row (K or V of one token and KV head) is held as 128 codes of 4 bits with one scale and one minimum in the rows' type and stands
+ * for code * scale + minimum:
+ *   minimum = T(min), scale = max(T((max - minimum) / 15), floor), code = clamp(rint((x - minimum) / scale), 0, 15)
+ * in fp32, T() rounding to the rows' type; the floor is 2^-24 (fp16) or 2^-60 (bf16).  A row with Inf or NaN (bf16: or with a range
+ * of more than 15 * 2^60) reads back as NaN.  16 tokens of a KV head lie together in 2176 bytes: 16 rows of 64 bytes of K codes (byte i:
+ * dim 2i in the low nibble), the same of V, 16 pairs (scale, minimum) of K, 16 of V; a page is [kv_heads][page_size / 16] of these.
+ *
+ * A slot is page * page_size + offset.  What the device finds out of range (slots, pages, positions, lengths) is left out, never read
+ * or written, and recorded: qw3_ws_check returns QW3_ERR_RANGE.  The workspace must belong to the current device. */
+enum Qw3Dtype { QW3_F16 = 0, QW3_BF16 = 1 };
+enum Qw3RopeLayout {
+    QW3_ROPE_HALVES = 0,  /* dim i turns with dim i + rot_dim / 2 */
+    QW3_ROPE_PAIRS = 1    /* dim 2i turns with dim 2i + 1, as the reference does (Inference.cu:150-177) */
+};
+
+typedef struct Qw3Kv4Pool {
+    void*   d_pages;      /* [n_pages][page_stride bytes], 16-byte aligned */
+    int64_t n_pages;      /* n_pages * page_size < 2^31 */
+    int64_t page_stride;  /* bytes from page to page: a multiple of 16, at least kv_heads * page_size * 136 (more where the
+                             pages of several layers are interleaved) */
+    int32_t page_size;    /* tokens a page: a multiple of 16, 16 to 1024 */
+    int32_t kv_heads;
+    int32_t head_dim;     /* 128 */
+    int32_t dtype;        /* enum Qw3Dtype, of rows, scales and minima */
+} Qw3Kv4Pool;
+
+typedef struct Qw3PageArgs {
+    const int32_t* d_ctx_len;   /* [n_req] tokens a request has in the cache */
+    const int32_t* d_new_len;   /* [n_req] tokens it adds, 0 for an idle one */
+    int32_t  n_req;             /* 1 to 16384 */
+    int32_t  page_size;
+    int32_t* d_block_table;     /* [n_req][table_stride], in/out: entry i is the page of tokens i * page_size onwards */
+    int64_t  table_stride;
+    int32_t  max_blocks;        /* entries of a row that may be used */
+    int32_t  free_capacity;     /* entries of d_free */
+    const int32_t* d_free;      /* stack of free pages, top at d_free[*d_n_free - 1] */
+    const int32_t* d_n_free;
+    int32_t* d_n_free_out;      /* what is left; may be d_n_free itself */
+    int32_t* d_cu;              /* [n_req + 1] new tokens before each request, and in all */
+    int32_t* d_kv_len;          /* [n_req] ctx + new; may be d_ctx_len itself */
+    int32_t* d_pos;             /* [max_tokens] position of each new token, 0 behind the last */
+    int32_t* d_slot;            /* [max_tokens] its slot, -1 behind the last */
+    int32_t  max_tokens;
+} Qw3PageArgs;
+
+/* Pages for the requests' new tokens, from the top of the stack in the order of requests and blocks, and the position and slot of every new
+ * token.  A call that cannot be served (a negative length, a table too narrow, too few pages, more than max_tokens tokens) changes neither
+ * table nor stack, returns no slots (all -1, cu 0, kv_len = ctx) and is reported by qw3_ws_check. */
+int qw3_page_slots(const Qw3PageArgs* args, qw3_ws_t ws, void* stream);
+
+typedef struct Qw3Kv4AppendArgs {
+    const void* d_qkv;      /* [tokens][qkv_stride]: heads rows of q, kv_heads of k, kv_heads of v, 16-byte aligned */
+    int64_t  qkv_stride;    /* elements, a multiple of 8 */
+    int64_t  tokens;
+    int32_t  heads;
+    int32_t  layout;        /* enum Qw3RopeLayout */
+    int32_t  rot_dim;       /* dims that turn, a multiple of 16 up to 128; 0: none, and d_pos, d_cos, d_sin are not read */
+    int32_t  reserved;      /* 0 */
+    const int32_t* d_slot;  /* [tokens]; below 0: the token is not stored.  The slots of a call differ */
+    const int32_t* d_pos;   /* [tokens]; a token whose position is outside the tables is left out whole */
+    const float* d_cos;     /* [max_pos][rot_dim / 2], fp32, 16-byte aligned: whatever angles the model has */
+    const float* d_sin;
+    int64_t  max_pos;
+    void*    d_q_out;       /* [tokens][heads][128] rotated q */
+    void*    d_k_out;       /* [tokens][kv_heads][128] rotated k before quantisation (for the prompt's own attention), or NULL */
+} Qw3Kv4AppendArgs;
+
+/* Rotation of q and k (fp32, one rounding), and k and v into the cache. */
+int qw3_rope_kv4_append(const Qw3Kv4Pool* pool, const Qw3Kv4AppendArgs* args, qw3_ws_t ws, void* stream);
+
+/* The rows of `tokens` slots as dense [tokens][kv_heads][128] K and V, zeros for a slot below 0: a cached prefix that a prompt attends to
+ * with qw3_attn_packed. */
+int qw3_kv4_read(const Qw3Kv4Pool* pool, const int32_t* d_slot, int64_t tokens, void* d_k_out, void* d_v_out, qw3_ws_t ws, void* stream);
+
+typedef struct Qw3AttnKv4Args {
+    const void* d_q;               /* [n_req][q_stride]: heads rows of 128, rotated, 16-byte aligned */
+    int64_t  q_stride;             /* elements, a multiple of 8 */
+    int32_t  n_req;
+    int32_t  heads;                /* a multiple of kv_heads; head h reads KV head h / (heads / kv_heads) */
+    const int32_t* d_block_table;  /* [n_req][table_stride] */
+    int64_t  table_stride;
+    int32_t  max_blocks;           /* entries of a row that may be read */
+    float    scale;                /* of the scores; 0: 1 / sqrt(128) */
+    const int32_t* d_kv_len;       /* [n_req] tokens to attend to; 0 gives a row of zeros */
+    void*    d_out;                /* [n_req][heads][128] */
+} Qw3AttnKv4Args;
+
+/* Attention of one token a request over its cached tokens (attentionKernel, Inference.cu:182-266, intended math), read as codes: the rows
+ * are never expanded.  Scores, probabilities' sums and outputs are fp32; probabilities times V scales enter the products as fp16. */
+int qw3_attn_kv4_decode(const Qw3Kv4Pool* pool, const Qw3AttnKv4Args* args, qw3_ws_t ws, void* stream);
 
 /* Embedding column gather straight from the packed [hidden][vocab] matrix (gather lambda,
  * Inference.cu:1310-1315).  Token from *d_token when it is not NULL, else `token`. */
