@@ -28,7 +28,7 @@ EXPORTS = [
     "qw3_set_batched_prefill",
     "qw3_set_chained_decode",
     "qw3_kv_upload", "qw3_layer_decode", "qw3_stage_export", "qw3_stage_connect", "qw3_stage_layers",
-    "qw3_page_slots", "qw3_rope_kv4_append", "qw3_kv4_read", "qw3_attn_kv4_decode",
+    "qw3_page_slots", "qw3_rope_kv4_append", "qw3_kv4_read", "qw3_attn_kv4_decode", "qw3_attn_packed",
     "qw3_fused_plan", "qw3_fused_repack_host", "qw3_stage_hidden", "qw3_tp_export", "qw3_tp_connect",
 ]
 
@@ -78,6 +78,13 @@ class AttnKv4Args(C.Structure):
     _fields_ = [("d_q", C.c_void_p), ("q_stride", C.c_int64), ("n_req", C.c_int32), ("heads", C.c_int32), ("d_block_table", C.c_void_p),
                 ("table_stride", C.c_int64), ("max_blocks", C.c_int32), ("scale", C.c_float), ("d_kv_len", C.c_void_p),
                 ("d_out", C.c_void_p)]
+
+
+class AttnPackedArgs(C.Structure):
+    _fields_ = [("d_q", C.c_void_p), ("q_stride", C.c_int64), ("d_k", C.c_void_p), ("k_stride", C.c_int64), ("d_v", C.c_void_p),
+                ("v_stride", C.c_int64), ("q_rows", C.c_int64), ("k_rows", C.c_int64), ("d_cu_q", C.c_void_p), ("d_cu_k", C.c_void_p),
+                ("n_seq", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32),
+                ("scale", C.c_float), ("d_out", C.c_void_p)]
 
 
 def build(force=False, verbose=False):
@@ -133,6 +140,7 @@ def lib():
         "qw3_rope_kv4_append": [C.POINTER(Kv4Pool), C.POINTER(Kv4AppendArgs), vp, vp],
         "qw3_kv4_read": [C.POINTER(Kv4Pool), vp, i64, vp, vp, vp, vp],
         "qw3_attn_kv4_decode": [C.POINTER(Kv4Pool), C.POINTER(AttnKv4Args), vp, vp],
+        "qw3_attn_packed": [C.POINTER(AttnPackedArgs), vp, vp],
         "qw3_config_default": [C.POINTER(Config)],
         "qw3_create": [C.c_char_p, C.POINTER(Config), C.POINTER(vp)],
         "qw3_destroy": [vp],

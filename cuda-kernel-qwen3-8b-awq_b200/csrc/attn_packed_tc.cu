@@ -1,0 +1,500 @@
+// Causal attention of packed prompts of different lengths, heads grouped over KV heads, on the 5th-generation tensor cores (attentionKernel,
+// Inference.cu:182-266, intended math).
+//
+// The queries of a sequence are its last rows: row i of nq sees keys 0 .. nk - nq + i.  One CTA takes 256 rows as two tiles of 128.  Where the
+// group's size has a factor `pack` of two, a row is a (token, head) pair of `pack` heads of the group: they read the same keys, so a tile
+// covers 128 / pack tokens, short sequences fill it, and less of the tiles on the diagonal is masked.  Both tiles read the same 64-key tiles of K and V.
+// Twelve warps:
+//   warp 0      TMA producer: the q rows once, then K and V tiles (64 keys x 128 dims, two 64-dim halves, 128-byte swizzle)
+//   warp 1      MMA issuer: S = Q K^T (K-major operands from shared memory), O += P V with P from tensor memory and V MN-major as it lies
+//   warp 2      zeroes the V rows behind the sequence in the last tile: they are other sequences' or nobody's, and 0 * NaN is NaN
+//   warps 4..7, 8..11   one row a thread of the upper / lower tile: S from tensor memory, online softmax, P back in its place
+// Tensor memory, per tile: O 128 columns, two S buffers of 64; P takes 32 columns of the S it comes from, rounded to the rows' type, whose
+// 8 or 11 bits the result has as well; its sum is taken before.  An fp16 P is kept between 2^8 and 2^15 at the row's maximum, so that its
+// normal numbers reach 22 powers of two below.  O is rescaled only when a row's maximum has grown by more than 7 (bf16: 8) powers of two.
+// Bound: 512 cycles of MMAs per 128 x 64 scores beside 512 cycles of exponentials.
+// All waits are bounded.  After one that gives up the error word is set, rows that are not finished are written as NaN, and the CTA
+// leaves when its copies and MMAs in flight are done.
+#include <atomic>
+
+#include "kv4.cuh"
+#include "tc05.cuh"
+
+namespace qw3 {
+
+constexpr int PK_ROWS = 128, PK_KEYS = 64, PK_STAGES = 4;
+constexpr int PK_THREADS = 384;
+constexpr int PK_Q_BYTES = PK_ROWS * 256;   // one tile of q rows: two halves of 64 dims
+constexpr int PK_KV_BYTES = PK_KEYS * 256;  // one tile of K or V
+constexpr size_t PK_SMEM = 2 * PK_Q_BYTES + 2 * (size_t)PK_STAGES * PK_KV_BYTES + 512;
+
+__device__ __forceinline__ float pk_ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+struct PackedParams {
+    Qw3AttnPackedArgs a;
+    float c;        // scale * log2(e)
+    int pack;       // heads that share a tile
+    int* err;
+};
+
+// One row by a warp, from global memory and in 32-bit arithmetic: rows whose tile holds Inf or NaN in V behind the row.  The tensor
+// cores multiply these by the zeros of the masked probabilities, and the sum is NaN; here nothing past the row's last key is read.
+template <class T>
+__device__ __noinline__ void packed_row(const T* q, const T* k, long long k_stride, const T* v, long long v_stride, int n_keys, float c, T* dst, int lane) {
+    using R = RowType<T>;
+    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // outputs 4 lane .. 4 lane + 3
+    for (int k0 = 0; k0 < n_keys; k0 += 32) {
+        float s = -INFINITY;
+        if (k0 + lane < n_keys) {
+            const uint4* kr = reinterpret_cast<const uint4*>(k + (k0 + lane) * k_stride);
+            const uint4* qr = reinterpret_cast<const uint4*>(q);
+            s = 0.0f;
+            for (int i = 0; i < 16; ++i) {
+                const uint4 a = qr[i], b = kr[i];
+                const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 x = R::unpack(aw[e]), y = R::unpack(bw[e]);
+                    s = fmaf(x.y, y.y, fmaf(x.x, y.x, s));
+                }
+            }
+        }
+        float mn = fmaxf(m, s);
+        for (int d = 16; d > 0; d >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
+        const float f = m == -INFINITY ? 0.0f : pk_ex2((m - mn) * c), pr = s == -INFINITY ? 0.0f : pk_ex2((s - mn) * c);
+        m = mn;
+        l = l * f + pr;   // this lane's keys
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= f;
+        for (int j = 0; j < 32 && k0 + j < n_keys; ++j) {
+            const float pj = __shfl_sync(0xffffffffu, pr, j);
+            const uint2 w = *reinterpret_cast<const uint2*>(v + (k0 + j) * v_stride + 4 * lane);
+            const float2 a = R::unpack(w.x), b = R::unpack(w.y);
+            o[0] = fmaf(pj, a.x, o[0]);
+            o[1] = fmaf(pj, a.y, o[1]);
+            o[2] = fmaf(pj, b.x, o[2]);
+            o[3] = fmaf(pj, b.y, o[3]);
+        }
+    }
+    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    *reinterpret_cast<uint2*>(dst + 4 * lane) = make_uint2(R::pack(o[0] / l, o[1] / l), R::pack(o[2] / l, o[3] / l));
+}
+
+template <class T>
+__global__ void __launch_bounds__(PK_THREADS, 1)
+attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                   const PackedParams p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ int s_place[4];   // the CTA's sequence: first row of q and of k, rows of q, of k; and its block of rows
+    __shared__ int s_block;
+    using R = RowType<T>;
+    constexpr bool HALF = R::FLOOR > 1e-9f;                        // fp16
+    constexpr float SHIFT = HALF ? 8.0f : 0.0f, LAG = HALF ? 7.0f : 8.0f;
+    uint8_t* q_s = smem;
+    uint8_t* k_s = q_s + 2 * PK_Q_BYTES;
+    uint8_t* v_s = k_s + PK_STAGES * PK_KV_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + PK_STAGES * PK_KV_BYTES);
+    const uint32_t q_full = smem_u32(bars), k_full = q_full + 8, v_full = k_full + 8 * PK_STAGES, k_empty = v_full + 8 * PK_STAGES,
+                   v_empty = k_empty + 8 * PK_STAGES, s_full = v_empty + 8 * PK_STAGES /* [tile][buffer] */, p_full = s_full + 32,
+                   pv_done = p_full + 32 /* [tile][buffer] */, drain = pv_done + 32, v_last = drain + 8, v_clean = v_last + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 + 4 * PK_STAGES + 12);
+    volatile int* s_dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const auto give_up = [&](int code) {
+        atomicCAS(p.err, 0, code);
+        *s_dead = 1;
+    };
+    const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
+    const int pack = p.pack, block_tokens = 2 * PK_ROWS / pack, tile_tokens = PK_ROWS / pack;
+    const int groups = p.a.heads / pack;
+    const int head0 = (int)(blockIdx.x % groups) * pack;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    // the block of rows: the last sequence's last block comes first (the blocks with the most keys of a sequence start first)
+    if (warp == 0) {
+        int left = (int)(blockIdx.x / groups), found = -1;
+        for (int b0 = p.a.n_seq; b0 > 0 && found < 0; b0 -= 32) {
+            const int b = b0 - 1 - lane;
+            int q0 = 0, nq = 0, k0 = 0, nk = 0, bad = 0;
+            if (b >= 0) {
+                const int qa = p.a.d_cu_q[b], qb = p.a.d_cu_q[b + 1], ka = p.a.d_cu_k[b], kb = p.a.d_cu_k[b + 1];
+                bad = qa < 0 || qb < qa || (long long)qb > p.a.q_rows || ka < 0 || kb < ka || (long long)kb > p.a.k_rows;
+                if (!bad) { q0 = qa; nq = qb - qa; k0 = ka; nk = kb - ka; }
+            }
+            const int blocks = (nq + block_tokens - 1) / block_tokens;
+            int sum = blocks;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int x = __shfl_up_sync(0xffffffffu, sum, d);
+                if (lane >= d) sum += x;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, left < sum);
+            if (hit != 0) {
+                found = __ffs(hit) - 1;
+                if (lane == found) {
+                    s_place[0] = q0; s_place[1] = k0; s_place[2] = nq; s_place[3] = nk;
+                    s_block = blocks - 1 - (left - (sum - blocks));
+                }
+            }
+            left -= __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (found < 0 && lane == 0) s_block = -1;
+        // CTA 0 looks at all sequences, for their reports
+        if (blockIdx.x == 0)
+            for (int b = lane; b < p.a.n_seq; b += 32) {
+                const int qa = p.a.d_cu_q[b], qb = p.a.d_cu_q[b + 1], ka = p.a.d_cu_k[b], kb = p.a.d_cu_k[b + 1];
+                if (qa < 0 || qb < qa || (long long)qb > p.a.q_rows || ka < 0 || kb < ka || (long long)kb > p.a.k_rows) kv4_error(p.err, KV4_ERR_PACKED_CU);
+            }
+    }
+    if (tid == 0) {
+        mbar_init(q_full, 1);
+        mbar_init(drain, 1);
+        mbar_init(v_last, 1);
+        mbar_init(v_clean, 1);
+        for (int s = 0; s < PK_STAGES; ++s) {
+            mbar_init(k_full + 8 * s, 1);
+            mbar_init(v_full + 8 * s, 1);
+            mbar_init(k_empty + 8 * s, 1);
+            mbar_init(v_empty + 8 * s, 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(p_full + 8 * i, 4);   // the four warps of the tile
+            mbar_init(pv_done + 8 * i, 1);
+        }
+        *s_dead = 0;
+        mbar_fence_init();
+    }
+    __syncthreads();
+    if (s_block < 0) return;
+    const int seq_q0 = s_place[0], seq_k0 = s_place[1], nq = s_place[2], nk = s_place[3];
+    const int t0 = s_block * block_tokens, past = nk - nq;   // token i of the block is t0 + i; it sees keys 0 .. past + t0 + i
+    const int n_keys = min(nk, past + min(t0 + block_tokens, nq));
+    T* const out = static_cast<T*>(p.a.d_out) + (size_t)(seq_q0 + t0) * p.a.heads * 128 + (size_t)head0 * 128;
+    if (n_keys <= 0) {   // no row of the block sees a key
+        const int rows = min(block_tokens, nq - t0) * pack;
+        for (int i = tid; i < rows * 16; i += PK_THREADS)
+            reinterpret_cast<uint4*>(out + ((size_t)(i / 16 / pack) * p.a.heads + i / 16 % pack) * 128)[i & 15] = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    const int n_tiles = (n_keys + PK_KEYS - 1) / PK_KEYS;
+    const bool ragged = n_keys % PK_KEYS != 0;
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;   // O of the tiles at columns 0 and 128, S at 256 + 128 tile + 64 buffer
+
+    if (warp == 0) {
+        if (elect_one()) {
+            bool ok = true;
+            const int kv_head = head0 / (p.a.heads / p.a.kv_heads);
+            mbar_expect_tx(q_full, 2 * PK_Q_BYTES);
+            for (int t = 0; t < 2; ++t)
+                for (int h = 0; h < 2; ++h)
+                    tma_load_3d(smem_u32(q_s + t * PK_Q_BYTES + h * (PK_Q_BYTES / 2)), &tm_q, 64 * h, head0, seq_q0 + t0 + tile_tokens * t, q_full);
+            int j = 0, kv = 0;
+            for (; j < n_tiles; ++j) {
+                const int s = j % PK_STAGES;
+                const uint32_t lap = (uint32_t)(j / PK_STAGES);
+                for (kv = 0; kv < 2; ++kv) {
+                    const uint32_t full = (kv ? v_full : k_full) + 8 * s, empty = (kv ? v_empty : k_empty) + 8 * s;
+                    uint8_t* dst = (kv ? v_s : k_s) + s * PK_KV_BYTES;
+                    if (lap > 0) ok = mbar_wait(empty, (lap - 1) & 1u);
+                    if (*s_dead != 0) ok = false;
+                    if (!ok) break;
+                    mbar_expect_tx(full, PK_KV_BYTES);
+                    for (int h = 0; h < 2; ++h)
+                        tma_load_3d(smem_u32(dst + h * (PK_KV_BYTES / 2)), kv ? &tm_v : &tm_k, 64 * h, seq_k0 + j * PK_KEYS, kv_head, full);
+                }
+                if (!ok) break;
+            }
+            if (ok && ragged) {   // this thread knows the lap that the barrier is in; warp 2 does not
+                ok = mbar_wait(v_full + 8 * ((n_tiles - 1) % PK_STAGES), (uint32_t)((n_tiles - 1) / PK_STAGES) & 1u);
+                mbar_arrive(v_last);
+            }
+            // drain: the last release arrivals land before the CTA may leave
+            for (int i = n_tiles < PK_STAGES ? 0 : n_tiles - PK_STAGES; i < n_tiles && ok; ++i) {
+                const uint32_t parity = (uint32_t)(i / PK_STAGES) & 1u;
+                ok = mbar_wait(k_empty + 8 * (i % PK_STAGES), parity) && mbar_wait(v_empty + 8 * (i % PK_STAGES), parity);
+            }
+            if (!ok) {
+                give_up(0x30041);
+                mbar_wait(q_full, 0);   // the copies in flight
+                for (int t = 0; t < 2; ++t) {
+                    const int asked = j < n_tiles && t < kv ? j + 1 : j;   // tiles of K, of V
+                    for (int i = max(asked - PK_STAGES, 0); i < asked; ++i)
+                        mbar_wait((t ? v_full : k_full) + 8 * (i % PK_STAGES), (uint32_t)(i / PK_STAGES) & 1u);
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (elect_one()) {
+            // D = f32, A and B of the rows' type.  S: N = 64 keys, both K-major.  P V: N = 128 dims, V MN-major (bit 16).
+            const uint32_t types = (1u << 4) | (HALF ? 0u : (1u << 7) | (1u << 10));
+            const uint32_t idesc_s = types | ((uint32_t)(PK_KEYS >> 3) << 17) | ((uint32_t)(PK_ROWS >> 4) << 24);
+            const uint32_t idesc_o = types | (1u << 16) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(PK_ROWS >> 4) << 24);
+            const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024), kd = make_smem_desc(smem_u32(k_s), 16, 1024);
+            const uint64_t vd = make_smem_desc(smem_u32(v_s), PK_KV_BYTES / 2, 1024);   // 64-dim halves, 8-key groups
+            auto scores = [&](int t, int j) {   // S of tile t against key tile j
+                const uint32_t d = tmem + 256 + 128 * t + 64 * (j & 1);
+                const uint64_t a = qd + (uint64_t)(t * (PK_Q_BYTES >> 4)), b = kd + (uint64_t)((j % PK_STAGES) * (PK_KV_BYTES >> 4));
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks)
+                    umma_f16(d, a + (uint64_t)((ks >> 2) * (PK_Q_BYTES >> 5) + (ks & 3) * 2), b + (uint64_t)((ks >> 2) * (PK_KV_BYTES >> 5) + (ks & 3) * 2),
+                             idesc_s, ks > 0 ? 1u : 0u);
+                umma_commit(s_full + 16 * t + 8 * (j & 1));
+            };
+            bool ok = mbar_wait(q_full, 0);
+            for (int j = 0; j < 2 && j < n_tiles && ok; ++j) {
+                ok = mbar_wait(k_full + 8 * j, 0);
+                if (!ok) break;
+                scores(0, j);
+                scores(1, j);
+                umma_commit(k_empty + 8 * j);
+            }
+            for (int j = 0; j < n_tiles && ok; ++j) {
+                const int s = j % PK_STAGES, b = j & 1;
+                ok = *s_dead == 0 && (j == n_tiles - 1 && ragged ? mbar_wait(v_clean, 0) : mbar_wait(v_full + 8 * s, (uint32_t)(j / PK_STAGES) & 1u));
+                for (int t = 0; t < 2 && ok; ++t) {
+                    ok = mbar_wait(p_full + 16 * t + 8 * b, (uint32_t)(j >> 1) & 1u);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t a = tmem + 256 + 128 * t + 64 * b;
+                    const uint64_t v = vd + (uint64_t)(s * (PK_KV_BYTES >> 4));
+#pragma unroll
+                    for (int ks = 0; ks < PK_KEYS / 16; ++ks)
+                        umma_f16_ts(tmem + 128 * t, a + 8 * ks, v + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
+                    umma_commit(pv_done + 16 * t + 8 * b);
+                    if (t == 1) umma_commit(v_empty + 8 * s);
+                    // the next scores of the buffer: issued after, and so executed after, the product that reads P there
+                    if (j + 2 < n_tiles) {
+                        const int s2 = (j + 2) % PK_STAGES;
+                        if (t == 0) ok = mbar_wait(k_full + 8 * s2, (uint32_t)((j + 2) / PK_STAGES) & 1u);
+                        if (!ok) break;
+                        scores(t, j + 2);
+                        if (t == 1) umma_commit(k_empty + 8 * s2);
+                    }
+                }
+            }
+            if (!ok) give_up(0x30042);
+            if (!ok || *s_dead != 0) {   // the MMAs in flight
+                umma_commit(drain);
+                mbar_wait(drain, 0);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 2) {
+        if (ragged) {
+            const int s = (n_tiles - 1) % PK_STAGES, from = n_keys % PK_KEYS;
+            const bool ok = __all_sync(0xffffffffu, mbar_wait(v_last, 0));
+            if (ok) {
+                for (int i = lane; i < (PK_KEYS - from) * 16; i += 32) {   // rows of 128 bytes in either half
+                    const int h = i / ((PK_KEYS - from) * 8), in = i - h * (PK_KEYS - from) * 8;
+                    *reinterpret_cast<uint4*>(v_s + s * PK_KV_BYTES + h * (PK_KV_BYTES / 2) + from * 128 + in * 16) = make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            } else if (lane == 0) {
+                give_up(0x30044);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(v_clean);
+        }
+    } else if (warp >= 4) {
+        const int t = (warp - 4) >> 2, q = warp & 3;
+        const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16);
+        const uint32_t o_at = lane_base + 128 * t, s_at = lane_base + 256 + 128 * t;
+        const int row = 32 * q + lane, token = tile_tokens * t + row / pack;   // of the block
+        const int pos = min(past + t0 + token, n_keys - 1);                    // last key the row sees
+        const int pos_first = min(past + t0 + tile_tokens * t + 32 * q / pack, n_keys - 1);   // of the warp's first row
+        const float c = p.c;
+        float m = -INFINITY, l = 0.0f;           // m: maximum in use (raw scores)
+        float oh = -SHIFT, ol = 0.0f;            // P = 2^(s c - oh - ol)
+        bool large = false;                      // m c has no fraction left in fp32: then oh = m c, ol its rounding error, and m is taken off s first
+        bool ok = true;
+        for (int j = 0; j < n_tiles && ok; ++j) {
+            const int b = j & 1;
+            ok = __all_sync(0xffffffffu, *s_dead == 0 && mbar_wait(s_full + 16 * t + 8 * b, (uint32_t)(j >> 1) & 1u));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t sr[64];
+            float s[64];
+            tmem_ld32(s_at + 64 * b, sr);
+            tmem_ld32(s_at + 64 * b + 32, sr + 32);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 64; ++e) s[e] = __uint_as_float(sr[e]);
+            const int k0 = j * PK_KEYS;
+            if (k0 + PK_KEYS - 1 > pos_first) {   // some row of the warp does not see the whole tile
+#pragma unroll
+                for (int e = 0; e < 64; ++e) s[e] = k0 + e <= pos ? s[e] : -INFINITY;
+            }
+            float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int e = 4; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
+            const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            if (__any_sync(0xffffffffu, (mt - m) * c > LAG || large)) {   // rare after the first tile
+                const float mn = fmaxf(m, mt), mc = mn == -INFINITY ? 0.0f : mn * c;
+                const bool nl = fabsf(mc) >= 1048576.0f;
+                const float nh = nl ? mc : mc - SHIFT, nlow = nl ? fmaf(mn, c, -mc) - SHIFT : 0.0f;
+                const float f = m == -INFINITY ? 0.0f : pk_ex2((oh - nh) + (ol - nlow));
+                if (j > 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(pv_done + 16 * t + 8 * (b ^ 1), (uint32_t)((j - 1) >> 1) & 1u));
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        uint32_t o[32];
+                        tmem_ld32(o_at + 32 * h, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st32(o_at + 32 * h, o);
+                    }
+                }
+                l *= f;
+                m = mn;
+                oh = nh;
+                ol = nlow;
+                large = nl;
+                if (__any_sync(0xffffffffu, large)) {
+                    const float base = large ? m : 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 64; ++e) s[e] -= base;
+                }
+            }
+            const float off = large ? -SHIFT : oh;
+            float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float a0 = pk_ex2(fmaf(s[32 * h + 2 * e], c, -off)), a1 = pk_ex2(fmaf(s[32 * h + 2 * e + 1], c, -off));
+                    ls[(2 * e) & 3] += a0;
+                    ls[(2 * e + 1) & 3] += a1;
+                    w[e] = R::pack(a0, a1);
+                }
+                tmem_st16(s_at + 64 * b + 16 * h, w);
+            }
+            l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 16 * t + 8 * b);
+        }
+        for (int j = n_tiles < 2 ? 0 : n_tiles - 2; j < n_tiles && ok; ++j)
+            ok = __all_sync(0xffffffffu, mbar_wait(pv_done + 16 * t + 8 * (j & 1), (uint32_t)(j >> 1) & 1u));
+        if (!ok && lane == 0) give_up(0x30043);
+        __syncwarp();
+        tc_fence_after();
+        const bool mine = t0 + token < nq;
+        T* const dst = out + ((size_t)token * p.a.heads + row % pack) * 128;
+        const float r = pos < 0 ? 0.0f : 1.0f / l;   // a row that sees no key is zeros
+        float finite = 0.0f;   // NaN as soon as an output is NaN or Inf
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            uint32_t o[32];
+            __syncwarp();
+            tmem_ld32(o_at + 32 * h, o);
+            tmem_wait_ld();
+            if (mine) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float x = __uint_as_float(o[e + 2 * k]) * r, y = __uint_as_float(o[e + 2 * k + 1]) * r;
+                        finite = fmaf(x, 0.0f, fmaf(y, 0.0f, finite));
+                        w[k] = !ok ? 0x7fff7fffu : pos < 0 ? 0u : R::pack(x, y);
+                    }
+                    *reinterpret_cast<uint4*>(dst + 32 * h + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        }
+        __syncwarp();   // a row that is done again has been stored
+        for (uint32_t redo = ok ? __ballot_sync(0xffffffffu, mine && pos >= 0 && finite != 0.0f) : 0u; redo != 0; redo &= redo - 1) {
+            const int rr = 32 * q + __ffs(redo) - 1, tok = tile_tokens * t + rr / pack, head = head0 + rr % pack;
+            const int kv_head = head / (p.a.heads / p.a.kv_heads);
+            packed_row<T>(static_cast<const T*>(p.a.d_q) + (seq_q0 + t0 + tok) * p.a.q_stride + head * 128,
+                          static_cast<const T*>(p.a.d_k) + seq_k0 * p.a.k_stride + kv_head * 128, p.a.k_stride,
+                          static_cast<const T*>(p.a.d_v) + seq_k0 * p.a.v_stride + kv_head * 128, p.a.v_stride, past + t0 + tok + 1, c,
+                          out + ((size_t)tok * p.a.heads + rr % pack) * 128, lane);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <class T>
+static int packed_launch(const Qw3AttnPackedArgs& a, const Workspace* ws, bool pdl, cudaStream_t st) {
+    PackedParams p;
+    p.a = a;
+    p.c = (float)((a.scale == 0.0f ? 0.08838834764831845 : (double)a.scale) * 1.4426950408889634);
+    const int group = a.heads / a.kv_heads;
+    p.pack = group & -group;
+    if (p.pack > 16) p.pack = 16;
+    p.err = ws->err;
+    CUtensorMap tm_q, tm_k, tm_v;
+    const uint64_t qd[3] = {128, (uint64_t)a.heads, (uint64_t)a.q_rows}, qs[2] = {256, (uint64_t)a.q_stride * 2};
+    const uint32_t qb[3] = {64, (uint32_t)p.pack, (uint32_t)(PK_ROWS / p.pack)}, kb[3] = {64, PK_KEYS, 1};
+    int rc = encode_f16_map(&tm_q, a.d_q, 3, qd, qs, qb);
+    if (rc != QW3_OK) return rc;
+    if (a.k_rows > 0) {
+        const uint64_t kd[3] = {128, (uint64_t)a.k_rows, (uint64_t)a.kv_heads}, ks[2] = {(uint64_t)a.k_stride * 2, 256}, vs[2] = {(uint64_t)a.v_stride * 2, 256};
+        rc = encode_f16_map(&tm_k, a.d_k, 3, kd, ks, kb);
+        if (rc == QW3_OK) rc = encode_f16_map(&tm_v, a.d_v, 3, kd, vs, kb);
+        if (rc != QW3_OK) return rc;
+    } else {
+        tm_k = tm_v = tm_q;   // no sequence has a key: no copy is made
+    }
+    static std::atomic<bool> attr_set[64];   // per device: the kernel's shared-memory limit is raised once
+    const int dev = ws->device;
+    if (dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
+        QW3_CUDA(cudaFuncSetAttribute(attn_packed_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PK_SMEM));
+        if (dev < 64) attr_set[dev].store(true, std::memory_order_release);
+    }
+    // every sequence ends with one block that may not be full
+    const int64_t block_tokens = 2 * PK_ROWS / p.pack, blocks = (a.q_rows / block_tokens + a.n_seq) * (a.heads / p.pack);
+    QW3_REQUIRE(blocks <= 0x7fffffff, "qw3_attn_packed: too many rows");
+    QW3_CUDA(kv4_launch(attn_packed_kernel<T>, dim3((unsigned)blocks), dim3(PK_THREADS), PK_SMEM, st, pdl, 1, tm_q, tm_k, tm_v, p));
+    return QW3_OK;
+}
+
+}  // namespace qw3
+
+using namespace qw3;
+
+extern "C" int qw3_attn_packed(const Qw3AttnPackedArgs* a, qw3_ws_t ws, void* stream) {
+    const char* who = "qw3_attn_packed";
+    QW3_REQUIRE(a && ws, "%s: null argument", who);
+    QW3_REQUIRE(a->head_dim == 128, "%s: head_dim must be 128", who);
+    QW3_REQUIRE(a->dtype == QW3_F16 || a->dtype == QW3_BF16, "%s: dtype must be QW3_F16 or QW3_BF16", who);
+    QW3_REQUIRE(a->kv_heads > 0 && a->heads > 0 && a->heads <= 4096 && a->heads % a->kv_heads == 0, "%s: heads must be a multiple of kv_heads", who);
+    QW3_REQUIRE(a->q_rows >= 0 && a->q_rows <= 0x7fffffff - 1024 && a->k_rows >= 0 && a->k_rows <= 0x7fffffff - 1024 && a->n_seq >= 0, "%s: rows or n_seq out of range", who);
+    QW3_REQUIRE(a->scale >= 0.0f && a->scale - a->scale == 0.0f, "%s: scale must be finite and not below 0", who);
+    if (a->q_rows == 0 || a->n_seq == 0) return QW3_OK;
+    QW3_REQUIRE(a->d_q && a->d_out && a->d_cu_q && a->d_cu_k && (a->k_rows == 0 || (a->d_k && a->d_v)), "%s: null pointer", who);
+    const auto stride_ok = [](int64_t s, int heads) { return s >= (int64_t)heads * 128 && s % 8 == 0 && s < ((int64_t)1 << 31); };
+    QW3_REQUIRE(stride_ok(a->q_stride, a->heads) && (a->k_rows == 0 || (stride_ok(a->k_stride, a->kv_heads) && stride_ok(a->v_stride, a->kv_heads))),
+                "%s: strides must be multiples of 8 and hold the heads", who);
+    QW3_REQUIRE(((reinterpret_cast<uintptr_t>(a->d_q) | reinterpret_cast<uintptr_t>(a->d_out) | reinterpret_cast<uintptr_t>(a->d_k) | reinterpret_cast<uintptr_t>(a->d_v)) & 15) == 0,
+                "%s: rows must be 16-byte aligned", who);
+    const int rc = ws_on_device(who, ws);
+    if (rc != QW3_OK) return rc;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return a->dtype == QW3_F16 ? packed_launch<__half>(*a, ws_struct(ws), ws_pdl(ws), st) : packed_launch<__nv_bfloat16>(*a, ws_struct(ws), ws_pdl(ws), st);
+}

@@ -269,3 +269,27 @@ def attn_kv4_decode(q, cache, block_table, kv_len, ws, scale=None):
     a = cabi.AttnKv4Args(q.data_ptr(), stride, n, heads, block_table.data_ptr(), table_stride, block_table.shape[1], scale or 0.0, kv_len.data_ptr(), out.data_ptr())
     _on(dev, "qw3_attn_kv4_decode", C.byref(cache.pool), C.byref(a), ws.h)
     return out
+
+
+def attn_packed(q, k, v, cu_q, cu_k, ws, scale=None, out=None):
+    """Causal attention of packed sequences: q [q_rows][heads][128], k and v [k_rows][kv_heads][128] (rows may be further apart), sequence b in
+    rows cu_q[b] .. cu_q[b + 1] of q and cu_k[b] .. cu_k[b + 1] of k and v.  Its queries are its last rows: row i of nq sees keys
+    0 .. nk - nq + i, a row that sees none is zeros.  Rows behind the last sequence are left as they were (undefined in a new `out`)."""
+    dev, dtype = q.device, q.dtype
+    _want(dtype in _DTYPES, "q: torch.float16 or torch.bfloat16 expected")
+    _want(scale is None or scale > 0, "scale: above 0 expected")
+    heads, q_stride = _rows128(q, None, "q", dev, dtype)
+    kv, k_stride = _rows128(k, None, "k", dev, dtype)
+    _, v_stride = _rows128(v, kv, "v", dev, dtype)
+    _want(v.shape[0] == k.shape[0], "k and v: the same number of rows expected")
+    n = cu_q.numel() - 1
+    _want(n >= 0, "cu_q: [sequences + 1] expected")
+    _ints(cu_q, (n + 1,), "cu_q", dev)
+    _ints(cu_k, (n + 1,), "cu_k", dev)
+    if out is None:
+        out = torch.empty(q.shape[0], heads, 128, dtype=dtype, device=dev)
+    _want(out.device == dev and out.dtype == dtype and out.is_contiguous() and out.numel() == q.shape[0] * heads * 128, "out: contiguous [q_rows][heads][128] expected")
+    a = cabi.AttnPackedArgs(q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, q.shape[0], k.shape[0], cu_q.data_ptr(), cu_k.data_ptr(), n,
+                            heads, kv, 128, _DTYPES[dtype], scale or 0.0, out.data_ptr())
+    _on(dev, "qw3_attn_packed", C.byref(a), ws.h)
+    return out

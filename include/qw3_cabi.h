@@ -270,6 +270,33 @@ typedef struct Qw3AttnKv4Args {
  * are never expanded.  Scores, probabilities' sums and outputs are fp32; probabilities times V scales enter the products as fp16. */
 int qw3_attn_kv4_decode(const Qw3Kv4Pool* pool, const Qw3AttnKv4Args* args, qw3_ws_t ws, void* stream);
 
+typedef struct Qw3AttnPackedArgs {
+    const void* d_q;          /* [q_rows][q_stride]: heads rows of 128, rotated; rows 16-byte aligned, strides in elements, multiples of 8 */
+    int64_t  q_stride;
+    const void* d_k;          /* [k_rows][k_stride]: kv_heads rows of 128, rotated */
+    int64_t  k_stride;
+    const void* d_v;          /* [k_rows][v_stride] */
+    int64_t  v_stride;
+    int64_t  q_rows;          /* rows of the buffers; the sequences may end before */
+    int64_t  k_rows;
+    const int32_t* d_cu_q;    /* [n_seq + 1] first row of each sequence in q, and the end of the last */
+    const int32_t* d_cu_k;    /* [n_seq + 1] the same in k and v */
+    int32_t  n_seq;
+    int32_t  heads;           /* a multiple of kv_heads; head h reads KV head h / (heads / kv_heads) */
+    int32_t  kv_heads;
+    int32_t  head_dim;        /* 128 */
+    int32_t  dtype;           /* enum Qw3Dtype */
+    float    scale;           /* of the scores, above 0; 0: 1 / sqrt(128) */
+    void*    d_out;           /* [q_rows][heads][128] */
+} Qw3AttnPackedArgs;
+
+/* Causal attention of packed sequences (attentionKernel, Inference.cu:182-266, intended math; the reference has one sequence and as
+ * many KV heads as heads).  The queries of a sequence are its last rows: row i of its nq sees its keys 0 .. nk - nq + i, so that a prompt whose
+ * beginning is in the cache attends to all of it; a row that sees no key is zeros.  Rows of d_out that belong to no sequence are left as
+ * they were, and a sequence whose rows are not inside the buffers is left out (QW3_ERR_RANGE from qw3_ws_check).  Nothing that a row does not
+ * see reaches it, Inf and NaN included.  Scores and sums are fp32, probabilities are rounded to the rows' type. */
+int qw3_attn_packed(const Qw3AttnPackedArgs* args, qw3_ws_t ws, void* stream);
+
 /* Embedding column gather straight from the packed [hidden][vocab] matrix (gather lambda,
  * Inference.cu:1310-1315).  Token from *d_token when it is not NULL, else `token`. */
 int qw3_embed_gather_w4(const void* d_packed, const void* d_scale, const void* d_zp, int64_t n_groups_alloc,

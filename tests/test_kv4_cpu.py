@@ -11,7 +11,8 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PTR = 4096   # an address that is never read: every call below is refused before
 
 
-@pytest.mark.parametrize("struct,cls", [("Qw3Kv4Pool", "Kv4Pool"), ("Qw3PageArgs", "PageArgs"), ("Qw3Kv4AppendArgs", "Kv4AppendArgs"), ("Qw3AttnKv4Args", "AttnKv4Args")])
+@pytest.mark.parametrize("struct,cls", [("Qw3Kv4Pool", "Kv4Pool"), ("Qw3PageArgs", "PageArgs"), ("Qw3Kv4AppendArgs", "Kv4AppendArgs"), ("Qw3AttnKv4Args", "AttnKv4Args"),
+                                        ("Qw3AttnPackedArgs", "AttnPackedArgs")])
 def test_argument_blocks_match_the_header(pkg, struct, cls):
     header = open(os.path.join(ROOT, "include", "qw3_cabi.h")).read()
     body = header[header.index("typedef struct %s {" % struct):header.index("} %s;" % struct)]
@@ -107,3 +108,35 @@ def test_python_checks_name_what_is_wrong(ops):
                  (lens, lens, 16, table[:2], lens, one, 4), (lens, lens, 16, table, lens, one, 4)):
         with pytest.raises(ValueError):
             ops.page_slots(*args, _Ws())
+
+
+def _packed(cabi, **kw):
+    a = cabi.AttnPackedArgs(PTR, 512, PTR, 256, PTR, 256, 10, 10, PTR, PTR, 1, 4, 2, 128, 0, 0.0, PTR)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("bad", [dict(d_q=None), dict(d_k=None), dict(d_v=None), dict(d_out=None), dict(d_cu_q=None), dict(d_cu_k=None), dict(d_q=PTR + 8), dict(d_v=PTR + 2),
+                                 dict(d_out=PTR + 4), dict(q_stride=504), dict(q_stride=516), dict(k_stride=128), dict(v_stride=260), dict(q_rows=-1), dict(k_rows=2 ** 31),
+                                 dict(n_seq=-1), dict(heads=5), dict(heads=0), dict(kv_heads=0), dict(head_dim=64), dict(dtype=3), dict(scale=-1.0), dict(scale=float("nan")),
+                                 dict(scale=float("inf"))])
+def test_packed_attention_refuses(pkg, bad):
+    cabi = pkg.cabi
+    assert cabi.lib().qw3_attn_packed(C.byref(_packed(cabi, **bad)), PTR, None) == cabi.QW3_ERR_ARG
+    assert b"qw3_attn_packed" in cabi.lib().qw3_last_error()
+    assert cabi.lib().qw3_attn_packed(None, PTR, None) == cabi.QW3_ERR_ARG
+    assert cabi.lib().qw3_attn_packed(C.byref(_packed(cabi)), None, None) == cabi.QW3_ERR_ARG
+    assert cabi.lib().qw3_attn_packed(C.byref(_packed(cabi, n_seq=0)), PTR, None) == cabi.QW3_OK
+
+
+def test_packed_attention_python_checks(ops):
+    q, k, cu = torch.zeros(5, 4, 128).half(), torch.zeros(7, 2, 128).half(), torch.zeros(3, dtype=torch.int32)
+    for args in ((q.float(), k.float(), k.float(), cu, cu), (q, k.bfloat16(), k, cu, cu), (q, k, k[:6], cu, cu), (q, k, k[:, :1], cu, cu), (q, k, k, cu[:2], cu),
+                 (q, k, k, cu.long(), cu), (q, k, k, cu[:0], cu), (q[..., :64], k, k, cu, cu), (q, k, k, cu, cu)):   # the last: not on a GPU
+        with pytest.raises(ValueError):
+            ops.attn_packed(*args, _Ws())
+    with pytest.raises(ValueError):
+        ops.attn_packed(q, k, k, cu, cu, _Ws(), scale=-1.0)
+    with pytest.raises(ValueError):
+        ops.attn_packed(q, k, k, cu, cu, _Ws(), out=torch.zeros(5, 4, 128))
