@@ -5,10 +5,10 @@
 // The codes go into the tensor cores as they are: a nibble in the low bits of a half is the subnormal code * 2^-24 (or * 2^-20 four bits
 // further up), so a mask is all the unpacking there is, products are exact, and scales are applied to fp32 sums.  V's scale is folded into the
 // exponent: u_j = score_j + log2(sv_j), P_j = 2^(u_j - max u + 8) enters the second product as fp16 (the largest is between 2^8 and 2^15, so
-// the 11 bits reach 22 powers of two below it, whatever the scales are), and the sums of p and p mv take P_j / sv_j in fp32.
-// The two terms of the output are far larger than their sum (codes are not centred), and the tensor cores cut off what an accumulator
-// cannot hold: after four chunks at most the products go to fp32 sums in shared memory, rounded to nearest (a list of 40 K
-// tokens: error 2.0e-3 of the output's size without that, 2.1e-4 with it).
+// the 11 bits reach 22 powers of two below it, whatever the scales are), and the sums of p and p (mv + 8 sv) take P_j / sv_j in fp32.
+// The sum of P code is far larger than that of P (code - 8), and the tensor cores cut off what an accumulator cannot hold, which
+// shortens it: one more product sums P * 8 the same way, and the difference goes to fp32 sums in shared memory after eight chunks
+// at most (a list of 40 K tokens: error KD_ERR of the output's size, 2.0e-3 without either).
 //
 // A warp works on 32 tokens at a time, two tiles of 16 that bulk copies bring into its own ring of two: S^T = K Q^T (16 tokens x 8 heads
 // of the group), then O^T += V^T P^T, with mma.sync m16n8k16.  At 136 bytes a token and KV head the kernel is bound by HBM; one m16n8k16 a
@@ -22,7 +22,7 @@ namespace qw3 {
 
 constexpr int KD_WARPS = 4, KD_THREADS = 32 * KD_WARPS, KD_STAGES = 2, KD_CTAS = 4;   // CTAs an SM
 constexpr int KD_CHUNK = 32, KD_STAGE_BYTES = 2 * KV4_TILE_BYTES;
-constexpr int KD_FLUSH = 4;            // chunks whose products are summed in an accumulator
+constexpr int KD_FLUSH = 8;            // chunks whose products are summed in an accumulator
 constexpr int KD_MIN_CHUNKS = 8;       // chunks a CTA takes at least
 constexpr int KD_PART = 1024 + 32;     // floats of a partial state: outputs, then (maximum, sum of p, sum of p mv) of eight heads
 constexpr int KD_MAX_GRID = 1024;
@@ -31,9 +31,11 @@ static_assert(2 * (size_t)KD_MAX_GRID * KD_PART <= WS_PARTIALS && KD_MAX_GRID <=
 struct KdSmem {
     uint8_t ring[KD_WARPS][KD_STAGES][KD_STAGE_BYTES];
     float4 o[KD_WARPS][8][32];        // sums of a warp, in the order of its fragments
+    float4 token[KD_WARPS][KD_CHUNK];  // of the chunk's tokens: scale of K * 2^24, minimum of K, log2 of V's scale, 1 / V's scale
+    float mid[KD_WARPS][KD_CHUNK];     // and V's minimum + 8 * scale
     float stat[KD_WARPS][8][3];
     uint64_t bar[KD_WARPS][KD_STAGES];
-    int valid[KD_WARPS][KD_STAGES];   // tokens of the two tiles, 16 bits each
+    int valid[KD_WARPS][KD_STAGES][2]; // tokens of the two tiles
     int last;
 };
 
@@ -60,6 +62,14 @@ __device__ __forceinline__ uint32_t kd_transpose(uint32_t x) {
 __device__ __forceinline__ void kd_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
+}
+
+// D = A * B
+__device__ __forceinline__ void kd_mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 struct KdParams {
@@ -152,52 +162,59 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
         } while (q.n == 0);
     };
 
-    // copies: chunk number `k` of this warp is number warp + 4 k of the CTA; the page of the next one is looked up one ahead
+    // copies: chunk number k of this warp is number warp + 4 k of the CTA.  Lane i looks up tile i % 2 of the i / 2-th of sixteen chunks, once
+    // in sixteen, and issues its copy when its turn comes.
+    const int my_chunks = (n_mine - warp + KD_WARPS - 1) / KD_WARPS;
     KdPlace ahead = place;
-    int ahead_at = 0, issued = 0;       // of the CTA's chunks, of this warp's
-    int tokens = 0;                     // lanes 0 and 1: of the tile to be copied
+    int ahead_at = 0, issued = 0;   // `ahead` is the place of the CTA's chunk number ahead_at; chunks issued
+    int tokens = 0;                 // of this lane's tile
     const uint8_t* src = nullptr;
-    const auto look_up = [&](int at) {
-        if (at >= n_mine) return;
-        int left = at - ahead_at;
-        ahead_at = at;
-        while (left >= ahead.n - ahead.c) {
-            left -= ahead.n - ahead.c;
-            ahead.c = 0;
-            next_request(ahead);
-        }
-        ahead.c += left;
-        if (lane < 2) {
-            const int tile = 2 * ahead.c + lane;
-            const int n = length(ahead.b) - 16 * tile;
-            tokens = n < 0 ? 0 : n < 16 ? n : 16;
-            if (tokens > 0) {
-                const int in = tile / tiles_page, page = p.a.d_block_table[ahead.b * p.a.table_stride + in];
+    const auto look_up = [&]() {
+        const int k = issued + lane / 2, at = warp + KD_WARPS * k;
+        tokens = 0;
+        KdPlace q = ahead;
+        if (k < my_chunks) {
+            int left = at - ahead_at;
+            while (left >= q.n - q.c) {
+                left -= q.n - q.c;
+                q.c = 0;
+                next_request(q);
+            }
+            q.c += left;
+            const int tile = 2 * q.c + (lane & 1), n = length(q.b) - 16 * tile;
+            if (n > 0) {
+                const int in = tile / tiles_page, page = p.a.d_block_table[q.b * p.a.table_stride + in];
                 if (page < 0 || page >= p.pool.n_pages) {
                     kv4_error(p.err, KV4_ERR_DECODE_PAGE);
-                    tokens = 0;
                 } else {
+                    tokens = min(n, 16);
                     src = static_cast<const uint8_t*>(p.pool.d_pages) + page * p.pool.page_stride +
-                          ((long long)(ahead.ht / p.q_tiles) * tiles_page + (tile - in * tiles_page)) * KV4_TILE_BYTES;
+                          ((long long)(q.ht / p.q_tiles) * tiles_page + (tile - in * tiles_page)) * KV4_TILE_BYTES;
                 }
             }
         }
+        __syncwarp();
+        // the next sixteen are found from the last of these (used only where there is one)
+        ahead.ht = __shfl_sync(0xffffffffu, q.ht, 31);
+        ahead.b = __shfl_sync(0xffffffffu, q.b, 31);
+        ahead.c = __shfl_sync(0xffffffffu, q.c, 31);
+        ahead.n = __shfl_sync(0xffffffffu, q.n, 31);
+        ahead_at = warp + KD_WARPS * (issued + 15);
     };
-    const auto issue = [&]() {   // the chunk that was looked up; then looks up the one after
+    const auto issue = [&]() {
+        if ((issued & 15) == 0) look_up();
         const int s = issued % KD_STAGES;
         const uint32_t bar = smem_u32(&sm.bar[warp][s]);
-        const int n0 = __shfl_sync(0xffffffffu, tokens, 0), n1 = __shfl_sync(0xffffffffu, tokens, 1);
-        if (lane == 0) {
-            sm.valid[warp][s] = n0 | n1 << 16;
-            mbar_expect_tx(bar, (uint32_t)KV4_TILE_BYTES * ((n0 > 0) + (n1 > 0)));
+        const bool turn = lane / 2 == (issued & 15), copies = turn && tokens > 0;
+        const int n = __popc(__ballot_sync(0xffffffffu, copies));
+        if (turn) {
+            sm.valid[warp][s][lane & 1] = tokens;
+            if ((lane & 1) == 0) mbar_expect_tx(bar, (uint32_t)KV4_TILE_BYTES * n);
         }
         __syncwarp();
-        if (lane < 2 && tokens > 0) kd_copy(smem_u32(&sm.ring[warp][s][lane * KV4_TILE_BYTES]), src, KV4_TILE_BYTES, bar);
+        if (copies) kd_copy(smem_u32(&sm.ring[warp][s][(lane & 1) * KV4_TILE_BYTES]), src, KV4_TILE_BYTES, bar);
         ++issued;
-        look_up(warp + KD_WARPS * issued);
     };
-    const int my_chunks = (n_mine - warp + KD_WARPS - 1) / KD_WARPS;
-    look_up(warp);
     for (int s = 0; s < KD_STAGES && issued < my_chunks; ++s) issue();
 
     const int row0 = g ^ ((g >> 1) & 1);   // token of a tile that index g of a fragment stands for (and + 8): neighbours in t are of either parity,
@@ -264,76 +281,88 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
         }
 
         int unflushed = 0;   // chunks in the accumulators
-        const auto flush = [&](float (&o)[8][4], float r0, float r1) {   // (sums + accumulators) times a factor a head
+        float o[8][4], eight[4];   // dims 16 g + 4 (i / 2) + i % 2 and + 2, heads 2t and 2t + 1: sums of P code, and of P * 8; odd i: 16 times that
+        const auto clear = [&] {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+            eight[0] = eight[1] = eight[2] = eight[3] = 0.0f;
+            unflushed = 0;
+        };
+        const auto flush = [&](float r0, float r1) {   // (sums + accumulators) times a factor a head
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 float4* const at = &sm.o[warp][i][lane];
                 const float4 a = *at;
-                *at = make_float4((a.x + o[i][0]) * r0, (a.y + o[i][1]) * r1, (a.z + o[i][2]) * r0, (a.w + o[i][3]) * r1);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+                const float up = i & 1 ? -16.0f : -1.0f, e0 = eight[0], e1 = eight[1];   // all rows of the product are the same
+                *at = make_float4((a.x + fmaf(up, e0, o[i][0])) * r0, (a.y + fmaf(up, e1, o[i][1])) * r1, (a.z + fmaf(up, e0, o[i][2])) * r0,
+                                  (a.w + fmaf(up, e1, o[i][3])) * r1);
             }
-            unflushed = 0;
+            clear();
         };
 #pragma unroll
         for (int i = 0; i < 8; ++i) sm.o[warp][i][lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float o[8][4], mu0 = -INFINITY, mu1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, m0 = 0.0f, m1 = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+        clear();
+        float mu0 = -INFINITY, mu1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, m0 = 0.0f, m1 = 0.0f;
 
         for (; warp + KD_WARPS * used < part_end; ++used) {
             const int s = used % KD_STAGES;
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.bar[warp][s]), (uint32_t)(used / KD_STAGES) & 1u));
             if (!ok) continue;   // reported below
-            const int both = sm.valid[warp][s];
             const uint8_t* const stage = sm.ring[warp][s];
-            float u[2][4];       // score, then u: tokens row0, row0 + 8 x heads 2t, 2t + 1
-            float inv[2][2], mv[2][2];
+            {   // lane i: what belongs to token i of the chunk; behind the last one nothing is left but codes, which are finite, times zero
+                const uint8_t* const tile = stage + (lane >> 4) * KV4_TILE_BYTES + 4 * (lane & 15);
+                const float2 ks = R::unpack(*reinterpret_cast<const uint32_t*>(tile + KV4_KP)), vs = R::unpack(*reinterpret_cast<const uint32_t*>(tile + KV4_VP));
+                const bool in = (lane & 15) < sm.valid[warp][s][lane >> 4];
+                sm.token[warp][lane] = in ? make_float4(ks.x * 16777216.0f, ks.y, kd_lg2(vs.x), kd_rcp(vs.x)) : make_float4(0.0f, 0.0f, -INFINITY, 0.0f);
+                sm.mid[warp][lane] = in ? fmaf(8.0f, vs.x, vs.y) : 0.0f;
+            }
+            __syncwarp();
+            float u[2][4];       // tokens row0, row0 + 8 x heads 2t, 2t + 1
+            float inv[2][2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int n = both >> (16 * e) & 0xffff;
                 const uint8_t* const tile = stage + e * KV4_TILE_BYTES;
                 const uint4 ka = *reinterpret_cast<const uint4*>(tile + row0 * 64 + 16 * t), kb = *reinterpret_cast<const uint4*>(tile + row0 * 64 + 512 + 16 * t);
                 const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
-                float lo[4] = {0.0f, 0.0f, 0.0f, 0.0f}, hi[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float lo[4], hi[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t a8 = wa[j] >> 8, b8 = wb[j] >> 8;
-                    mma_16816(lo, wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu, qf[j][0], qf[j][1]);
-                    mma_16816(hi, wa[j] & 0x00f000f0u, wb[j] & 0x00f000f0u, a8 & 0x00f000f0u, b8 & 0x00f000f0u, qf[j][2], qf[j][3]);
+                    if (j == 0) {
+                        kd_mma_first(lo, wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu, qf[j][0], qf[j][1]);
+                        kd_mma_first(hi, wa[j] & 0x00f000f0u, wb[j] & 0x00f000f0u, a8 & 0x00f000f0u, b8 & 0x00f000f0u, qf[j][2], qf[j][3]);
+                    } else {
+                        mma_16816(lo, wa[j] & 0x000f000fu, wb[j] & 0x000f000fu, a8 & 0x000f000fu, b8 & 0x000f000fu, qf[j][0], qf[j][1]);
+                        mma_16816(hi, wa[j] & 0x00f000f0u, wb[j] & 0x00f000f0u, a8 & 0x00f000f0u, b8 & 0x00f000f0u, qf[j][2], qf[j][3]);
+                    }
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {   // token row0 + 8 h
-                    const bool in = row0 + 8 * h < n;
-                    const uint32_t kp = *reinterpret_cast<const uint32_t*>(tile + KV4_KP + 4 * row0 + 32 * h);
-                    const uint32_t vp = *reinterpret_cast<const uint32_t*>(tile + KV4_VP + 4 * row0 + 32 * h);
-                    const float2 ks = R::unpack(kp), vs = R::unpack(vp);
-                    const float sk = ks.x * 16777216.0f, lg = kd_lg2(vs.x);
-                    const float s0 = fmaf(sk, fmaf(hi[2 * h], 0.0625f, lo[2 * h]), ks.y * qs0), s1 = fmaf(sk, fmaf(hi[2 * h + 1], 0.0625f, lo[2 * h + 1]), ks.y * qs1);
-                    u[e][2 * h] = in ? fmaf(f0, s0, lg) : -INFINITY;
-                    u[e][2 * h + 1] = in ? fmaf(f1, s1, lg) : -INFINITY;
-                    inv[e][h] = in ? kd_rcp(vs.x) : 0.0f;
-                    mv[e][h] = in ? vs.y : 0.0f;
+                    const float4 k = sm.token[warp][16 * e + row0 + 8 * h];
+                    const float s0 = fmaf(k.x, fmaf(hi[2 * h], 0.0625f, lo[2 * h]), k.y * qs0), s1 = fmaf(k.x, fmaf(hi[2 * h + 1], 0.0625f, lo[2 * h + 1]), k.y * qs1);
+                    u[e][2 * h] = fmaf(f0, s0, k.z);
+                    u[e][2 * h + 1] = fmaf(f1, s1, k.z);
+                    inv[e][h] = k.w;
                 }
             }
             float x0m = fmaxf(fmaxf(u[0][0], u[0][2]), fmaxf(u[1][0], u[1][2])), x1m = fmaxf(fmaxf(u[0][1], u[0][3]), fmaxf(u[1][1], u[1][3]));
-#pragma unroll
-            for (int d = 4; d < 32; d *= 2) {
-                x0m = fmaxf(x0m, __shfl_xor_sync(0xffffffffu, x0m, d));
-                x1m = fmaxf(x1m, __shfl_xor_sync(0xffffffffu, x1m, d));
-            }
             if (__any_sync(0xffffffffu, x0m > mu0 + 7.0f || x1m > mu1 + 7.0f)) {   // rare after the first chunks
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) {
+                    x0m = fmaxf(x0m, __shfl_xor_sync(0xffffffffu, x0m, d));
+                    x1m = fmaxf(x1m, __shfl_xor_sync(0xffffffffu, x1m, d));
+                }
                 const float n0 = fmaxf(mu0, x0m), n1 = fmaxf(mu1, x1m);
                 const float r0 = mu0 == -INFINITY ? 0.0f : kd_ex2(mu0 - n0), r1 = mu1 == -INFINITY ? 0.0f : kd_ex2(mu1 - n1);
                 mu0 = n0;
                 mu1 = n1;
                 l0 *= r0; m0 *= r0;
                 l1 *= r1; m1 *= r1;
-                flush(o, r0, r1);
+                flush(r0, r1);
             }
-            if (unflushed == KD_FLUSH) flush(o, 1.0f, 1.0f);
+            if (unflushed == KD_FLUSH) flush(1.0f, 1.0f);
             ++unflushed;
             const float z0 = mu0 == -INFINITY ? 0.0f : mu0 - 8.0f, z1 = mu1 == -INFINITY ? 0.0f : mu1 - 8.0f;
 #pragma unroll
@@ -342,21 +371,19 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
                 uint32_t pf[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
+                    const float mid = sm.mid[warp][16 * e + row0 + 8 * h];
                     const float p0 = kd_ex2(u[e][2 * h] - z0), p1 = kd_ex2(u[e][2 * h + 1] - z1);
-                    const uint32_t pp = RowType<__half>::pack(p0, p1);
-                    // all sums take the rounded P, so that its error meets the value and not its far larger terms; below fp16's normal
-                    // numbers, where the products no longer matter but p itself may (a tiny scale), the unrounded one
-                    const float2 pr = RowType<__half>::unpack(pp);
-                    const float w0 = (p0 >= 6.103515625e-5f ? pr.x : p0) * inv[e][h], w1 = (p1 >= 6.103515625e-5f ? pr.y : p1) * inv[e][h];
+                    const float w0 = p0 * inv[e][h], w1 = p1 * inv[e][h];
                     l0 += w0;
                     l1 += w1;
-                    m0 = fmaf(w0, mv[e][h], m0);
-                    m1 = fmaf(w1, mv[e][h], m1);
-                    pf[h] = kd_transpose(pp);
+                    m0 = fmaf(w0, mid, m0);
+                    m1 = fmaf(w1, mid, m1);
+                    pf[h] = kd_transpose(RowType<__half>::pack(p0, p1));
                 }
                 const int ra = 2 * t + (t & 1), rb = 2 * t + (~t & 1);   // tokens of indexes 2t and 2t + 1
                 const uint2 a0 = *reinterpret_cast<const uint2*>(tile + ra * 64 + 8 * g), b0 = *reinterpret_cast<const uint2*>(tile + rb * 64 + 8 * g);
                 const uint2 a1 = *reinterpret_cast<const uint2*>(tile + ra * 64 + 512 + 8 * g), b1 = *reinterpret_cast<const uint2*>(tile + rb * 64 + 512 + 8 * g);
+                mma_16816(eight, 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[0], pf[1]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {   // dims 16 g + 4 i .. + 3
                     const int sel = i & 1 ? 0x7632 : 0x5410;
@@ -385,7 +412,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
             st[0] = mu0; st[1] = l0; st[2] = m0;
             st[3] = mu1; st[4] = l1; st[5] = m1;
         }
-        flush(o, 1.0f, 1.0f);
+        flush(1.0f, 1.0f);
         __syncthreads();
         // thread (i, lane): dims 16 g + 4 i .. + 3 of heads 2t and 2t + 1
         const int i = warp;
