@@ -17,13 +17,20 @@
 // warps of a CTA take its chunks in turn and join their states in shared memory, and pairs that are cut by the border of a CTA are joined
 // from the workspace by the last CTA to arrive, in order of the parts: results do not depend on timing.
 #include "kv4.cuh"
+#include "tc05.cuh"
 
 namespace qw3 {
 
-constexpr int KD_WARPS = 4, KD_THREADS = 32 * KD_WARPS, KD_STAGES = 2, KD_CTAS = 4;   // CTAs an SM
+#ifndef ST_
+#define ST_ 2
+#define CT_ 3
+#endif
+constexpr int KD_WARPS = 4, KD_THREADS = 32 * KD_WARPS, KD_STAGES = ST_, KD_CTAS = CT_;   // CTAs an SM
 constexpr int KD_CHUNK = 32, KD_STAGE_BYTES = 2 * KV4_TILE_BYTES;
 constexpr int KD_FLUSH = 8;            // chunks whose products are summed in an accumulator
 constexpr int KD_MIN_CHUNKS = 8;       // chunks a CTA takes at least
+constexpr int KD_WHOLE = 32;           // pairs of so many chunks are not cut: joining two parts costs some 4 us, eight chunks a warp 3
+constexpr int KD_PAIR = 6;             // what a pair costs a CTA beside its chunks (q, joining the warps' states), in chunks
 constexpr int KD_PART = 1024 + 32;     // floats of a partial state: outputs, then (maximum, sum of p, sum of p mv) of eight heads
 constexpr int KD_MAX_GRID = 1024;
 static_assert(2 * (size_t)KD_MAX_GRID * KD_PART <= WS_PARTIALS && KD_MAX_GRID <= WS_MAX_TILES, "workspace");
@@ -35,7 +42,7 @@ struct KdSmem {
     float mid[KD_WARPS][KD_CHUNK];     // and V's minimum + 8 * scale
     float stat[KD_WARPS][8][3];
     uint64_t bar[KD_WARPS][KD_STAGES];
-    int valid[KD_WARPS][KD_STAGES][2]; // tokens of the two tiles
+    int valid[KD_WARPS][KD_STAGES];    // tokens of the two tiles, 16 bits each
     int last;
 };
 
@@ -107,29 +114,38 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
         const int n = p.a.d_kv_len[b];
         return n < 0 ? 0 : (long long)n > p.most_tokens ? (int)p.most_tokens : n;
     };
-    // requests without tokens: rows of zeros
-    for (int b = blockIdx.x; b < B; b += gridDim.x) {
-        const int n = p.a.d_kv_len[b];
-        if (tid == 0 && (n < 0 || (long long)n > p.most_tokens)) kv4_error(p.err, KV4_ERR_DECODE_LEN);
-        if (length(b) == 0)
-            for (int i = tid; i < p.a.heads * 16; i += KD_THREADS) reinterpret_cast<uint4*>(static_cast<T*>(p.a.d_out) + (size_t)b * p.a.heads * 128)[i] = make_uint4(0, 0, 0, 0);
-    }
-    // this CTA's part of the list
+    // this CTA's part of the list.  Places are counted twice: in chunks, and, to give all CTAs the same work, with KD_PAIR more for each pair
     long long per_head = 0;
-    for (int b = lane; b < B; b += 32) per_head += (length(b) + KD_CHUNK - 1) / KD_CHUNK;
+    int busy = 0;   // requests that have tokens
+    for (int b = lane; b < B; b += 32) {
+        const int n = (length(b) + KD_CHUNK - 1) / KD_CHUNK;
+        per_head += n;
+        busy += n > 0;
+    }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) per_head += __shfl_xor_sync(0xffffffffu, per_head, d);
-    const long long total = per_head * p.heads_t;
-    const long long wanted = total / KD_MIN_CHUNKS;
-    const int grid = (int)(wanted < 1 ? 1 : wanted < (long long)gridDim.x ? wanted : (long long)gridDim.x);
-    if (total == 0 || (int)blockIdx.x >= grid) return;
-    const long long x0 = total * blockIdx.x / grid, x1 = total * (blockIdx.x + 1) / grid;
-    const int n_mine = (int)(x1 - x0);   // a list of 2^31 chunks would be 10 TB
-    KdPlace place;
-    {
-        place.ht = (int)(x0 / per_head);
-        long long y = x0 - place.ht * per_head;
-        for (int b0 = 0;; b0 += 32) {
+    busy = __reduce_add_sync(0xffffffffu, busy);
+    const long long chunks = per_head * p.heads_t, per_head_w = per_head + (long long)KD_PAIR * busy, total = per_head_w * p.heads_t;
+    // so many CTAs that a part is worth starting one, and that joining the parts of a pair does not take longer than they do
+    const float balanced = sqrtf(2.0f * (float)chunks * (float)((long long)busy * p.heads_t));
+    const long long wanted = min((long long)balanced, chunks / KD_MIN_CHUNKS);
+    const int grid = (int)max(1ll, min(wanted, (long long)gridDim.x));
+    long long x[2] = {0, 0};        // first chunk and the one behind the last
+    KdPlace place = {0, 0, 0, 0};   // of the first
+    if (chunks > 0 && (int)blockIdx.x < grid) {
+        long long y[2];
+        int ht[2];
+        bool found[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const long long w = total * (blockIdx.x + e) / grid;
+            ht[e] = (int)(w / per_head_w);
+            y[e] = w - ht[e] * per_head_w;
+            found[e] = w == total;
+            x[e] = found[e] ? chunks : ht[e] * per_head;
+        }
+        int before = 0;             // chunks of the requests before the thirty-two
+        for (int b0 = 0; b0 < B && !(found[0] && found[1]); b0 += 32) {
             const int n = b0 + lane < B ? (length(b0 + lane) + KD_CHUNK - 1) / KD_CHUNK : 0;
             int s = n;
 #pragma unroll
@@ -137,17 +153,26 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
                 const int a = __shfl_up_sync(0xffffffffu, s, d);
                 if (lane >= d) s += a;
             }
-            const int all = __shfl_sync(0xffffffffu, s, 31);
-            if (y < all) {
-                const int l = __ffs(__ballot_sync(0xffffffffu, y < s)) - 1;
-                place.b = b0 + l;
-                place.n = __shfl_sync(0xffffffffu, n, l);
-                place.c = (int)y - __shfl_sync(0xffffffffu, s - n, l);
-                break;
+            const uint32_t any = __ballot_sync(0xffffffffu, n > 0);
+            const int ws = s + KD_PAIR * __popc(any & (0xffffffffu >> (31 - lane))), all = __shfl_sync(0xffffffffu, ws, 31);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (!found[e] && y[e] < all) {
+                    found[e] = true;
+                    const int l = __ffs(__ballot_sync(0xffffffffu, y[e] < ws)) - 1;
+                    const int nl = __shfl_sync(0xffffffffu, n, l), sl = __shfl_sync(0xffffffffu, s, l), wl = __shfl_sync(0xffffffffu, ws, l);
+                    // behind its first KD_PAIR places a pair is cut, a short one is not
+                    const int c = nl <= KD_WHOLE ? 0 : max(0, nl - (wl - (int)y[e]));
+                    x[e] += before + (sl - nl) + c;
+                    if (e == 0) place = {ht[0], b0 + l, c, nl};
+                }
+                y[e] -= all;
             }
-            y -= all;
+            before += __shfl_sync(0xffffffffu, s, 31);
         }
     }
+    const long long x0 = x[0];
+    const int n_mine = (int)(x[1] - x0);   // a list of 2^31 chunks would be 10 TB
     const auto next_request = [&](KdPlace& q) {   // the next one that has chunks
         do {
             if (++q.b == B) {
@@ -162,15 +187,29 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
         } while (q.n == 0);
     };
 
-    // copies: chunk number k of this warp is number warp + 4 k of the CTA.  Lane i looks up tile i % 2 of the i / 2-th of sixteen chunks, once
-    // in sixteen, and issues its copy when its turn comes.
+    const auto rank_of = [&](int b) {   // requests before b that have tokens
+        int r = 0;
+        for (int i = lane; i < b; i += 32) r += length(i) > 0;
+        return __reduce_add_sync(0xffffffffu, r);
+    };
+
+    // copies: chunk number k of this warp is number warp + 4 k of the CTA.  Thirty-two are looked up at once, one a lane.
     const int my_chunks = (n_mine - warp + KD_WARPS - 1) / KD_WARPS;
     KdPlace ahead = place;
     int ahead_at = 0, issued = 0;   // `ahead` is the place of the CTA's chunk number ahead_at; chunks issued
-    int tokens = 0;                 // of this lane's tile
-    const uint8_t* src = nullptr;
+    int tokens = 0;                 // of the lane's chunk, in its two tiles: 16 bits each
+    const uint8_t *src0 = nullptr, *src1 = nullptr;
+    const auto tile_at = [&](const KdPlace& q, int tile) -> const uint8_t* {   // null where the page is outside the pool
+        const int in = tile / tiles_page, page = p.a.d_block_table[q.b * p.a.table_stride + in];
+        if (page < 0 || page >= p.pool.n_pages) {
+            kv4_error(p.err, KV4_ERR_DECODE_PAGE);
+            return nullptr;
+        }
+        return static_cast<const uint8_t*>(p.pool.d_pages) + page * p.pool.page_stride +
+               ((long long)(q.ht / p.q_tiles) * tiles_page + (tile - in * tiles_page)) * KV4_TILE_BYTES;
+    };
     const auto look_up = [&]() {
-        const int k = issued + lane / 2, at = warp + KD_WARPS * k;
+        const int k = issued + lane, at = warp + KD_WARPS * k;
         tokens = 0;
         KdPlace q = ahead;
         if (k < my_chunks) {
@@ -181,41 +220,53 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
                 next_request(q);
             }
             q.c += left;
-            const int tile = 2 * q.c + (lane & 1), n = length(q.b) - 16 * tile;
-            if (n > 0) {
-                const int in = tile / tiles_page, page = p.a.d_block_table[q.b * p.a.table_stride + in];
-                if (page < 0 || page >= p.pool.n_pages) {
-                    kv4_error(p.err, KV4_ERR_DECODE_PAGE);
-                } else {
-                    tokens = min(n, 16);
-                    src = static_cast<const uint8_t*>(p.pool.d_pages) + page * p.pool.page_stride +
-                          ((long long)(q.ht / p.q_tiles) * tiles_page + (tile - in * tiles_page)) * KV4_TILE_BYTES;
-                }
+            const int tile = 2 * q.c, n0 = length(q.b) - 16 * tile, n1 = n0 - 16;
+            if (n0 > 0) {
+                src0 = tile_at(q, tile);
+                if (src0 != nullptr) tokens = min(n0, 16);
+            }
+            if (n1 > 0) {
+                src1 = tile_at(q, tile + 1);
+                if (src1 != nullptr) tokens |= min(n1, 16) << 16;
             }
         }
         __syncwarp();
-        // the next sixteen are found from the last of these (used only where there is one)
+        // the next thirty-two are found from the last of these (used only where there is one)
         ahead.ht = __shfl_sync(0xffffffffu, q.ht, 31);
         ahead.b = __shfl_sync(0xffffffffu, q.b, 31);
         ahead.c = __shfl_sync(0xffffffffu, q.c, 31);
         ahead.n = __shfl_sync(0xffffffffu, q.n, 31);
-        ahead_at = warp + KD_WARPS * (issued + 15);
+        ahead_at = warp + KD_WARPS * (issued + 31);
     };
     const auto issue = [&]() {
-        if ((issued & 15) == 0) look_up();
-        const int s = issued % KD_STAGES;
-        const uint32_t bar = smem_u32(&sm.bar[warp][s]);
-        const bool turn = lane / 2 == (issued & 15), copies = turn && tokens > 0;
-        const int n = __popc(__ballot_sync(0xffffffffu, copies));
-        if (turn) {
-            sm.valid[warp][s][lane & 1] = tokens;
-            if ((lane & 1) == 0) mbar_expect_tx(bar, (uint32_t)KV4_TILE_BYTES * n);
+        const int turn = issued & 31;
+        if (turn == 0) look_up();
+        const int s = issued % KD_STAGES, n = __shfl_sync(0xffffffffu, tokens, turn);
+        const unsigned long long a = __shfl_sync(0xffffffffu, (unsigned long long)src0, turn), b = __shfl_sync(0xffffffffu, (unsigned long long)src1, turn);
+        if (elect_one()) {
+            const uint32_t bar = smem_u32(&sm.bar[warp][s]), to = smem_u32(sm.ring[warp][s]);
+            const bool n0 = (n & 0xffff) != 0, n1 = n >> 16 != 0;
+            sm.valid[warp][s] = n;
+            mbar_expect_tx(bar, (n0 ? KV4_TILE_BYTES : 0) + (n1 ? KV4_TILE_BYTES : 0));
+            if (n0 && n1 && b - a == KV4_TILE_BYTES) {   // of one page
+                kd_copy(to, reinterpret_cast<const void*>(a), 2 * KV4_TILE_BYTES, bar);
+            } else {
+                if (n0) kd_copy(to, reinterpret_cast<const void*>(a), KV4_TILE_BYTES, bar);
+                if (n1) kd_copy(to + KV4_TILE_BYTES, reinterpret_cast<const void*>(b), KV4_TILE_BYTES, bar);
+            }
         }
         __syncwarp();
-        if (copies) kd_copy(smem_u32(&sm.ring[warp][s][(lane & 1) * KV4_TILE_BYTES]), src, KV4_TILE_BYTES, bar);
         ++issued;
     };
     for (int s = 0; s < KD_STAGES && issued < my_chunks; ++s) issue();
+
+    // requests without tokens: rows of zeros
+    for (int b = blockIdx.x; b < B; b += gridDim.x) {
+        const int n = p.a.d_kv_len[b];
+        if (tid == 0 && (n < 0 || (long long)n > p.most_tokens)) kv4_error(p.err, KV4_ERR_DECODE_LEN);
+        if (length(b) == 0)
+            for (int i = tid; i < p.a.heads * 16; i += KD_THREADS) reinterpret_cast<uint4*>(static_cast<T*>(p.a.d_out) + (size_t)b * p.a.heads * 128)[i] = make_uint4(0, 0, 0, 0);
+    }
 
     const int row0 = g ^ ((g >> 1) & 1);   // token of a tile that index g of a fragment stands for (and + 8): neighbours in t are of either parity,
                                            // which halves the bank conflicts of the V rows
@@ -280,7 +331,8 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
             qs1 = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
         }
 
-        int unflushed = 0;   // chunks in the accumulators
+        int unflushed = 0;      // chunks in the accumulators
+        bool flushed = false;   // sm.o holds sums
         float o[8][4], eight[4];   // dims 16 g + 4 (i / 2) + i % 2 and + 2, heads 2t and 2t + 1: sums of P code, and of P * 8; odd i: 16 times that
         const auto clear = [&] {
 #pragma unroll
@@ -288,21 +340,19 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
             eight[0] = eight[1] = eight[2] = eight[3] = 0.0f;
-            unflushed = 0;
         };
         const auto flush = [&](float r0, float r1) {   // (sums + accumulators) times a factor a head
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 float4* const at = &sm.o[warp][i][lane];
-                const float4 a = *at;
+                const float4 a = flushed ? *at : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 const float up = i & 1 ? -16.0f : -1.0f, e0 = eight[0], e1 = eight[1];   // all rows of the product are the same
                 *at = make_float4((a.x + fmaf(up, e0, o[i][0])) * r0, (a.y + fmaf(up, e1, o[i][1])) * r1, (a.z + fmaf(up, e0, o[i][2])) * r0,
                                   (a.w + fmaf(up, e1, o[i][3])) * r1);
             }
-            clear();
+            unflushed = 0;
+            flushed = true;
         };
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sm.o[warp][i][lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         clear();
         float mu0 = -INFINITY, mu1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, m0 = 0.0f, m1 = 0.0f;
 
@@ -314,7 +364,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
             {   // lane i: what belongs to token i of the chunk; behind the last one nothing is left but codes, which are finite, times zero
                 const uint8_t* const tile = stage + (lane >> 4) * KV4_TILE_BYTES + 4 * (lane & 15);
                 const float2 ks = R::unpack(*reinterpret_cast<const uint32_t*>(tile + KV4_KP)), vs = R::unpack(*reinterpret_cast<const uint32_t*>(tile + KV4_VP));
-                const bool in = (lane & 15) < sm.valid[warp][s][lane >> 4];
+                const bool in = (lane & 15) < (sm.valid[warp][s] >> (lane & 16) & 0xffff);
                 sm.token[warp][lane] = in ? make_float4(ks.x * 16777216.0f, ks.y, kd_lg2(vs.x), kd_rcp(vs.x)) : make_float4(0.0f, 0.0f, -INFINITY, 0.0f);
                 sm.mid[warp][lane] = in ? fmaf(8.0f, vs.x, vs.y) : 0.0f;
             }
@@ -360,9 +410,15 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
                 mu1 = n1;
                 l0 *= r0; m0 *= r0;
                 l1 *= r1; m1 *= r1;
-                flush(r0, r1);
+                if (flushed || unflushed > 0) {
+                    flush(r0, r1);
+                    clear();
+                }
             }
-            if (unflushed == KD_FLUSH) flush(1.0f, 1.0f);
+            if (unflushed == KD_FLUSH) {
+                flush(1.0f, 1.0f);
+                clear();
+            }
             ++unflushed;
             const float z0 = mu0 == -INFINITY ? 0.0f : mu0 - 8.0f, z1 = mu1 == -INFINITY ? 0.0f : mu1 - 8.0f;
 #pragma unroll
@@ -442,8 +498,13 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
             accumulate(lo, sm.o[w][2 * i][lane], fa, fb);
             accumulate(hi, sm.o[w][2 * i + 1][lane], fa, fb);
         }
-        const long long start = x0 + done - place.c, end = start + place.n;   // the pair's chunks in the list
-        const int first = owner_of(start, grid, total), parts = owner_of(end - 1, grid, total) - first + 1;
+        int first = 0, parts = 1;   // CTAs that have a part of the pair
+        if (place.n > KD_WHOLE && (place.c > 0 || done + place.n > n_mine)) {
+            // its first chunk in the places that count KD_PAIR for each pair: chunks before it, and the pairs
+            const long long start = x0 + done - place.c + (long long)KD_PAIR * ((long long)place.ht * busy + rank_of(place.b) + 1);
+            first = owner_of(start, grid, total);
+            parts = owner_of(start + place.n - 1, grid, total) - first + 1;
+        }
         bool write = true;
         if (parts > 1) {
             const auto slot = [&](int k) { return p.part + (size_t)(k == 0 ? 2 * first + 1 : 2 * (first + k)) * KD_PART; };
@@ -466,23 +527,64 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
             write = sm.last != 0;
             if (write) {
                 __threadfence();
-                top[0] = top[1] = -INFINITY;
-                l[0] = l[1] = m[0] = m[1] = 0.0f;
+                // maxima and factors of the parts, sixty-four at a time, a head and every sixteenth part a thread
+                float* const scratch = reinterpret_cast<float*>(sm.o);   // [64][8] factors, [16][8] of the threads
+                const int h8 = tid & 7, k8 = tid >> 3;
+                float st[4][3], mx = -INFINITY;
+                const auto load = [&](int k0) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+#pragma unroll
+                        for (int e = 0; e < 3; ++e) {
+                            const int k = k0 + k8 + 16 * u;
+                            st[u][e] = k < parts ? __ldcg(slot(k) + 1024 + 3 * h8 + e) : e == 0 ? -INFINITY : 0.0f;
+                        }
+                };
+                for (int k0 = (parts - 1) / 64 * 64; k0 >= 0; k0 -= 64) {   // the first sixty-four stay in registers
+                    load(k0);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) mx = fmaxf(mx, st[u][0]);
+                }
+                __syncthreads();   // sm.o has been read
+                scratch[512 + tid] = mx;
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < 16; ++k) mx = fmaxf(mx, scratch[512 + 8 * k + h8]);
+                float sl = 0.0f, smv = 0.0f;
                 lo = hi = make_float4(0, 0, 0, 0);
-                for (int k = 0; k < parts; ++k) {
-                    const float* const st = slot(k) + 1024 + 6 * t;
-                    top[0] = fmaxf(top[0], __ldcg(st));
-                    top[1] = fmaxf(top[1], __ldcg(st + 3));
+                for (int k0 = 0; k0 < parts; k0 += 64) {
+                    if (k0 > 0) {
+                        __syncthreads();
+                        load(k0);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {   // a part without tokens adds nothing, one that gave up adds its NaN
+                        const bool none = st[u][0] == -INFINITY;
+                        const float f = none ? 0.0f : kd_ex2(st[u][0] - mx);
+                        scratch[8 * (k8 + 16 * u) + h8] = f;
+                        sl += none ? (st[u][1] != st[u][1] ? st[u][1] : 0.0f) : st[u][1] * f;
+                        smv += none ? 0.0f : st[u][2] * f;
+                    }
+                    __syncthreads();
+#pragma unroll 8
+                    for (int k = k0; k < min(parts, k0 + 64); ++k) {
+                        const float4* const from = reinterpret_cast<const float4*>(slot(k));
+                        const float fa = scratch[8 * (k - k0) + 2 * t], fb = scratch[8 * (k - k0) + 2 * t + 1];
+                        accumulate(lo, __ldcg(from + (2 * i) * 32 + lane), fa, fb);
+                        accumulate(hi, __ldcg(from + (2 * i + 1) * 32 + lane), fa, fb);
+                    }
                 }
-#pragma unroll 4
-                for (int k = 0; k < parts; ++k) {
-                    const float* const from = slot(k);
-                    const float* const st = from + 1024 + 6 * t;
-                    const float4 a = __ldcg(reinterpret_cast<const float4*>(from) + (2 * i) * 32 + lane), b = __ldcg(reinterpret_cast<const float4*>(from) + (2 * i + 1) * 32 + lane);
-                    const float fa = add(0, __ldcg(st), __ldcg(st + 1), __ldcg(st + 2)), fb = add(1, __ldcg(st + 3), __ldcg(st + 4), __ldcg(st + 5));
-                    accumulate(lo, a, fa, fb);
-                    accumulate(hi, b, fa, fb);
-                }
+                scratch[512 + tid] = sl;
+                scratch[640 + tid] = smv;
+                __syncthreads();
+                l[0] = l[1] = m[0] = m[1] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        l[h] += scratch[512 + 8 * k + 2 * t + h];
+                        m[h] += scratch[640 + 8 * k + 2 * t + h];
+                    }
             }
         }
         if (write) {
