@@ -16,16 +16,14 @@
 // The 32-token chunks of all (KV head, request) pairs form one list that is cut into equal parts, one a CTA, whatever the lengths are; the four
 // warps of a CTA take its chunks in turn and join their states in shared memory, and pairs that are cut by the border of a CTA are joined
 // from the workspace by the last CTA to arrive, in order of the parts: results do not depend on timing.
+#include <atomic>
+
 #include "kv4.cuh"
 #include "tc05.cuh"
 
 namespace qw3 {
 
-#ifndef ST_
-#define ST_ 2
-#define CT_ 3
-#endif
-constexpr int KD_WARPS = 4, KD_THREADS = 32 * KD_WARPS, KD_STAGES = ST_, KD_CTAS = CT_;   // CTAs an SM
+constexpr int KD_WARPS = 4, KD_THREADS = 32 * KD_WARPS, KD_STAGES = 2, KD_CTAS = 3;   // CTAs an SM
 constexpr int KD_CHUNK = 32, KD_STAGE_BYTES = 2 * KV4_TILE_BYTES;
 constexpr int KD_FLUSH = 8;            // chunks whose products are summed in an accumulator
 constexpr int KD_MIN_CHUNKS = 8;       // chunks a CTA takes at least
@@ -187,6 +185,15 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
         } while (q.n == 0);
     };
 
+    // q of the eight heads, on its way while the copies are prepared
+    uint4 w[4];
+    const auto load_q = [&] {
+        const int kvh = place.ht / p.q_tiles, q_tile = place.ht - kvh * p.q_tiles, h = 8 * q_tile + g;
+        const uint4* src_q = reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.d_q) + place.b * p.a.q_stride + (size_t)(kvh * p.group + h) * 128 + 32 * t);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = h < p.group ? src_q[j] : make_uint4(0, 0, 0, 0);
+    };
+    if (n_mine > 0) load_q();
     const auto rank_of = [&](int b) {   // requests before b that have tokens
         int r = 0;
         for (int i = lane; i < b; i += 32) r += length(i) > 0;
@@ -281,10 +288,6 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
         uint32_t qf[4][4];   // word j of a row: low nibbles k 0..7, 8..15, high nibbles the same
         float f0, f1, qs0, qs1;
         {
-            uint4 w[4];
-            const uint4* src_q = reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.d_q) + place.b * p.a.q_stride + (size_t)(head0 + g) * 128 + 32 * t);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = g < nq ? src_q[j] : make_uint4(0, 0, 0, 0);
             float sum = 0.0f, big = 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -511,7 +514,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
             float* const mine = slot((int)blockIdx.x - first);
             reinterpret_cast<float4*>(mine)[(2 * i) * 32 + lane] = lo;
             reinterpret_cast<float4*>(mine)[(2 * i + 1) * 32 + lane] = hi;
-            if (i == 0 && g == 0) {
+            if (warp == 0 && g == 0) {
                 float* const st = mine + 1024 + 6 * t;
                 st[0] = top[0]; st[1] = l[0]; st[2] = m[0];
                 st[3] = top[1]; st[4] = l[1]; st[5] = m[1];
@@ -603,6 +606,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
         if (done < n_mine) {
             place.c = 0;
             next_request(place);
+            load_q();
             __syncthreads();   // sm.o and sm.stat are read
         }
     }
@@ -649,7 +653,12 @@ extern "C" int qw3_attn_kv4_decode(const Qw3Kv4Pool* pool, const Qw3AttnKv4Args*
     if (grid > KD_MAX_GRID) grid = KD_MAX_GRID;
     if (most < grid) grid = most < 1.0 ? 1 : (int)most;
     const auto kernel = pool->dtype == QW3_F16 ? attn_kv4_decode_kernel<__half> : attn_kv4_decode_kernel<__nv_bfloat16>;
-    QW3_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(KdSmem)));
+    static std::atomic<bool> attr_set[64];   // per device: the kernels' shared-memory limit is raised once
+    if (w->device >= 64 || !attr_set[w->device].load(std::memory_order_acquire)) {
+        QW3_CUDA(cudaFuncSetAttribute(attn_kv4_decode_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(KdSmem)));
+        QW3_CUDA(cudaFuncSetAttribute(attn_kv4_decode_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(KdSmem)));
+        if (w->device < 64) attr_set[w->device].store(true, std::memory_order_release);
+    }
     QW3_CUDA(kv4_launch(kernel, dim3(grid), dim3(KD_THREADS), sizeof(KdSmem), static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, p));
     return QW3_OK;
 }

@@ -143,35 +143,47 @@ def _want(cond, message):
 
 def _rows128(t, heads, what, device, dtype):
     """Rows of `heads` x 128 values, the heads of a token together: [tokens][heads][128], or [tokens][heads * 128] where heads is given."""
-    _want(t.device == device and t.dtype == dtype, f"{what}: {dtype} on {device} expected")
-    if t.dim() == 3:
-        _want(t.shape[2] == 128 and t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == 128), f"{what}: [tokens][heads][128] expected, the heads of a token together")
-        n = t.shape[1]
+    shape, stride = t.shape, t.stride()
+    if t.dtype != dtype or t.device != device:
+        raise ValueError(f"{what}: {dtype} on {device} expected")
+    if len(shape) == 3:
+        n = shape[1]
+        if shape[2] != 128 or stride[2] != 1 or (n > 1 and stride[1] != 128):
+            raise ValueError(f"{what}: [tokens][heads][128] expected, the heads of a token together")
     else:
-        _want(t.dim() == 2 and t.shape[1] % 128 == 0 and t.stride(1) == 1, f"{what}: [tokens][heads * 128] expected")
-        n = t.shape[1] // 128
-    _want(heads is None or n == heads, f"{what}: {heads} heads expected, not {n}")
-    return n, (t.stride(0) if t.shape[0] > 1 else n * 128)
+        if len(shape) != 2 or shape[1] % 128 or stride[1] != 1:
+            raise ValueError(f"{what}: [tokens][heads * 128] expected")
+        n = shape[1] // 128
+    if heads is not None and n != heads:
+        raise ValueError(f"{what}: {heads} heads expected, not {n}")
+    return n, (stride[0] if shape[0] > 1 else n * 128)
 
 
-def _ints(t, shape, what, device):
-    _want(t.device == device and t.dtype == torch.int32 and t.is_contiguous() and tuple(t.shape) == shape, f"{what}: contiguous int32 {list(shape)} on {device} expected")
+def _ints(t, n, what, device):
+    if t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous int32 [{n}] on {device} expected")
+    return t.data_ptr()
 
 
 def _table(t, rows, device):
-    _want(t.device == device and t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] == rows and t.shape[1] > 0 and (t.shape[1] == 1 or t.stride(1) == 1),
-          f"block_table: int32 [{rows}][blocks] on {device} expected")
-    return t.stride(0) if rows > 1 else t.shape[1]
+    shape = t.shape
+    if t.dtype != torch.int32 or t.device != device or len(shape) != 2 or shape[0] != rows or shape[1] == 0 or (shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"block_table: int32 [{rows}][blocks] on {device} expected")
+    return t.stride(0) if rows > 1 else shape[1]
 
 
 def _on(device, name, *args):
     """Calls entry point `name` on the device's current stream."""
-    _want(device.type == "cuda", f"{name}: CUDA tensors expected")
-    if device.index == torch.cuda.current_device():
-        cabi.check(getattr(cabi.lib(), name)(*args, _stream()), name)
+    if device.type != "cuda":
+        raise ValueError(f"{name}: CUDA tensors expected")
+    fn, stream = getattr(cabi.lib(), name), torch._C._cuda_getCurrentRawStream(device.index)
+    if device.index == torch._C._cuda_getDevice():
+        status = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            cabi.check(getattr(cabi.lib(), name)(*args, _stream()), name)
+            status = fn(*args, stream)
+    if status:
+        cabi.check(status, name)
 
 
 class Kv4Cache:
@@ -185,7 +197,9 @@ class Kv4Cache:
         _want(pages.shape[1] >= kv_heads * page_size * 136, f"pages: {kv_heads * page_size * 136} bytes a page expected")
         self.pages, self.page_size, self.kv_heads, self.dtype = pages, page_size, kv_heads, dtype
         stride = pages.stride(0) if pages.shape[0] > 1 else kv_heads * page_size * 136
+        self.device = pages.device
         self.pool = cabi.Kv4Pool(pages.data_ptr(), pages.shape[0], stride, page_size, kv_heads, 128, _DTYPES[dtype])
+        self.ref = C.byref(self.pool)
 
     @classmethod
     def alloc(cls, n_pages, page_size, kv_heads, dtype=torch.float16, device="cuda"):
@@ -196,24 +210,20 @@ def page_slots(ctx_len, new_len, page_size, block_table, free_pages, n_free, max
     """Pages for new_len[b] more tokens of each request, taken from the top of the stack free_pages[: n_free].  Updates block_table; returns
     (cu, pos, slots, kv_len, n_free_out): new tokens before each request, position and slot of each new token (0 and -1 behind the last),
     the new lengths and what is left of the stack.  kv_len=ctx_len and n_free_out=n_free update those in place."""
-    dev = ctx_len.device
-    n = ctx_len.numel()
-    _ints(ctx_len, (n,), "ctx_len", dev)
-    _ints(new_len, (n,), "new_len", dev)
+    dev, n = ctx_len.device, ctx_len.shape[0]
+    d_ctx = _ints(ctx_len, n, "ctx_len", dev)
+    d_new = _ints(new_len, n, "new_len", dev)
     _want(free_pages.dim() == 1, "free_pages: one dimension expected")
-    _ints(free_pages, (free_pages.numel(),), "free_pages", dev)
-    _ints(n_free, (1,), "n_free", dev)
+    d_free = _ints(free_pages, free_pages.shape[0], "free_pages", dev)
+    d_n_free = _ints(n_free, 1, "n_free", dev)
     stride = _table(block_table, n, dev)
     _want(0 <= max_tokens < 2 ** 31, "max_tokens: out of range")
-    out = torch.empty(n + 1 + 2 * max_tokens, dtype=torch.int32, device=dev)
-    cu, pos, slots = out[:n + 1], out[n + 1:n + 1 + max_tokens], out[n + 1 + max_tokens:]
-    kv_len = torch.empty_like(ctx_len) if kv_len is None else kv_len
-    n_free_out = torch.empty_like(n_free) if n_free_out is None else n_free_out
-    _ints(kv_len, (n,), "kv_len", dev)
-    _ints(n_free_out, (1,), "n_free_out", dev)
-    a = cabi.PageArgs(ctx_len.data_ptr(), new_len.data_ptr(), n, page_size, block_table.data_ptr(), stride, block_table.shape[1], free_pages.numel(),
-                      free_pages.data_ptr(), n_free.data_ptr(), n_free_out.data_ptr(), cu.data_ptr(), kv_len.data_ptr(), pos.data_ptr(), slots.data_ptr(),
-                      max_tokens)
+    cu, pos, slots, own_len, own_free = torch.empty(2 * n + 2 + 2 * max_tokens, dtype=torch.int32, device=dev).split_with_sizes(
+        (n + 1, max_tokens, max_tokens, n, 1))
+    kv_len = own_len if kv_len is None else kv_len
+    n_free_out = own_free if n_free_out is None else n_free_out
+    a = cabi.PageArgs(d_ctx, d_new, n, page_size, block_table.data_ptr(), stride, block_table.shape[1], free_pages.shape[0], d_free, d_n_free,
+                      _ints(n_free_out, 1, "n_free_out", dev), cu.data_ptr(), _ints(kv_len, n, "kv_len", dev), pos.data_ptr(), slots.data_ptr(), max_tokens)
     _on(dev, "qw3_page_slots", C.byref(a), ws.h)
     return cu, pos, slots, kv_len, n_free_out
 
@@ -222,52 +232,52 @@ def rope_kv4_append(qkv, cache, slots, pos, cos, sin, heads, ws, pairs=False):
     """Rotates q and k of the rows qkv = [tokens][(heads + 2 kv_heads) * 128] by the angles of cos, sin = fp32 [max_pos][rot_dim / 2] (None: not
     at all) at pos, and stores k and v in 4 bits in their slots (below 0: not stored).  Returns the rotated q [tokens][heads][128] and
     k [tokens][kv_heads][128].  pairs: dims 2i and 2i + 1 turn together, as in rope_kv_append; else i and i + rot_dim / 2."""
-    dev, kv = qkv.device, cache.kv_heads
-    _want(cache.pages.device == dev, "qkv and the cache's pages: one device expected")
-    _, stride = _rows128(qkv, heads + 2 * kv, "qkv", dev, cache.dtype)
+    dev, kv, dtype = qkv.device, cache.kv_heads, cache.dtype
+    _want(cache.device == dev, "qkv and the cache's pages: one device expected")
+    _, stride = _rows128(qkv, heads + 2 * kv, "qkv", dev, dtype)
     tokens = qkv.shape[0]
-    _ints(slots, (tokens,), "slots", dev)
-    rot = 0
+    d_slots = _ints(slots, tokens, "slots", dev)
+    rot, max_pos, d_pos, d_cos, d_sin = 0, 0, None, None, None
     if cos is not None:
-        _ints(pos, (tokens,), "pos", dev)
+        d_pos = _ints(pos, tokens, "pos", dev)
         for t, what in ((cos, "cos"), (sin, "sin")):
-            _want(t is not None and t.device == dev and t.dtype == torch.float32 and t.dim() == 2 and t.is_contiguous() and t.shape == cos.shape and t.shape[0] > 0,
+            _want(t is not None and t.dtype == torch.float32 and t.device == dev and t.dim() == 2 and t.is_contiguous() and t.shape == cos.shape,
                   f"{what}: contiguous float32 [max_pos][rot_dim / 2] on {dev} expected")
-        rot = 2 * cos.shape[1]
-    q = torch.empty(tokens, heads, 128, dtype=cache.dtype, device=dev)
-    k = torch.empty(tokens, kv, 128, dtype=cache.dtype, device=dev)
-    a = cabi.Kv4AppendArgs(qkv.data_ptr(), stride, tokens, heads, cabi.ROPE_PAIRS if pairs else cabi.ROPE_HALVES, rot, 0, slots.data_ptr(),
-                           pos.data_ptr() if rot else None, cos.data_ptr() if rot else None, sin.data_ptr() if rot else None, cos.shape[0] if rot else 0,
+        max_pos, rot = cos.shape
+        rot *= 2
+        _want(max_pos > 0 and rot > 0, "cos: [max_pos][rot_dim / 2] expected")
+        d_cos, d_sin = cos.data_ptr(), sin.data_ptr()
+    q, k = torch.empty((heads + kv) * tokens, 128, dtype=dtype, device=dev).split_with_sizes((heads * tokens, kv * tokens))
+    a = cabi.Kv4AppendArgs(qkv.data_ptr(), stride, tokens, heads, cabi.ROPE_PAIRS if pairs else cabi.ROPE_HALVES, rot, 0, d_slots, d_pos, d_cos, d_sin, max_pos,
                            q.data_ptr(), k.data_ptr())
-    _on(dev, "qw3_rope_kv4_append", C.byref(cache.pool), C.byref(a), ws.h)
-    return q, k
+    _on(dev, "qw3_rope_kv4_append", cache.ref, C.byref(a), ws.h)
+    return q.view(tokens, heads, 128), k.view(tokens, kv, 128)
 
 
 def kv4_read(cache, slots, ws):
     """The rows of the slots as dense K and V, [tokens][kv_heads][128] each; zeros for a slot below 0."""
-    dev = cache.pages.device
+    dev = cache.device
     _want(slots.dim() == 1, "slots: one dimension expected")
-    tokens = slots.numel()
-    _ints(slots, (tokens,), "slots", dev)
-    k = torch.empty(tokens, cache.kv_heads, 128, dtype=cache.dtype, device=dev)
-    v = torch.empty_like(k)
-    _on(dev, "qw3_kv4_read", C.byref(cache.pool), slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr(), ws.h)
+    tokens = slots.shape[0]
+    d_slots = _ints(slots, tokens, "slots", dev)
+    k, v = torch.empty(2, tokens, cache.kv_heads, 128, dtype=cache.dtype, device=dev).unbind()
+    _on(dev, "qw3_kv4_read", cache.ref, d_slots, tokens, k.data_ptr(), v.data_ptr(), ws.h)
     return k, v
 
 
 def attn_kv4_decode(q, cache, block_table, kv_len, ws, scale=None):
     """Attention of one token a request, q = [requests][heads][128] after rotation, over the request's kv_len tokens in the cache; a row of
     zeros where there are none.  scale: of the scores, 1 / sqrt(128) by default."""
-    dev = q.device
-    _want(cache.pages.device == dev, "q and the cache's pages: one device expected")
+    dev, dtype = q.device, cache.dtype
+    _want(cache.device == dev, "q and the cache's pages: one device expected")
     _want(scale is None or scale != 0, "scale: 0 is not a scale")
-    heads, stride = _rows128(q, None, "q", dev, cache.dtype)
+    heads, stride = _rows128(q, None, "q", dev, dtype)
     n = q.shape[0]
-    _ints(kv_len, (n,), "kv_len", dev)
+    d_len = _ints(kv_len, n, "kv_len", dev)
     table_stride = _table(block_table, n, dev)
-    out = torch.empty(n, heads, 128, dtype=cache.dtype, device=dev)
-    a = cabi.AttnKv4Args(q.data_ptr(), stride, n, heads, block_table.data_ptr(), table_stride, block_table.shape[1], scale or 0.0, kv_len.data_ptr(), out.data_ptr())
-    _on(dev, "qw3_attn_kv4_decode", C.byref(cache.pool), C.byref(a), ws.h)
+    out = torch.empty(n, heads, 128, dtype=dtype, device=dev)
+    a = cabi.AttnKv4Args(q.data_ptr(), stride, n, heads, block_table.data_ptr(), table_stride, block_table.shape[1], scale or 0.0, d_len, out.data_ptr())
+    _on(dev, "qw3_attn_kv4_decode", cache.ref, C.byref(a), ws.h)
     return out
 
 
@@ -284,12 +294,13 @@ def attn_packed(q, k, v, cu_q, cu_k, ws, scale=None, out=None):
     _want(v.shape[0] == k.shape[0], "k and v: the same number of rows expected")
     n = cu_q.numel() - 1
     _want(n >= 0, "cu_q: [sequences + 1] expected")
-    _ints(cu_q, (n + 1,), "cu_q", dev)
-    _ints(cu_k, (n + 1,), "cu_k", dev)
+    d_cu_q, d_cu_k = _ints(cu_q, n + 1, "cu_q", dev), _ints(cu_k, n + 1, "cu_k", dev)
     if out is None:
         out = torch.empty(q.shape[0], heads, 128, dtype=dtype, device=dev)
-    _want(out.device == dev and out.dtype == dtype and out.is_contiguous() and out.numel() == q.shape[0] * heads * 128, "out: contiguous [q_rows][heads][128] expected")
-    a = cabi.AttnPackedArgs(q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, q.shape[0], k.shape[0], cu_q.data_ptr(), cu_k.data_ptr(), n,
+    else:
+        _want(out.device == dev and out.dtype == dtype and out.is_contiguous() and out.numel() == q.shape[0] * heads * 128,
+              "out: contiguous [q_rows][heads][128] expected")
+    a = cabi.AttnPackedArgs(q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, q.shape[0], k.shape[0], d_cu_q, d_cu_k, n,
                             heads, kv, 128, _DTYPES[dtype], scale or 0.0, out.data_ptr())
     _on(dev, "qw3_attn_packed", C.byref(a), ws.h)
     return out
