@@ -126,19 +126,41 @@ __global__ void __launch_bounds__(PS_THREADS) page_slots_kernel(const Qw3PageArg
 }
 
 // ---- rotation, quantisation, store -----------------------------------------------------------------------------------------------
-// A half-warp takes a row of 128 dims, eight to a lane; a CTA takes one token, whose cosines and sines its lanes keep for all heads.
-// Products and sums of the rotation are rounded one by one (no contraction), so that a row's codes do not depend on the compiler.
-// K is quantised from the fp32 rotated row, not from its rounding.
-constexpr int AP_THREADS = 256, AP_GROUPS = AP_THREADS / 16;
+// A half-warp takes a row of 128 dims, eight to a lane; a CTA takes one token, whose cosines and sines its lanes keep for all heads, sixteen
+// rows a round and the loads of three rounds at once (few tokens: one round a CTA).  Products and sums of the rotation are rounded one by
+// one (no contraction), so that a row's codes do not depend on the compiler.  K is quantised from the fp32 rotated row, not from its rounding.
+constexpr int AP_THREADS = 256, AP_GROUPS = AP_THREADS / 16, AP_BATCH = 3;
+
+__device__ __forceinline__ float min_nan(float a, float b) {   // NaN where either is
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
 template <class T, bool PAIRS>
-__global__ void __launch_bounds__(AP_THREADS)
-rope_kv4_append_kernel(const Qw3Kv4Pool pool, const Qw3Kv4AppendArgs p, int* err) {
+__global__ void __launch_bounds__(AP_THREADS, 4)
+rope_kv4_append_kernel(const Qw3Kv4Pool pool, const Qw3Kv4AppendArgs p, int rounds_a_cta, int* err) {
     using R = RowType<T>;
     const int tid = threadIdx.x, group = tid >> 4, l = tid & 15;
     const int token = blockIdx.x, kv = pool.kv_heads, P = pool.page_size, rot = p.rot_dim;
+    const int rows = p.heads + 2 * kv, r0 = blockIdx.y * rounds_a_cta, r1 = min(r0 + rounds_a_cta, (rows + AP_GROUPS - 1) / AP_GROUPS);
     pdl_launch_dependents();
     pdl_wait();
+    const T* const row = static_cast<const T*>(p.d_qkv) + (size_t)token * p.qkv_stride + 8 * l;
+    uint4 w[AP_BATCH];
+    const auto load = [&](int r) {
+#pragma unroll
+        for (int u = 0; u < AP_BATCH; ++u) {
+            const int j = group + AP_GROUPS * (r + u);
+            w[u] = r + u < r1 && j < rows ? *reinterpret_cast<const uint4*>(row + (size_t)j * 128) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    load(r0);
     const int slot = p.d_slot[token];
     const int pos = rot > 0 ? p.d_pos[token] : 0;
     if (rot > 0 && (pos < 0 || pos >= p.max_pos)) {
@@ -149,7 +171,7 @@ rope_kv4_append_kernel(const Qw3Kv4Pool pool, const Qw3Kv4AppendArgs p, int* err
     if (page >= pool.n_pages && tid == 0) kv4_error(err, KV4_ERR_APPEND_SLOT);
     const bool store = page >= 0 && page < pool.n_pages;
     uint8_t* const tile0 = static_cast<uint8_t*>(pool.d_pages) + (store ? page * pool.page_stride + (in_page >> 4) * KV4_TILE_BYTES : 0);
-    const int r = in_page & 15;
+    const int r_in = in_page & 15;
 
     float cs[8], sn[8];
     const bool turns = 8 * l < rot;
@@ -158,116 +180,134 @@ rope_kv4_append_kernel(const Qw3Kv4Pool pool, const Qw3Kv4AppendArgs p, int* err
     const int mate = PAIRS ? l : upper ? l - rot / 16 : l + rot / 16;
     if (turns) {
         const size_t at = (size_t)pos * (rot / 2) + (PAIRS ? 4 * l : 8 * (upper ? mate : l));
+#pragma unroll
         for (int e = 0; e < (PAIRS ? 4 : 8); e += 4) {
             const float4 c = *reinterpret_cast<const float4*>(p.d_cos + at + e), s = *reinterpret_cast<const float4*>(p.d_sin + at + e);
             cs[e] = c.x; cs[e + 1] = c.y; cs[e + 2] = c.z; cs[e + 3] = c.w;
             sn[e] = s.x; sn[e + 1] = s.y; sn[e + 2] = s.z; sn[e + 3] = s.w;
         }
     }
-    const T* const row = static_cast<const T*>(p.d_qkv) + (size_t)token * p.qkv_stride + 8 * l;
-    const int rows = p.heads + 2 * kv, last = (rows + AP_GROUPS - 1) / AP_GROUPS * AP_GROUPS;   // whole rounds: the shuffles need every lane
-    for (int j = group; j < last; j += AP_GROUPS) {
-        const uint4 w = j < rows ? *reinterpret_cast<const uint4*>(row + (size_t)j * 128) : make_uint4(0, 0, 0, 0);
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-        float x[8];
+    for (int r = r0; r < r1; r += AP_BATCH) {
+        if (r > r0) load(r);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = R::unpack(ws[e]);
-            x[2 * e] = f.x;
-            x[2 * e + 1] = f.y;
-        }
-        const bool is_q = j < p.heads, is_k = !is_q && j < p.heads + kv;
-        float y[8];
+        for (int u = 0; u < AP_BATCH; ++u) {
+            if (r + u >= r1) break;
+            const int j = group + AP_GROUPS * (r + u);   // may be past the last row: the shuffles need every lane
+            const uint32_t ws[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+            float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = PAIRS ? 0.0f : __shfl_sync(0xffffffffu, x[e], mate, 16);
-        if ((is_q || is_k) && turns) {
-            if (PAIRS) {
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = R::unpack(ws[e]);
+                x[2 * e] = f.x;
+                x[2 * e + 1] = f.y;
+            }
+            const bool is_q = j < p.heads, is_k = !is_q && j < p.heads + kv;
+            if (rot > 0 && __any_sync(0xffffffffu, is_q || is_k)) {
+                float y[8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float a = x[2 * e], b = x[2 * e + 1];
-                    x[2 * e] = __fsub_rn(__fmul_rn(a, cs[e]), __fmul_rn(b, sn[e]));
-                    x[2 * e + 1] = __fadd_rn(__fmul_rn(b, cs[e]), __fmul_rn(a, sn[e]));
-                }
-            } else {
+                for (int e = 0; e < 8; ++e) y[e] = PAIRS ? 0.0f : __shfl_sync(0xffffffffu, x[e], mate, 16);
+                if ((is_q || is_k) && turns) {
+                    if (PAIRS) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float own = __fmul_rn(x[e], cs[e]), other = __fmul_rn(y[e], sn[e]);
-                    x[e] = upper ? __fadd_rn(own, other) : __fsub_rn(own, other);
+                        for (int e = 0; e < 4; ++e) {
+                            const float a = x[2 * e], b = x[2 * e + 1];
+                            x[2 * e] = __fsub_rn(__fmul_rn(a, cs[e]), __fmul_rn(b, sn[e]));
+                            x[2 * e + 1] = __fadd_rn(__fmul_rn(b, cs[e]), __fmul_rn(a, sn[e]));
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float own = __fmul_rn(x[e], cs[e]), other = __fmul_rn(y[e], sn[e]);
+                            x[e] = upper ? __fadd_rn(own, other) : __fsub_rn(own, other);
+                        }
+                    }
                 }
             }
-        }
-        if (j < rows && (is_q || (is_k && p.d_k_out != nullptr))) {
-            T* const dst = is_q ? static_cast<T*>(p.d_q_out) + ((size_t)token * p.heads + j) * 128
-                                : static_cast<T*>(p.d_k_out) + ((size_t)token * kv + j - p.heads) * 128;
-            *reinterpret_cast<uint4*>(dst + 8 * l) = make_uint4(R::pack(x[0], x[1]), R::pack(x[2], x[3]), R::pack(x[4], x[5]), R::pack(x[6], x[7]));
-        }
-        float lo = x[0], hi = x[0];
-        bool finite = true;   // a difference that is not 0 is of Inf or NaN
+            if (j < rows && (is_q || (is_k && p.d_k_out != nullptr))) {
+                T* const dst = is_q ? static_cast<T*>(p.d_q_out) + ((size_t)token * p.heads + j) * 128
+                                    : static_cast<T*>(p.d_k_out) + ((size_t)token * kv + j - p.heads) * 128;
+                *reinterpret_cast<uint4*>(dst + 8 * l) = make_uint4(R::pack(x[0], x[1]), R::pack(x[2], x[3]), R::pack(x[4], x[5]), R::pack(x[6], x[7]));
+            }
+            const bool quantise = !is_q && j < rows && store;
+            if (!__any_sync(0xffffffffu, quantise)) continue;
+            float lo = x[0], hi = x[0];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            lo = fminf(lo, x[e]);
-            hi = fmaxf(hi, x[e]);
-            finite = finite && x[e] - x[e] == 0.0f;
-        }
+            for (int e = 1; e < 8; ++e) {
+                lo = min_nan(lo, x[e]);
+                hi = max_nan(hi, x[e]);
+            }
 #pragma unroll
-        for (int d = 8; d > 0; d >>= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-        }
-        const uint32_t alive = __ballot_sync(0xffffffffu, finite) >> (tid & 16) & 0xffffu;
-        if (is_q || j >= rows || !store) continue;
-        // minimum and scale as they are stored: the codes are those of the rounded pair
-        const uint32_t m_bits = R::pack(lo, lo) & 0xffffu;
-        const float m = R::unpack(m_bits).x;
-        float s = R::unpack(R::pack(__fdiv_rn(__fsub_rn(hi, m), 15.0f), 0.0f)).x;
-        const bool whole = alive == 0xffffu && s <= R::CEIL;
-        s = fmaxf(s, R::FLOOR);
-        uint32_t codes = 0;
+            for (int d = 8; d > 0; d >>= 1) {
+                lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+                hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+            }
+            if (!quantise) continue;
+            // minimum and scale as they are stored: the codes are those of the rounded pair
+            const uint32_t m_bits = R::pack(lo, lo) & 0xffffu;
+            const float m = R::unpack(m_bits).x;
+            float s = R::unpack(R::pack(__fdiv_rn(__fsub_rn(hi, m), 15.0f), 0.0f)).x;
+            const bool whole = s <= R::CEIL;   // not with Inf or NaN in the row
+            s = fmaxf(s, R::FLOOR);
+            const float inv = __frcp_rn(s);
+            uint32_t codes = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float c = rintf(__fdiv_rn(__fsub_rn(x[e], m), s));
-            codes |= (uint32_t)(int)fminf(fmaxf(c, 0.0f), 15.0f) << (4 * e);
+            for (int e = 0; e < 8; ++e) {
+                // the quotient rounded to nearest, which decides where it is halfway between two codes: one correction with the correctly
+                // rounded reciprocal (P. Markstein, Computation of elementary functions on the IBM RISC System/6000, 1990); where it is so
+                // small that the remainder underflows the code is 0
+                const float d = __fsub_rn(x[e], m), q = __fmul_rn(d, inv), c = rintf(fmaf(fmaf(-q, s, d), inv, q));
+                codes |= (uint32_t)(int)fminf(fmaxf(c, 0.0f), 15.0f) << (4 * e);
+            }
+            // a row with Inf or NaN reads back as NaN
+            const uint32_t pair = (R::pack(s, 0.0f) & 0xffffu) | (m_bits << 16);
+            uint8_t* const tile = tile0 + (size_t)(j - p.heads - (is_k ? 0 : kv)) * (P / 16) * KV4_TILE_BYTES;
+            *reinterpret_cast<uint32_t*>(tile + (is_k ? 0 : KV4_V) + r_in * 64 + 4 * l) = whole ? codes : 0u;
+            if (l == 0) *reinterpret_cast<uint32_t*>(tile + (is_k ? KV4_KP : KV4_VP) + r_in * 4) = whole ? pair : (R::pack(1.0f, 0.0f) & 0xffffu) | 0x7fff0000u;
         }
-        // a row with Inf or NaN reads back as NaN
-        const uint32_t pair = (R::pack(s, 0.0f) & 0xffffu) | (m_bits << 16);
-        uint8_t* const tile = tile0 + (size_t)(j - p.heads - (is_k ? 0 : kv)) * (P / 16) * KV4_TILE_BYTES;
-        *reinterpret_cast<uint32_t*>(tile + (is_k ? 0 : KV4_V) + r * 64 + 4 * l) = whole ? codes : 0u;
-        if (l == 0) *reinterpret_cast<uint32_t*>(tile + (is_k ? KV4_KP : KV4_VP) + r * 4) = whole ? pair : (R::pack(1.0f, 0.0f) & 0xffffu) | 0x7fff0000u;
     }
 }
 
 // ---- rows read back --------------------------------------------------------------------------------------------------------------
-// A half-warp takes a row: four bytes of codes in, sixteen out, a lane.  A slot below zero gives a row of zeros.
-constexpr int RD_THREADS = 256, RD_GROUPS = RD_THREADS / 16;
+// A half-warp takes four rows at a time: four bytes of codes in, sixteen out, a lane, of K and of V.  A slot below zero gives zeros.
+constexpr int RD_THREADS = 256, RD_GROUPS = RD_THREADS / 16, RD_ROWS = 4;
 
 template <class T>
 __global__ void __launch_bounds__(RD_THREADS)
-kv4_read_kernel(const Qw3Kv4Pool pool, const int32_t* __restrict__ d_slot, int64_t tokens, T* __restrict__ k_out, T* __restrict__ v_out, int* err) {
+kv4_read_kernel(const Qw3Kv4Pool pool, const int32_t* __restrict__ d_slot, uint32_t rows, T* __restrict__ k_out, T* __restrict__ v_out, int* err) {
     using R = RowType<T>;
     pdl_launch_dependents();
     pdl_wait();
-    const int l = threadIdx.x & 15, kv = pool.kv_heads, P = pool.page_size;
-    const int64_t rows = tokens * kv;
-    for (int64_t i = (int64_t)blockIdx.x * RD_GROUPS + (threadIdx.x >> 4); i < rows; i += (int64_t)gridDim.x * RD_GROUPS) {
-        const int64_t token = i / kv;
-        const int head = (int)(i - token * kv), slot = d_slot[token];
-        const int page = slot >= 0 ? slot / P : -1, in_page = slot - page * P;
-        if (page >= pool.n_pages && l == 0) kv4_error(err, KV4_ERR_READ_SLOT);
-        const bool there = page >= 0 && page < pool.n_pages;
-        const uint8_t* const tile = static_cast<const uint8_t*>(pool.d_pages) + (there ? page * pool.page_stride + ((int64_t)head * (P / 16) + (in_page >> 4)) * KV4_TILE_BYTES : 0);
-        const int r = in_page & 15;
+    const int l = threadIdx.x & 15;
+    const uint32_t kv = pool.kv_heads, P = pool.page_size, first = blockIdx.x * (RD_GROUPS * RD_ROWS) + (threadIdx.x >> 4);
+    uint32_t codes[RD_ROWS][2], pair[RD_ROWS][2];
+#pragma unroll
+    for (int u = 0; u < RD_ROWS; ++u) {
+        const uint32_t i = first + RD_GROUPS * u, token = i / kv, head = i - token * kv;
+        const int slot = i < rows ? d_slot[token] : -1;
+        const uint32_t page = (uint32_t)slot / P, in_page = (uint32_t)slot - page * P;
+        const bool there = slot >= 0 && page < pool.n_pages;
+        if (slot >= 0 && !there && l == 0) kv4_error(err, KV4_ERR_READ_SLOT);
+        codes[u][0] = codes[u][1] = pair[u][0] = pair[u][1] = 0;
+        if (there) {
+            const uint8_t* const tile = static_cast<const uint8_t*>(pool.d_pages) + page * pool.page_stride + ((int64_t)head * (P / 16) + (in_page >> 4)) * KV4_TILE_BYTES;
+            const uint32_t r = in_page & 15;
+            codes[u][0] = *reinterpret_cast<const uint32_t*>(tile + r * 64 + 4 * l);
+            codes[u][1] = *reinterpret_cast<const uint32_t*>(tile + KV4_V + r * 64 + 4 * l);
+            pair[u][0] = *reinterpret_cast<const uint32_t*>(tile + KV4_KP + r * 4);
+            pair[u][1] = *reinterpret_cast<const uint32_t*>(tile + KV4_VP + r * 4);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < RD_ROWS; ++u) {
+        const uint32_t i = first + RD_GROUPS * u;
+        if (i >= rows) break;
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
-            uint32_t codes = 0, pair = 0;
-            if (there) {
-                codes = *reinterpret_cast<const uint32_t*>(tile + (v ? KV4_V : 0) + r * 64 + 4 * l);
-                pair = *reinterpret_cast<const uint32_t*>(tile + (v ? KV4_VP : KV4_KP) + r * 4);
-            }
-            const float2 sm = R::unpack(pair);
+            const float2 sm = R::unpack(pair[u][v]);
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)   // code * scale is exact in fp32
-                w[e] = R::pack(fmaf((float)(codes >> (8 * e) & 15u), sm.x, sm.y), fmaf((float)(codes >> (8 * e + 4) & 15u), sm.x, sm.y));
+                w[e] = R::pack(fmaf((float)(codes[u][v] >> (8 * e) & 15u), sm.x, sm.y), fmaf((float)(codes[u][v] >> (8 * e + 4) & 15u), sm.x, sm.y));
             *reinterpret_cast<uint4*>((v ? v_out : k_out) + (size_t)i * 128 + 8 * l) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
@@ -340,7 +380,10 @@ int qw3_rope_kv4_append(const Qw3Kv4Pool* pool, const Qw3Kv4AppendArgs* a, qw3_w
                 "%s: rows and tables must be 16-byte aligned", who);
     const auto kernel = pool->dtype == QW3_F16 ? (a->layout == QW3_ROPE_PAIRS ? rope_kv4_append_kernel<__half, true> : rope_kv4_append_kernel<__half, false>)
                                                : (a->layout == QW3_ROPE_PAIRS ? rope_kv4_append_kernel<__nv_bfloat16, true> : rope_kv4_append_kernel<__nv_bfloat16, false>);
-    QW3_CUDA(kv4_launch(kernel, dim3((unsigned)a->tokens), dim3(AP_THREADS), 0, static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, *pool, *a, ws_struct(ws)->err));
+    // few tokens: their rounds side by side, so that all SMs take part
+    const int rounds = (a->heads + 2 * pool->kv_heads + AP_GROUPS - 1) / AP_GROUPS, each = a->tokens < 2 * ws_struct(ws)->sm_count ? 1 : rounds;
+    QW3_CUDA(kv4_launch(kernel, dim3((unsigned)a->tokens, (rounds + each - 1) / each), dim3(AP_THREADS), 0, static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, *pool, *a,
+                        each, ws_struct(ws)->err));
     return QW3_OK;
 }
 
@@ -352,13 +395,14 @@ int qw3_kv4_read(const Qw3Kv4Pool* pool, const int32_t* d_slot, int64_t tokens, 
     if (tokens == 0) return QW3_OK;
     QW3_REQUIRE(d_slot && d_k_out && d_v_out, "%s: null pointer", who);
     QW3_REQUIRE(aligned16(d_k_out) && aligned16(d_v_out), "%s: rows must be 16-byte aligned", who);
-    const int64_t ctas = (tokens * pool->kv_heads + RD_GROUPS - 1) / RD_GROUPS, most = (int64_t)ws_struct(ws)->sm_count * 8;
-    const dim3 grid((unsigned)(ctas < most ? ctas : most));
+    const int64_t rows = tokens * pool->kv_heads;   // 512 bytes of output each
+    QW3_REQUIRE(rows <= 0x7fffffff - RD_GROUPS * RD_ROWS, "%s: too many rows", who);
+    const dim3 grid((unsigned)((rows + RD_GROUPS * RD_ROWS - 1) / (RD_GROUPS * RD_ROWS)));
     if (pool->dtype == QW3_F16)
-        QW3_CUDA(kv4_launch(kv4_read_kernel<__half>, grid, dim3(RD_THREADS), 0, static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, *pool, d_slot, tokens,
+        QW3_CUDA(kv4_launch(kv4_read_kernel<__half>, grid, dim3(RD_THREADS), 0, static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, *pool, d_slot, (uint32_t)rows,
                         static_cast<__half*>(d_k_out), static_cast<__half*>(d_v_out), ws_struct(ws)->err));
     else
-        QW3_CUDA(kv4_launch(kv4_read_kernel<__nv_bfloat16>, grid, dim3(RD_THREADS), 0, static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, *pool, d_slot, tokens,
+        QW3_CUDA(kv4_launch(kv4_read_kernel<__nv_bfloat16>, grid, dim3(RD_THREADS), 0, static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, *pool, d_slot, (uint32_t)rows,
                         static_cast<__nv_bfloat16*>(d_k_out), static_cast<__nv_bfloat16*>(d_v_out), ws_struct(ws)->err));
     return QW3_OK;
 }

@@ -160,7 +160,7 @@ def _rows128(t, heads, what, device, dtype):
 
 
 def _ints(t, n, what, device):
-    if t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.device != device or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{what}: contiguous int32 [{n}] on {device} expected")
     return t.data_ptr()
 
