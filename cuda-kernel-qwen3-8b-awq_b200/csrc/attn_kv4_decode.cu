@@ -64,11 +64,6 @@ __device__ __forceinline__ uint32_t kd_transpose(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
-__device__ __forceinline__ void kd_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
-}
-
 // D = A * B
 __device__ __forceinline__ void kd_mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -256,10 +251,10 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
             sm.valid[warp][s] = n;
             mbar_expect_tx(bar, (n0 ? KV4_TILE_BYTES : 0) + (n1 ? KV4_TILE_BYTES : 0));
             if (n0 && n1 && b - a == KV4_TILE_BYTES) {   // of one page
-                kd_copy(to, reinterpret_cast<const void*>(a), 2 * KV4_TILE_BYTES, bar);
+                bulk_load(to, reinterpret_cast<const void*>(a), 2 * KV4_TILE_BYTES, bar);
             } else {
-                if (n0) kd_copy(to, reinterpret_cast<const void*>(a), KV4_TILE_BYTES, bar);
-                if (n1) kd_copy(to + KV4_TILE_BYTES, reinterpret_cast<const void*>(b), KV4_TILE_BYTES, bar);
+                if (n0) bulk_load(to, reinterpret_cast<const void*>(a), KV4_TILE_BYTES, bar);
+                if (n1) bulk_load(to + KV4_TILE_BYTES, reinterpret_cast<const void*>(b), KV4_TILE_BYTES, bar);
             }
         }
         __syncwarp();

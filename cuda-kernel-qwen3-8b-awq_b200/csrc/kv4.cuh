@@ -52,6 +52,11 @@ template <> struct RowType<__nv_bfloat16> {
     }
 };
 
+// untiled bulk copy global -> shared; addresses and size are multiples of 16
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 __device__ __forceinline__ void kv4_error(int* err, int code) { atomicCAS(err, 0, code); }
 
 // Launch helper: optional programmatic dependent launch and cluster size.

@@ -126,11 +126,28 @@ __global__ void __launch_bounds__(PS_THREADS) page_slots_kernel(const Qw3PageArg
 }
 
 // ---- rotation, quantisation, store -----------------------------------------------------------------------------------------------
-// A half-warp takes a row of 128 dims, eight to a lane; a CTA takes one token, whose cosines and sines its lanes keep for all heads, sixteen
-// rows a round and the loads of three rounds at once (few tokens: one round a CTA).  Products and sums of the rotation are rounded one by
-// one (no contraction), so that a row's codes do not depend on the compiler.  K is quantised from the fp32 rotated row, not from its rounding.
-constexpr int AP_THREADS = 256, AP_GROUPS = AP_THREADS / 16, AP_BATCH = 3;
+// A CTA takes the rows of one token, or, of few tokens, sixteen of them, so that all SMs take part; one bulk copy brings them, while slot,
+// position and the cosines and sines, which the lanes keep for all heads, are looked up.  A half-warp takes a row of 128 dims, eight to a
+// lane.  Products and sums of the rotation are rounded one by one (no contraction), so that a row's codes do not depend on the compiler.  K
+// is quantised from the fp32 rotated row, not from its rounding.  Bound by issue slots: AP_NOTE
+constexpr int AP_THREADS = 256, AP_GROUPS = AP_THREADS / 16, AP_MAX_ROUNDS = 6;
 
+// two fp32 operations in one instruction, each rounded to nearest
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(*reinterpret_cast<unsigned long long*>(&r)) : "l"(*reinterpret_cast<const unsigned long long*>(&a)), "l"(*reinterpret_cast<const unsigned long long*>(&b)));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*reinterpret_cast<unsigned long long*>(&r)) : "l"(*reinterpret_cast<const unsigned long long*>(&a)), "l"(*reinterpret_cast<const unsigned long long*>(&b)));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(*reinterpret_cast<unsigned long long*>(&r)) : "l"(*reinterpret_cast<const unsigned long long*>(&a)), "l"(*reinterpret_cast<const unsigned long long*>(&b)), "l"(*reinterpret_cast<const unsigned long long*>(&c)));
+    return r;
+}
 __device__ __forceinline__ float min_nan(float a, float b) {   // NaN where either is
     float r;
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -141,40 +158,57 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+// over the lanes of `mask`
+__device__ __forceinline__ float min_nan_over(float a, uint32_t mask) {
+    float r;
+    asm volatile("redux.sync.min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "r"(mask));
+    return r;
+}
+__device__ __forceinline__ float max_nan_over(float a, uint32_t mask) {
+    float r;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "r"(mask));
+    return r;
+}
+// a / b rounded to nearest, for normal b and inv = 1 / b rounded to nearest: one correction by the remainder, which is exact (P. Markstein,
+// Computation of elementary functions on the IBM RISC System/6000, 1990).  Where a is so small that it underflows, the caller's result is 0.
+__device__ __forceinline__ float2 quotient(float2 a, float b, float inv) {
+    const float2 i = make_float2(inv, inv), q = mul2(a, i);
+    return fma2(fma2(make_float2(-q.x, -q.y), make_float2(b, b), a), i, q);
+}
 
 template <class T, bool PAIRS>
 __global__ void __launch_bounds__(AP_THREADS, 4)
 rope_kv4_append_kernel(const Qw3Kv4Pool pool, const Qw3Kv4AppendArgs p, int rounds_a_cta, int* err) {
     using R = RowType<T>;
-    const int tid = threadIdx.x, group = tid >> 4, l = tid & 15;
+    extern __shared__ __align__(128) uint4 ap_rows[];
+    __shared__ uint64_t bar;
+    const int tid = threadIdx.x, group = tid >> 4, l = tid & 15, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const uint32_t half = tid & 16 ? 0xffff0000u : 0x0000ffffu;   // the lanes of the row
     const int token = blockIdx.x, kv = pool.kv_heads, P = pool.page_size, rot = p.rot_dim;
-    const int rows = p.heads + 2 * kv, r0 = blockIdx.y * rounds_a_cta, r1 = min(r0 + rounds_a_cta, (rows + AP_GROUPS - 1) / AP_GROUPS);
+    const int rows = p.heads + 2 * kv, first = blockIdx.y * rounds_a_cta * AP_GROUPS, last = min(first + rounds_a_cta * AP_GROUPS, rows);
     pdl_launch_dependents();
+    if (tid == 0) {
+        mbar_init(smem_u32(&bar), 1);
+        mbar_fence_init();
+    }
     pdl_wait();
-    const T* const row = static_cast<const T*>(p.d_qkv) + (size_t)token * p.qkv_stride + 8 * l;
-    uint4 w[AP_BATCH];
-    const auto load = [&](int r) {
-#pragma unroll
-        for (int u = 0; u < AP_BATCH; ++u) {
-            const int j = group + AP_GROUPS * (r + u);
-            w[u] = r + u < r1 && j < rows ? *reinterpret_cast<const uint4*>(row + (size_t)j * 128) : make_uint4(0, 0, 0, 0);
-        }
-    };
-    load(r0);
+    if (tid == 0) {
+        const uint32_t bytes = (uint32_t)(last - first) * 256;
+        mbar_expect_tx(smem_u32(&bar), bytes);
+        bulk_load(smem_u32(ap_rows), static_cast<const T*>(p.d_qkv) + (size_t)token * p.qkv_stride + (size_t)first * 128, bytes, smem_u32(&bar));
+    }
     const int slot = p.d_slot[token];
     const int pos = rot > 0 ? p.d_pos[token] : 0;
-    if (rot > 0 && (pos < 0 || pos >= p.max_pos)) {
-        if (tid == 0) kv4_error(err, KV4_ERR_APPEND_POS);
-        return;
-    }
+    const bool known = rot == 0 || (pos >= 0 && pos < p.max_pos);
+    if (!known && tid == 0) kv4_error(err, KV4_ERR_APPEND_POS);
     const int page = slot >= 0 ? slot / P : -1, in_page = slot - page * P;
     if (page >= pool.n_pages && tid == 0) kv4_error(err, KV4_ERR_APPEND_SLOT);
     const bool store = page >= 0 && page < pool.n_pages;
     uint8_t* const tile0 = static_cast<uint8_t*>(pool.d_pages) + (store ? page * pool.page_stride + (in_page >> 4) * KV4_TILE_BYTES : 0);
     const int r_in = in_page & 15;
 
-    float cs[8], sn[8];
-    const bool turns = 8 * l < rot;
+    float2 cs[4], sn[4];   // pairs: (c, c) and (-s, s) of a pair; halves: of two dims, the sines with the sign that they enter with
+    const bool turns = known && 8 * l < rot;
     // halves: lane l holds dims 8l .. 8l+7 of one half, lane `mate` their partners; pairs: four pairs in the lane
     const bool upper = !PAIRS && 16 * l >= rot;
     const int mate = PAIRS ? l : upper ? l - rot / 16 : l + rot / 16;
@@ -183,87 +217,77 @@ rope_kv4_append_kernel(const Qw3Kv4Pool pool, const Qw3Kv4AppendArgs p, int roun
 #pragma unroll
         for (int e = 0; e < (PAIRS ? 4 : 8); e += 4) {
             const float4 c = *reinterpret_cast<const float4*>(p.d_cos + at + e), s = *reinterpret_cast<const float4*>(p.d_sin + at + e);
-            cs[e] = c.x; cs[e + 1] = c.y; cs[e + 2] = c.z; cs[e + 3] = c.w;
-            sn[e] = s.x; sn[e + 1] = s.y; sn[e + 2] = s.z; sn[e + 3] = s.w;
+            if (PAIRS) {
+                cs[0] = make_float2(c.x, c.x); cs[1] = make_float2(c.y, c.y); cs[2] = make_float2(c.z, c.z); cs[3] = make_float2(c.w, c.w);
+                sn[0] = make_float2(-s.x, s.x); sn[1] = make_float2(-s.y, s.y); sn[2] = make_float2(-s.z, s.z); sn[3] = make_float2(-s.w, s.w);
+            } else {
+                const float sign = upper ? 1.0f : -1.0f;
+                cs[e / 2] = make_float2(c.x, c.y); cs[e / 2 + 1] = make_float2(c.z, c.w);
+                sn[e / 2] = make_float2(sign * s.x, sign * s.y); sn[e / 2 + 1] = make_float2(sign * s.z, sign * s.w);
+            }
         }
     }
-    for (int r = r0; r < r1; r += AP_BATCH) {
-        if (r > r0) load(r);
+    __syncthreads();
+    if (!mbar_wait(smem_u32(&bar), 0)) {
+        if (tid == 0) atomicCAS(err, 0, 0x30051);
+        mbar_wait(smem_u32(&bar), 0);   // the copy in flight
+        return;
+    }
+    if (!known) return;
+    for (int j0 = first + 2 * warp; j0 < last; j0 += AP_GROUPS) {   // the first of the warp's two rows
+        const int j = j0 + (group & 1);   // may be past the last row: the shuffles need every lane
+        const bool is_q = j < p.heads, is_k = !is_q && j < p.heads + kv;
+        const uint4 w = ap_rows[min(j, last - 1) * 16 - first * 16 + l];
+        float2 x[4] = {R::unpack(w.x), R::unpack(w.y), R::unpack(w.z), R::unpack(w.w)};
+        if (rot > 0 && j0 < p.heads + kv) {
+            float2 y[4];
 #pragma unroll
-        for (int u = 0; u < AP_BATCH; ++u) {
-            if (r + u >= r1) break;
-            const int j = group + AP_GROUPS * (r + u);   // may be past the last row: the shuffles need every lane
-            const uint32_t ws[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
-            float x[8];
+            for (int e = 0; e < 4; ++e)
+                y[e] = PAIRS ? make_float2(x[e].y, x[e].x) : make_float2(__shfl_sync(0xffffffffu, x[e].x, mate, 16), __shfl_sync(0xffffffffu, x[e].y, mate, 16));
+            if ((is_q || is_k) && turns) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = R::unpack(ws[e]);
-                x[2 * e] = f.x;
-                x[2 * e + 1] = f.y;
+                for (int e = 0; e < 4; ++e)   // scalar products: a packed one would be contracted into the sum
+                    x[e] = add2(make_float2(__fmul_rn(x[e].x, cs[e].x), __fmul_rn(x[e].y, cs[e].y)), make_float2(__fmul_rn(y[e].x, sn[e].x), __fmul_rn(y[e].y, sn[e].y)));
             }
-            const bool is_q = j < p.heads, is_k = !is_q && j < p.heads + kv;
-            if (rot > 0 && __any_sync(0xffffffffu, is_q || is_k)) {
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = PAIRS ? 0.0f : __shfl_sync(0xffffffffu, x[e], mate, 16);
-                if ((is_q || is_k) && turns) {
-                    if (PAIRS) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float a = x[2 * e], b = x[2 * e + 1];
-                            x[2 * e] = __fsub_rn(__fmul_rn(a, cs[e]), __fmul_rn(b, sn[e]));
-                            x[2 * e + 1] = __fadd_rn(__fmul_rn(b, cs[e]), __fmul_rn(a, sn[e]));
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float own = __fmul_rn(x[e], cs[e]), other = __fmul_rn(y[e], sn[e]);
-                            x[e] = upper ? __fadd_rn(own, other) : __fsub_rn(own, other);
-                        }
-                    }
-                }
-            }
-            if (j < rows && (is_q || (is_k && p.d_k_out != nullptr))) {
-                T* const dst = is_q ? static_cast<T*>(p.d_q_out) + ((size_t)token * p.heads + j) * 128
-                                    : static_cast<T*>(p.d_k_out) + ((size_t)token * kv + j - p.heads) * 128;
-                *reinterpret_cast<uint4*>(dst + 8 * l) = make_uint4(R::pack(x[0], x[1]), R::pack(x[2], x[3]), R::pack(x[4], x[5]), R::pack(x[6], x[7]));
-            }
-            const bool quantise = !is_q && j < rows && store;
-            if (!__any_sync(0xffffffffu, quantise)) continue;
-            float lo = x[0], hi = x[0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) {
-                lo = min_nan(lo, x[e]);
-                hi = max_nan(hi, x[e]);
-            }
-#pragma unroll
-            for (int d = 8; d > 0; d >>= 1) {
-                lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-                hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-            }
-            if (!quantise) continue;
-            // minimum and scale as they are stored: the codes are those of the rounded pair
-            const uint32_t m_bits = R::pack(lo, lo) & 0xffffu;
-            const float m = R::unpack(m_bits).x;
-            float s = R::unpack(R::pack(__fdiv_rn(__fsub_rn(hi, m), 15.0f), 0.0f)).x;
-            const bool whole = s <= R::CEIL;   // not with Inf or NaN in the row
-            s = fmaxf(s, R::FLOOR);
-            const float inv = __frcp_rn(s);
-            uint32_t codes = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                // the quotient rounded to nearest, which decides where it is halfway between two codes: one correction with the correctly
-                // rounded reciprocal (P. Markstein, Computation of elementary functions on the IBM RISC System/6000, 1990); where it is so
-                // small that the remainder underflows the code is 0
-                const float d = __fsub_rn(x[e], m), q = __fmul_rn(d, inv), c = rintf(fmaf(fmaf(-q, s, d), inv, q));
-                codes |= (uint32_t)(int)fminf(fmaxf(c, 0.0f), 15.0f) << (4 * e);
-            }
-            // a row with Inf or NaN reads back as NaN
-            const uint32_t pair = (R::pack(s, 0.0f) & 0xffffu) | (m_bits << 16);
-            uint8_t* const tile = tile0 + (size_t)(j - p.heads - (is_k ? 0 : kv)) * (P / 16) * KV4_TILE_BYTES;
-            *reinterpret_cast<uint32_t*>(tile + (is_k ? 0 : KV4_V) + r_in * 64 + 4 * l) = whole ? codes : 0u;
-            if (l == 0) *reinterpret_cast<uint32_t*>(tile + (is_k ? KV4_KP : KV4_VP) + r_in * 4) = whole ? pair : (R::pack(1.0f, 0.0f) & 0xffffu) | 0x7fff0000u;
         }
+        if (j < rows && (is_q || (is_k && p.d_k_out != nullptr))) {
+            T* const dst = is_q ? static_cast<T*>(p.d_q_out) + ((size_t)token * p.heads + j) * 128
+                                : static_cast<T*>(p.d_k_out) + ((size_t)token * kv + j - p.heads) * 128;
+            *reinterpret_cast<uint4*>(dst + 8 * l) = make_uint4(R::pack(x[0].x, x[0].y), R::pack(x[1].x, x[1].y), R::pack(x[2].x, x[2].y), R::pack(x[3].x, x[3].y));
+        }
+        if (!store || j0 + 1 < p.heads) continue;
+        float lo = min_nan(x[0].x, x[0].y), hi = max_nan(x[0].x, x[0].y);
+#pragma unroll
+        for (int e = 1; e < 4; ++e) {
+            lo = min_nan(lo, min_nan(x[e].x, x[e].y));
+            hi = max_nan(hi, max_nan(x[e].x, x[e].y));
+        }
+        lo = min_nan_over(lo, half);
+        hi = max_nan_over(hi, half);
+        if (is_q || j >= rows) continue;
+        // minimum and scale as they are stored: the codes are those of the rounded pair
+        const uint32_t m_bits = R::pack(lo, lo) & 0xffffu;
+        const float m = R::unpack(m_bits).x, range = __fsub_rn(hi, m);
+        float s = R::unpack(R::pack(quotient(make_float2(range, range), 15.0f, 1.0f / 15.0f).x, 0.0f)).x;
+        const bool whole = s <= R::CEIL;   // not with Inf or NaN in the row
+        s = fmaxf(s, R::FLOOR);
+        const float inv = __frcp_rn(s);
+        // 1.5 * 2^23 + quotient rounds the quotient to the nearest whole number, ties to even (that they are found is why the quotient is
+        // rounded correctly), and has it in its last bits
+        constexpr float MAGIC = 12582912.0f;
+        uint32_t codes = 0;
+#pragma unroll
+        for (int e = 3; e >= 0; --e) {
+            const float2 c = add2(quotient(add2(x[e], make_float2(-m, -m)), s, inv), make_float2(MAGIC, MAGIC));
+            codes = codes * 16u + __float_as_uint(fminf(fmaxf(c.y, MAGIC), MAGIC + 15.0f));
+            codes = codes * 16u + __float_as_uint(fminf(fmaxf(c.x, MAGIC), MAGIC + 15.0f));
+        }
+        codes -= 0x4b400000u * 0x11111111u;   // eight times the bits of MAGIC
+        // a row with Inf or NaN reads back as NaN
+        const uint32_t pair = (R::pack(s, 0.0f) & 0xffffu) | (m_bits << 16);
+        uint8_t* const tile = tile0 + (size_t)(j - p.heads - (is_k ? 0 : kv)) * (P / 16) * KV4_TILE_BYTES;
+        *reinterpret_cast<uint32_t*>(tile + (is_k ? 0 : KV4_V) + r_in * 64 + 4 * l) = whole ? codes : 0u;
+        if (l == 0) *reinterpret_cast<uint32_t*>(tile + (is_k ? KV4_KP : KV4_VP) + r_in * 4) = whole ? pair : (R::pack(1.0f, 0.0f) & 0xffffu) | 0x7fff0000u;
     }
 }
 
@@ -380,10 +404,10 @@ int qw3_rope_kv4_append(const Qw3Kv4Pool* pool, const Qw3Kv4AppendArgs* a, qw3_w
                 "%s: rows and tables must be 16-byte aligned", who);
     const auto kernel = pool->dtype == QW3_F16 ? (a->layout == QW3_ROPE_PAIRS ? rope_kv4_append_kernel<__half, true> : rope_kv4_append_kernel<__half, false>)
                                                : (a->layout == QW3_ROPE_PAIRS ? rope_kv4_append_kernel<__nv_bfloat16, true> : rope_kv4_append_kernel<__nv_bfloat16, false>);
-    // few tokens: their rounds side by side, so that all SMs take part
-    const int rounds = (a->heads + 2 * pool->kv_heads + AP_GROUPS - 1) / AP_GROUPS, each = a->tokens < 2 * ws_struct(ws)->sm_count ? 1 : rounds;
-    QW3_CUDA(kv4_launch(kernel, dim3((unsigned)a->tokens, (rounds + each - 1) / each), dim3(AP_THREADS), 0, static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, *pool, *a,
-                        each, ws_struct(ws)->err));
+    const int rounds = (a->heads + 2 * pool->kv_heads + AP_GROUPS - 1) / AP_GROUPS, parts = (rounds + AP_MAX_ROUNDS - 1) / AP_MAX_ROUNDS;
+    const int each = a->tokens < 2 * ws_struct(ws)->sm_count ? 1 : (rounds + parts - 1) / parts;
+    QW3_CUDA(kv4_launch(kernel, dim3((unsigned)a->tokens, (rounds + each - 1) / each), dim3(AP_THREADS), (size_t)each * AP_GROUPS * 256, static_cast<cudaStream_t>(stream),
+                        ws_pdl(ws), 1, *pool, *a, each, ws_struct(ws)->err));
     return QW3_OK;
 }
 
