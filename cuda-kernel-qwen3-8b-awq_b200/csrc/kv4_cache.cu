@@ -1,6 +1,8 @@
 // Paged 4-bit KV cache: pages handed out to requests that grow, rows rotated, quantised and stored, rows read back.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "kv4.cuh"
 
 namespace qw3 {
@@ -126,11 +128,12 @@ __global__ void __launch_bounds__(PS_THREADS) page_slots_kernel(const Qw3PageArg
 }
 
 // ---- rotation, quantisation, store -----------------------------------------------------------------------------------------------
-// A CTA takes the rows of one token, or, of few tokens, sixteen of them, so that all SMs take part; one bulk copy brings them, while slot,
-// position and the cosines and sines, which the lanes keep for all heads, are looked up.  A half-warp takes a row of 128 dims, eight to a
+// A CTA takes the rows of one token, or, of few tokens, a slice of them, so that all SMs take part; bulk copies bring them, while slot,
+// position and the cosines and sines, which the lanes keep for all heads, are looked up.  A warp takes two rows at a time, eight dims a
 // lane.  Products and sums of the rotation are rounded one by one (no contraction), so that a row's codes do not depend on the compiler.  K
-// is quantised from the fp32 rotated row, not from its rounding.  Bound by issue slots: AP_NOTE
-constexpr int AP_THREADS = 256, AP_GROUPS = AP_THREADS / 16, AP_MAX_ROUNDS = 6;
+// is quantised from the fp32 rotated row, not from its rounding.  Bound by issue slots: 4001 tokens, 32 KV
+// heads, bf16, 181 MB: 43 us, 4.2 TB/s.
+constexpr int AP_THREADS = 256, AP_WARPS = AP_THREADS / 32, AP_MAX_ROWS = 96;
 
 // two fp32 operations in one instruction, each rounded to nearest
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -158,16 +161,19 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// over the lanes of `mask`
-__device__ __forceinline__ float min_nan_over(float a, uint32_t mask) {
-    float r;
-    asm volatile("redux.sync.min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "r"(mask));
-    return r;
-}
-__device__ __forceinline__ float max_nan_over(float a, uint32_t mask) {
-    float r;
-    asm volatile("redux.sync.max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "r"(mask));
-    return r;
+// Over the lanes of either half-warp.  Two reductions over the whole warp: one with a mask a half would be run half after half.
+template <bool MAX>
+__device__ __forceinline__ float reduce_half(float a, bool upper) {
+    const float none = MAX ? -INFINITY : INFINITY;
+    float lo, hi;
+    if (MAX) {
+        asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(lo) : "f"(upper ? none : a));
+        asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(hi) : "f"(upper ? a : none));
+    } else {
+        asm volatile("redux.sync.min.NaN.f32 %0, %1, 0xffffffff;" : "=f"(lo) : "f"(upper ? none : a));
+        asm volatile("redux.sync.min.NaN.f32 %0, %1, 0xffffffff;" : "=f"(hi) : "f"(upper ? a : none));
+    }
+    return upper ? hi : lo;
 }
 // a / b rounded to nearest, for normal b and inv = 1 / b rounded to nearest: one correction by the remainder, which is exact (P. Markstein,
 // Computation of elementary functions on the IBM RISC System/6000, 1990).  Where a is so small that it underflows, the caller's result is 0.
@@ -178,14 +184,17 @@ __device__ __forceinline__ float2 quotient(float2 a, float b, float inv) {
 
 template <class T, bool PAIRS>
 __global__ void __launch_bounds__(AP_THREADS, 4)
-rope_kv4_append_kernel(const Qw3Kv4Pool pool, const Qw3Kv4AppendArgs p, int rounds_a_cta, int* err) {
+rope_kv4_append_kernel(const Qw3Kv4Pool pool, const Qw3Kv4AppendArgs p, int* err) {
     using R = RowType<T>;
     extern __shared__ __align__(128) uint4 ap_rows[];
     __shared__ uint64_t bar;
-    const int tid = threadIdx.x, group = tid >> 4, l = tid & 15, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-    const uint32_t half = tid & 16 ? 0xffff0000u : 0x0000ffffu;   // the lanes of the row
+    const int tid = threadIdx.x, l = tid & 15, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const bool second = (tid & 16) != 0;   // row of the warp's two
     const int token = blockIdx.x, kv = pool.kv_heads, P = pool.page_size, rot = p.rot_dim;
-    const int rows = p.heads + 2 * kv, first = blockIdx.y * rounds_a_cta * AP_GROUPS, last = min(first + rounds_a_cta * AP_GROUPS, rows);
+    // this CTA's slice: rows q0 .. q1 of q, k0 .. k1 of k and of v
+    const int q0 = p.heads * (int)blockIdx.y / (int)gridDim.y, q1 = p.heads * (int)(blockIdx.y + 1) / (int)gridDim.y;
+    const int k0 = kv * (int)blockIdx.y / (int)gridDim.y, k1 = kv * (int)(blockIdx.y + 1) / (int)gridDim.y;
+    const int nq = q1 - q0, nk = k1 - k0;
     pdl_launch_dependents();
     if (tid == 0) {
         mbar_init(smem_u32(&bar), 1);
@@ -193,9 +202,12 @@ rope_kv4_append_kernel(const Qw3Kv4Pool pool, const Qw3Kv4AppendArgs p, int roun
     }
     pdl_wait();
     if (tid == 0) {
-        const uint32_t bytes = (uint32_t)(last - first) * 256;
-        mbar_expect_tx(smem_u32(&bar), bytes);
-        bulk_load(smem_u32(ap_rows), static_cast<const T*>(p.d_qkv) + (size_t)token * p.qkv_stride + (size_t)first * 128, bytes, smem_u32(&bar));
+        const T* const row = static_cast<const T*>(p.d_qkv) + (size_t)token * p.qkv_stride;
+        const uint32_t b = smem_u32(&bar), to = smem_u32(ap_rows);
+        mbar_expect_tx(b, (uint32_t)(nq + 2 * nk) * 256);
+        if (nq > 0) bulk_load(to, row + (size_t)q0 * 128, (uint32_t)nq * 256, b);
+        if (nk > 0) bulk_load(to + (uint32_t)nq * 256, row + (size_t)(p.heads + k0) * 128, (uint32_t)nk * 256, b);
+        if (nk > 0) bulk_load(to + (uint32_t)(nq + nk) * 256, row + (size_t)(p.heads + kv + k0) * 128, (uint32_t)nk * 256, b);
     }
     const int slot = p.d_slot[token];
     const int pos = rot > 0 ? p.d_pos[token] : 0;
@@ -234,61 +246,70 @@ rope_kv4_append_kernel(const Qw3Kv4Pool pool, const Qw3Kv4AppendArgs p, int roun
         return;
     }
     if (!known) return;
-    for (int j0 = first + 2 * warp; j0 < last; j0 += AP_GROUPS) {   // the first of the warp's two rows
-        const int j = j0 + (group & 1);   // may be past the last row: the shuffles need every lane
-        const bool is_q = j < p.heads, is_k = !is_q && j < p.heads + kv;
-        const uint4 w = ap_rows[min(j, last - 1) * 16 - first * 16 + l];
-        float2 x[4] = {R::unpack(w.x), R::unpack(w.y), R::unpack(w.z), R::unpack(w.w)};
-        if (rot > 0 && j0 < p.heads + kv) {
-            float2 y[4];
+    // rows j0 .. of a part (0: q, 1: k, 2: v), `n` of them, which begin at row `at` of the shared memory
+    const auto run = [&](auto which, int j0, int n, int at) {
+        constexpr int PART = decltype(which)::value;
+        for (int i0 = 2 * warp; i0 < n; i0 += 2 * AP_WARPS) {
+            const int i = i0 + second, j = j0 + i;
+            const bool there = i < n;   // the shuffles need every lane
+            const uint4 w = ap_rows[(at + (there ? i : i0)) * 16 + l];
+            float2 x[4] = {R::unpack(w.x), R::unpack(w.y), R::unpack(w.z), R::unpack(w.w)};
+            if (PART < 2 && rot > 0) {
+                float2 y[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                y[e] = PAIRS ? make_float2(x[e].y, x[e].x) : make_float2(__shfl_sync(0xffffffffu, x[e].x, mate, 16), __shfl_sync(0xffffffffu, x[e].y, mate, 16));
-            if ((is_q || is_k) && turns) {
+                for (int e = 0; e < 4; ++e)
+                    y[e] = PAIRS ? make_float2(x[e].y, x[e].x) : make_float2(__shfl_sync(0xffffffffu, x[e].x, mate, 16), __shfl_sync(0xffffffffu, x[e].y, mate, 16));
+                if (turns) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)   // scalar products: a packed one would be contracted into the sum
-                    x[e] = add2(make_float2(__fmul_rn(x[e].x, cs[e].x), __fmul_rn(x[e].y, cs[e].y)), make_float2(__fmul_rn(y[e].x, sn[e].x), __fmul_rn(y[e].y, sn[e].y)));
+                    for (int e = 0; e < 4; ++e)   // scalar products: a packed one would be contracted into the sum
+                        x[e] = add2(make_float2(__fmul_rn(x[e].x, cs[e].x), __fmul_rn(x[e].y, cs[e].y)), make_float2(__fmul_rn(y[e].x, sn[e].x), __fmul_rn(y[e].y, sn[e].y)));
+                }
+            }
+            if (PART < 2) {
+                T* const to = static_cast<T*>(PART == 0 ? p.d_q_out : p.d_k_out);
+                if (there && (PART == 0 || to != nullptr))
+                    *reinterpret_cast<uint4*>(to + ((size_t)token * (PART == 0 ? p.heads : kv) + j) * 128 + 8 * l) =
+                        make_uint4(R::pack(x[0].x, x[0].y), R::pack(x[1].x, x[1].y), R::pack(x[2].x, x[2].y), R::pack(x[3].x, x[3].y));
+            }
+            if (PART > 0) {
+                float lo = min_nan(x[0].x, x[0].y), hi = max_nan(x[0].x, x[0].y);
+#pragma unroll
+                for (int e = 1; e < 4; ++e) {
+                    lo = min_nan(lo, min_nan(x[e].x, x[e].y));
+                    hi = max_nan(hi, max_nan(x[e].x, x[e].y));
+                }
+                lo = reduce_half<false>(lo, second);
+                hi = reduce_half<true>(hi, second);
+                // minimum and scale as they are stored: the codes are those of the rounded pair
+                const uint32_t m_bits = R::pack(lo, lo) & 0xffffu;
+                const float m = R::unpack(m_bits).x, range = __fsub_rn(hi, m);
+                float s = R::unpack(R::pack(quotient(make_float2(range, range), 15.0f, 1.0f / 15.0f).x, 0.0f)).x;
+                const bool whole = s <= R::CEIL;   // not with Inf or NaN in the row
+                s = fminf(fmaxf(s, R::FLOOR), R::CEIL);
+                const float inv = __frcp_rn(s);
+                // 1.5 * 2^23 + quotient rounds the quotient to the nearest whole number, ties to even (that they are found is why the quotient
+                // is rounded correctly), and has it in its last bits
+                constexpr float MAGIC = 12582912.0f;
+                uint32_t codes = 0;
+#pragma unroll
+                for (int e = 3; e >= 0; --e) {
+                    const float2 c = add2(quotient(add2(x[e], make_float2(-m, -m)), s, inv), make_float2(MAGIC, MAGIC));
+                    codes = codes * 16u + __float_as_uint(fminf(fmaxf(c.y, MAGIC), MAGIC + 15.0f));
+                    codes = codes * 16u + __float_as_uint(fminf(fmaxf(c.x, MAGIC), MAGIC + 15.0f));
+                }
+                codes -= 0x4b400000u * 0x11111111u;   // eight times the bits of MAGIC
+                if (there && store) {   // a row with Inf or NaN reads back as NaN
+                    uint8_t* const tile = tile0 + (size_t)j * (P / 16) * KV4_TILE_BYTES;
+                    const uint32_t pair = (R::pack(s, 0.0f) & 0xffffu) | (m_bits << 16);
+                    *reinterpret_cast<uint32_t*>(tile + (PART == 1 ? 0 : KV4_V) + r_in * 64 + 4 * l) = whole ? codes : 0u;
+                    if (l == 0) *reinterpret_cast<uint32_t*>(tile + (PART == 1 ? KV4_KP : KV4_VP) + r_in * 4) = whole ? pair : (R::pack(1.0f, 0.0f) & 0xffffu) | 0x7fff0000u;
+                }
             }
         }
-        if (j < rows && (is_q || (is_k && p.d_k_out != nullptr))) {
-            T* const dst = is_q ? static_cast<T*>(p.d_q_out) + ((size_t)token * p.heads + j) * 128
-                                : static_cast<T*>(p.d_k_out) + ((size_t)token * kv + j - p.heads) * 128;
-            *reinterpret_cast<uint4*>(dst + 8 * l) = make_uint4(R::pack(x[0].x, x[0].y), R::pack(x[1].x, x[1].y), R::pack(x[2].x, x[2].y), R::pack(x[3].x, x[3].y));
-        }
-        if (!store || j0 + 1 < p.heads) continue;
-        float lo = min_nan(x[0].x, x[0].y), hi = max_nan(x[0].x, x[0].y);
-#pragma unroll
-        for (int e = 1; e < 4; ++e) {
-            lo = min_nan(lo, min_nan(x[e].x, x[e].y));
-            hi = max_nan(hi, max_nan(x[e].x, x[e].y));
-        }
-        lo = min_nan_over(lo, half);
-        hi = max_nan_over(hi, half);
-        if (is_q || j >= rows) continue;
-        // minimum and scale as they are stored: the codes are those of the rounded pair
-        const uint32_t m_bits = R::pack(lo, lo) & 0xffffu;
-        const float m = R::unpack(m_bits).x, range = __fsub_rn(hi, m);
-        float s = R::unpack(R::pack(quotient(make_float2(range, range), 15.0f, 1.0f / 15.0f).x, 0.0f)).x;
-        const bool whole = s <= R::CEIL;   // not with Inf or NaN in the row
-        s = fmaxf(s, R::FLOOR);
-        const float inv = __frcp_rn(s);
-        // 1.5 * 2^23 + quotient rounds the quotient to the nearest whole number, ties to even (that they are found is why the quotient is
-        // rounded correctly), and has it in its last bits
-        constexpr float MAGIC = 12582912.0f;
-        uint32_t codes = 0;
-#pragma unroll
-        for (int e = 3; e >= 0; --e) {
-            const float2 c = add2(quotient(add2(x[e], make_float2(-m, -m)), s, inv), make_float2(MAGIC, MAGIC));
-            codes = codes * 16u + __float_as_uint(fminf(fmaxf(c.y, MAGIC), MAGIC + 15.0f));
-            codes = codes * 16u + __float_as_uint(fminf(fmaxf(c.x, MAGIC), MAGIC + 15.0f));
-        }
-        codes -= 0x4b400000u * 0x11111111u;   // eight times the bits of MAGIC
-        // a row with Inf or NaN reads back as NaN
-        const uint32_t pair = (R::pack(s, 0.0f) & 0xffffu) | (m_bits << 16);
-        uint8_t* const tile = tile0 + (size_t)(j - p.heads - (is_k ? 0 : kv)) * (P / 16) * KV4_TILE_BYTES;
-        *reinterpret_cast<uint32_t*>(tile + (is_k ? 0 : KV4_V) + r_in * 64 + 4 * l) = whole ? codes : 0u;
-        if (l == 0) *reinterpret_cast<uint32_t*>(tile + (is_k ? KV4_KP : KV4_VP) + r_in * 4) = whole ? pair : (R::pack(1.0f, 0.0f) & 0xffffu) | 0x7fff0000u;
-    }
+    };
+    run(std::integral_constant<int, 0>(), q0, nq, 0);
+    run(std::integral_constant<int, 1>(), k0, nk, nq);
+    run(std::integral_constant<int, 2>(), k0, nk, nq + nk);
 }
 
 // ---- rows read back --------------------------------------------------------------------------------------------------------------
@@ -404,10 +425,10 @@ int qw3_rope_kv4_append(const Qw3Kv4Pool* pool, const Qw3Kv4AppendArgs* a, qw3_w
                 "%s: rows and tables must be 16-byte aligned", who);
     const auto kernel = pool->dtype == QW3_F16 ? (a->layout == QW3_ROPE_PAIRS ? rope_kv4_append_kernel<__half, true> : rope_kv4_append_kernel<__half, false>)
                                                : (a->layout == QW3_ROPE_PAIRS ? rope_kv4_append_kernel<__nv_bfloat16, true> : rope_kv4_append_kernel<__nv_bfloat16, false>);
-    const int rounds = (a->heads + 2 * pool->kv_heads + AP_GROUPS - 1) / AP_GROUPS, parts = (rounds + AP_MAX_ROUNDS - 1) / AP_MAX_ROUNDS;
-    const int each = a->tokens < 2 * ws_struct(ws)->sm_count ? 1 : (rounds + parts - 1) / parts;
-    QW3_CUDA(kv4_launch(kernel, dim3((unsigned)a->tokens, (rounds + each - 1) / each), dim3(AP_THREADS), (size_t)each * AP_GROUPS * 256, static_cast<cudaStream_t>(stream),
-                        ws_pdl(ws), 1, *pool, *a, each, ws_struct(ws)->err));
+    // few tokens: slices of some sixteen rows side by side
+    const int rows = a->heads + 2 * pool->kv_heads, most = a->tokens < 2 * ws_struct(ws)->sm_count ? 16 : AP_MAX_ROWS, slices = (rows + most - 1) / most;
+    const size_t smem = 256 * ((size_t)(a->heads + slices - 1) / slices + 2 * ((size_t)(pool->kv_heads + slices - 1) / slices));
+    QW3_CUDA(kv4_launch(kernel, dim3((unsigned)a->tokens, slices), dim3(AP_THREADS), smem, static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, *pool, *a, ws_struct(ws)->err));
     return QW3_OK;
 }
 
