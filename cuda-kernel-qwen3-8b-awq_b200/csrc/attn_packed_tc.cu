@@ -3,16 +3,19 @@
 //
 // The queries of a sequence are its last rows: row i of nq sees keys 0 .. nk - nq + i.  One CTA takes 256 rows as two tiles of 128.  Where the
 // group's size has a factor `pack` of two, a row is a (token, head) pair of `pack` heads of the group: they read the same keys, so a tile
-// covers 128 / pack tokens, short sequences fill it, and less of the tiles on the diagonal is masked.  Both tiles read the same 64-key tiles of K and V.
+// covers 128 / pack tokens, short sequences fill it, and less of the tiles on the diagonal is masked.  Both tiles read the same tiles of 128 keys.
 // Twelve warps:
-//   warp 0      TMA producer: the q rows once, then K and V tiles (64 keys x 128 dims, two 64-dim halves, 128-byte swizzle)
+//   warp 0      TMA producer: the q rows once, then K and V tiles (128 keys x 128 dims, two 64-dim halves, 128-byte swizzle), five in a ring
 //   warp 1      MMA issuer: S = Q K^T (K-major operands from shared memory), O += P V with P from tensor memory and V MN-major as it lies
 //   warp 2      zeroes the V rows behind the sequence in the last tile: they are other sequences' or nobody's, and 0 * NaN is NaN
 //   warps 4..7, 8..11   one row a thread of the upper / lower tile: S from tensor memory, online softmax, P back in its place
-// Tensor memory, per tile: O 128 columns, two S buffers of 64; P takes 32 columns of the S it comes from, rounded to the rows' type, whose
-// 8 or 11 bits the result has as well; its sum is taken before.  An fp16 P is kept between 2^8 and 2^15 at the row's maximum, so that its
-// normal numbers reach 22 powers of two below.  O is rescaled only when a row's maximum has grown by more than 7 (bf16: 8) powers of two.
-// Bound: 512 cycles of MMAs per 128 x 64 scores beside 512 cycles of exponentials.
+// Tensor memory, per tile: O 128 columns, S 128, of which P takes the upper half as the exponentials consume it: the keys 64..127 first, so that
+// their product runs under the exponentials of the others.  While one tile is in its softmax the tensor cores work for the other.
+// 128 keys a tile: an MMA of 128 x 64 x 16 takes 48 cycles of shared-memory reads for 32 of products (64 keys a tile: 135 us for
+// 4001 rows, 129 with the softmax left out), one of 128 x 128 x 16 64 for 64.
+// P is rounded to the rows' type, whose 8 or 11 bits the result has as well; its sum is taken before.  An fp16 P is kept between 2^8 and
+// 2^15 at the row's maximum, so that its normal numbers reach 22 powers of two below.  O is rescaled only when a row's maximum has grown by
+// more than 7 (bf16: 8) powers of two.
 // All waits are bounded.  After one that gives up the error word is set, rows that are not finished are written as NaN, and the CTA
 // leaves when its copies and MMAs in flight are done.
 #include <atomic>
@@ -22,11 +25,11 @@
 
 namespace qw3 {
 
-constexpr int PK_ROWS = 128, PK_KEYS = 64, PK_STAGES = 4;
+constexpr int PK_ROWS = 128, PK_KEYS = 128, PK_STAGES = 5;
 constexpr int PK_THREADS = 384;
 constexpr int PK_Q_BYTES = PK_ROWS * 256;   // one tile of q rows: two halves of 64 dims
 constexpr int PK_KV_BYTES = PK_KEYS * 256;  // one tile of K or V
-constexpr size_t PK_SMEM = 2 * PK_Q_BYTES + 2 * (size_t)PK_STAGES * PK_KV_BYTES + 512;
+constexpr size_t PK_SMEM = 2 * PK_Q_BYTES + (size_t)PK_STAGES * PK_KV_BYTES + 512;
 
 __device__ __forceinline__ float pk_ex2(float x) {
     float r;
@@ -95,13 +98,11 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     constexpr bool HALF = R::FLOOR > 1e-9f;                        // fp16
     constexpr float SHIFT = HALF ? 8.0f : 0.0f, LAG = HALF ? 7.0f : 8.0f;
     uint8_t* q_s = smem;
-    uint8_t* k_s = q_s + 2 * PK_Q_BYTES;
-    uint8_t* v_s = k_s + PK_STAGES * PK_KV_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(v_s + PK_STAGES * PK_KV_BYTES);
-    const uint32_t q_full = smem_u32(bars), k_full = q_full + 8, v_full = k_full + 8 * PK_STAGES, k_empty = v_full + 8 * PK_STAGES,
-                   v_empty = k_empty + 8 * PK_STAGES, s_full = v_empty + 8 * PK_STAGES /* [tile][buffer] */, p_full = s_full + 32,
-                   pv_done = p_full + 32 /* [tile][buffer] */, drain = pv_done + 32, v_last = drain + 8, v_clean = v_last + 8;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 + 4 * PK_STAGES + 12);
+    uint8_t* kv_s = q_s + 2 * PK_Q_BYTES;   // tile 2j of the ring is K of key tile j, tile 2j + 1 V
+    uint64_t* bars = reinterpret_cast<uint64_t*>(kv_s + PK_STAGES * PK_KV_BYTES);
+    const uint32_t q_full = smem_u32(bars), full = q_full + 8, empty = full + 8 * PK_STAGES, s_full = empty + 8 * PK_STAGES /* [tile] */,
+                   p_full = s_full + 16 /* [tile][half] */, o_full = p_full + 32 /* [tile] */, drain = o_full + 16, v_last = drain + 8, v_clean = v_last + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * PK_STAGES + 12);
     volatile int* s_dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const auto give_up = [&](int code) {
@@ -157,16 +158,14 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         mbar_init(v_last, 1);
         mbar_init(v_clean, 1);
         for (int s = 0; s < PK_STAGES; ++s) {
-            mbar_init(k_full + 8 * s, 1);
-            mbar_init(v_full + 8 * s, 1);
-            mbar_init(k_empty + 8 * s, 1);
-            mbar_init(v_empty + 8 * s, 1);
+            mbar_init(full + 8 * s, 1);
+            mbar_init(empty + 8 * s, 1);
         }
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + 8 * i, 1);
-            mbar_init(p_full + 8 * i, 4);   // the four warps of the tile
-            mbar_init(pv_done + 8 * i, 1);
+            mbar_init(o_full + 8 * i, 1);
         }
+        for (int i = 0; i < 4; ++i) mbar_init(p_full + 8 * i, 4);   // the four warps of the tile
         *s_dead = 0;
         mbar_fence_init();
     }
@@ -183,7 +182,8 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         return;
     }
     const int n_tiles = (n_keys + PK_KEYS - 1) / PK_KEYS;
-    const bool ragged = n_keys % PK_KEYS != 0;
+    const bool short_last = n_keys - (n_tiles - 1) * PK_KEYS <= PK_KEYS / 2;   // of the last tile only the first half has keys
+    const bool ragged = n_keys % (PK_KEYS / 2) != 0;
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -191,7 +191,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;   // O of the tiles at columns 0 and 128, S at 256 + 128 tile + 64 buffer
+    const uint32_t tmem = *tmem_slot;   // O of the tiles at columns 0 and 128, S at 256 + 128 tile, P at 64 columns of that + 32 half
 
     if (warp == 0) {
         if (elect_one()) {
@@ -201,39 +201,26 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             for (int t = 0; t < 2; ++t)
                 for (int h = 0; h < 2; ++h)
                     tma_load_3d(smem_u32(q_s + t * PK_Q_BYTES + h * (PK_Q_BYTES / 2)), &tm_q, 64 * h, head0, seq_q0 + t0 + tile_tokens * t, q_full);
-            int j = 0, kv = 0;
-            for (; j < n_tiles; ++j) {
-                const int s = j % PK_STAGES;
-                const uint32_t lap = (uint32_t)(j / PK_STAGES);
-                for (kv = 0; kv < 2; ++kv) {
-                    const uint32_t full = (kv ? v_full : k_full) + 8 * s, empty = (kv ? v_empty : k_empty) + 8 * s;
-                    uint8_t* dst = (kv ? v_s : k_s) + s * PK_KV_BYTES;
-                    if (lap > 0) ok = mbar_wait(empty, (lap - 1) & 1u);
-                    if (*s_dead != 0) ok = false;
-                    if (!ok) break;
-                    mbar_expect_tx(full, PK_KV_BYTES);
-                    for (int h = 0; h < 2; ++h)
-                        tma_load_3d(smem_u32(dst + h * (PK_KV_BYTES / 2)), kv ? &tm_v : &tm_k, 64 * h, seq_k0 + j * PK_KEYS, kv_head, full);
-                }
+            int i = 0;
+            for (; i < 2 * n_tiles; ++i) {
+                const int s = i % PK_STAGES, j = i / 2, v = i & 1;
+                if (i >= PK_STAGES) ok = mbar_wait(empty + 8 * s, (uint32_t)(i / PK_STAGES - 1) & 1u);
+                if (*s_dead != 0) ok = false;
                 if (!ok) break;
+                mbar_expect_tx(full + 8 * s, PK_KV_BYTES);
+                for (int h = 0; h < 2; ++h)
+                    tma_load_3d(smem_u32(kv_s + s * PK_KV_BYTES + h * (PK_KV_BYTES / 2)), v ? &tm_v : &tm_k, 64 * h, seq_k0 + j * PK_KEYS, kv_head, full + 8 * s);
             }
             if (ok && ragged) {   // this thread knows the lap that the barrier is in; warp 2 does not
-                ok = mbar_wait(v_full + 8 * ((n_tiles - 1) % PK_STAGES), (uint32_t)((n_tiles - 1) / PK_STAGES) & 1u);
+                ok = mbar_wait(full + 8 * ((2 * n_tiles - 1) % PK_STAGES), (uint32_t)((2 * n_tiles - 1) / PK_STAGES) & 1u);
                 mbar_arrive(v_last);
             }
             // drain: the last release arrivals land before the CTA may leave
-            for (int i = n_tiles < PK_STAGES ? 0 : n_tiles - PK_STAGES; i < n_tiles && ok; ++i) {
-                const uint32_t parity = (uint32_t)(i / PK_STAGES) & 1u;
-                ok = mbar_wait(k_empty + 8 * (i % PK_STAGES), parity) && mbar_wait(v_empty + 8 * (i % PK_STAGES), parity);
-            }
+            for (int k = max(2 * n_tiles - PK_STAGES, 0); k < 2 * n_tiles && ok; ++k) ok = mbar_wait(empty + 8 * (k % PK_STAGES), (uint32_t)(k / PK_STAGES) & 1u);
             if (!ok) {
                 give_up(0x30041);
                 mbar_wait(q_full, 0);   // the copies in flight
-                for (int t = 0; t < 2; ++t) {
-                    const int asked = j < n_tiles && t < kv ? j + 1 : j;   // tiles of K, of V
-                    for (int i = max(asked - PK_STAGES, 0); i < asked; ++i)
-                        mbar_wait((t ? v_full : k_full) + 8 * (i % PK_STAGES), (uint32_t)(i / PK_STAGES) & 1u);
-                }
+                for (int k = max(i - PK_STAGES, 0); k < i; ++k) mbar_wait(full + 8 * (k % PK_STAGES), (uint32_t)(k / PK_STAGES) & 1u);
             }
         }
         __syncwarp();
@@ -241,48 +228,53 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         if (elect_one()) {
             // D = f32, A and B of the rows' type.  S: N = 64 keys, both K-major.  P V: N = 128 dims, V MN-major (bit 16).
             const uint32_t types = (1u << 4) | (HALF ? 0u : (1u << 7) | (1u << 10));
-            const uint32_t idesc_s = types | ((uint32_t)(PK_KEYS >> 3) << 17) | ((uint32_t)(PK_ROWS >> 4) << 24);
-            const uint32_t idesc_o = types | (1u << 16) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(PK_ROWS >> 4) << 24);
-            const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024), kd = make_smem_desc(smem_u32(k_s), 16, 1024);
-            const uint64_t vd = make_smem_desc(smem_u32(v_s), PK_KV_BYTES / 2, 1024);   // 64-dim halves, 8-key groups
-            auto scores = [&](int t, int j) {   // S of tile t against key tile j
-                const uint32_t d = tmem + 256 + 128 * t + 64 * (j & 1);
-                const uint64_t a = qd + (uint64_t)(t * (PK_Q_BYTES >> 4)), b = kd + (uint64_t)((j % PK_STAGES) * (PK_KV_BYTES >> 4));
+            const uint32_t rows = (uint32_t)(PK_ROWS >> 4) << 24, idesc_o = types | (1u << 16) | ((uint32_t)(128 >> 3) << 17) | rows;
+            const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024), kd = make_smem_desc(smem_u32(kv_s), 16, 1024);
+            const uint64_t vd = make_smem_desc(smem_u32(kv_s), PK_KV_BYTES / 2, 1024);   // 64-dim halves, 8-key groups
+            const auto scores = [&](int t, int j) {   // S of tile t against key tile j
+                const int s = 2 * j % PK_STAGES;
+                const uint32_t keys = j == n_tiles - 1 && short_last ? PK_KEYS / 2 : PK_KEYS, idesc = types | (keys >> 3) << 17 | rows;
+                const uint64_t a = qd + (uint64_t)(t * (PK_Q_BYTES >> 4)), b = kd + (uint64_t)(s * (PK_KV_BYTES >> 4));
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks)
-                    umma_f16(d, a + (uint64_t)((ks >> 2) * (PK_Q_BYTES >> 5) + (ks & 3) * 2), b + (uint64_t)((ks >> 2) * (PK_KV_BYTES >> 5) + (ks & 3) * 2),
-                             idesc_s, ks > 0 ? 1u : 0u);
-                umma_commit(s_full + 16 * t + 8 * (j & 1));
+                    umma_f16(tmem + 256 + 128 * t, a + (uint64_t)((ks >> 2) * (PK_Q_BYTES >> 5) + (ks & 3) * 2),
+                             b + (uint64_t)((ks >> 2) * (PK_KV_BYTES >> 5) + (ks & 3) * 2), idesc, ks > 0 ? 1u : 0u);
+                umma_commit(s_full + 8 * t);
+                if (t == 1) umma_commit(empty + 8 * s);
             };
-            bool ok = mbar_wait(q_full, 0);
-            for (int j = 0; j < 2 && j < n_tiles && ok; ++j) {
-                ok = mbar_wait(k_full + 8 * j, 0);
-                if (!ok) break;
-                scores(0, j);
-                scores(1, j);
-                umma_commit(k_empty + 8 * j);
+            const auto products = [&](int t, int j, int half, bool first) {   // O of tile t += P V of 64 keys
+                const uint64_t v = vd + (uint64_t)((2 * j + 1) % PK_STAGES * (PK_KV_BYTES >> 4) + half * (64 * 128 >> 4));
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+                    umma_f16_ts(tmem + 128 * t, tmem + 256 + 128 * t + 64 + 32 * half + 8 * ks, v + (uint64_t)(ks * (2048 >> 4)), idesc_o, first && ks == 0 ? 0u : 1u);
+            };
+            bool ok = mbar_wait(q_full, 0) && mbar_wait(full, 0);
+            if (ok) {
+                scores(0, 0);
+                scores(1, 0);
             }
             for (int j = 0; j < n_tiles && ok; ++j) {
-                const int s = j % PK_STAGES, b = j & 1;
-                ok = *s_dead == 0 && (j == n_tiles - 1 && ragged ? mbar_wait(v_clean, 0) : mbar_wait(v_full + 8 * s, (uint32_t)(j / PK_STAGES) & 1u));
+                const int iv = 2 * j + 1, ik = 2 * j + 2;   // tiles of the ring
+                const bool last = j == n_tiles - 1, both = !last || !short_last;
+                ok = *s_dead == 0 && (last && ragged ? mbar_wait(v_clean, 0) : mbar_wait(full + 8 * (iv % PK_STAGES), (uint32_t)(iv / PK_STAGES) & 1u));
                 for (int t = 0; t < 2 && ok; ++t) {
-                    ok = mbar_wait(p_full + 16 * t + 8 * b, (uint32_t)(j >> 1) & 1u);
+                    if (both) {
+                        ok = mbar_wait(p_full + 16 * t + 8, (uint32_t)j & 1u);
+                        if (!ok) break;
+                        tc_fence_after();
+                        products(t, j, 1, j == 0);
+                    }
+                    ok = mbar_wait(p_full + 16 * t, (uint32_t)j & 1u);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t a = tmem + 256 + 128 * t + 64 * b;
-                    const uint64_t v = vd + (uint64_t)(s * (PK_KV_BYTES >> 4));
-#pragma unroll
-                    for (int ks = 0; ks < PK_KEYS / 16; ++ks)
-                        umma_f16_ts(tmem + 128 * t, a + 8 * ks, v + (uint64_t)(ks * (2048 >> 4)), idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
-                    umma_commit(pv_done + 16 * t + 8 * b);
-                    if (t == 1) umma_commit(v_empty + 8 * s);
-                    // the next scores of the buffer: issued after, and so executed after, the product that reads P there
-                    if (j + 2 < n_tiles) {
-                        const int s2 = (j + 2) % PK_STAGES;
-                        if (t == 0) ok = mbar_wait(k_full + 8 * s2, (uint32_t)((j + 2) / PK_STAGES) & 1u);
+                    products(t, j, 0, j == 0 && !both);
+                    if (last) umma_commit(o_full + 8 * t);
+                    if (t == 1) umma_commit(empty + 8 * (iv % PK_STAGES));
+                    // the next scores: issued after, and so executed after, the products that read P there
+                    if (!last) {
+                        if (t == 0) ok = mbar_wait(full + 8 * (ik % PK_STAGES), (uint32_t)(ik / PK_STAGES) & 1u);
                         if (!ok) break;
-                        scores(t, j + 2);
-                        if (t == 1) umma_commit(k_empty + 8 * s2);
+                        scores(t, j + 1);
                     }
                 }
             }
@@ -295,12 +287,13 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         __syncwarp();
     } else if (warp == 2) {
         if (ragged) {
-            const int s = (n_tiles - 1) % PK_STAGES, from = n_keys % PK_KEYS;
+            uint8_t* const tile = kv_s + (2 * n_tiles - 1) % PK_STAGES * PK_KV_BYTES;
+            const int from = n_keys - (n_tiles - 1) * PK_KEYS, n = (short_last ? PK_KEYS / 2 : PK_KEYS) - from;
             const bool ok = __all_sync(0xffffffffu, mbar_wait(v_last, 0));
             if (ok) {
-                for (int i = lane; i < (PK_KEYS - from) * 16; i += 32) {   // rows of 128 bytes in either half
-                    const int h = i / ((PK_KEYS - from) * 8), in = i - h * (PK_KEYS - from) * 8;
-                    *reinterpret_cast<uint4*>(v_s + s * PK_KV_BYTES + h * (PK_KV_BYTES / 2) + from * 128 + in * 16) = make_uint4(0, 0, 0, 0);
+                for (int i = lane; i < n * 16; i += 32) {   // rows of 128 bytes in either half
+                    const int h = i / (n * 8), in = i - h * n * 8;
+                    *reinterpret_cast<uint4*>(tile + h * (PK_KV_BYTES / 2) + from * 128 + in * 16) = make_uint4(0, 0, 0, 0);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             } else if (lane == 0) {
@@ -312,7 +305,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     } else if (warp >= 4) {
         const int t = (warp - 4) >> 2, q = warp & 3;
         const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16);
-        const uint32_t o_at = lane_base + 128 * t, s_at = lane_base + 256 + 128 * t;
+        const uint32_t o_at = lane_base + 128 * t, s_at = lane_base + 256 + 128 * t, p_at = s_at + 64;
         const int row = 32 * q + lane, token = tile_tokens * t + row / pack;   // of the block
         const int pos = min(past + t0 + token, n_keys - 1);                    // last key the row sees
         const int pos_first = min(past + t0 + tile_tokens * t + 32 * q / pack, n_keys - 1);   // of the warp's first row
@@ -321,36 +314,70 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         float oh = -SHIFT, ol = 0.0f;            // P = 2^(s c - oh - ol)
         bool large = false;                      // m c has no fraction left in fp32: then oh = m c, ol its rounding error, and m is taken off s first
         bool ok = true;
+        float2 s[32];
+        const auto load = [&](int half, int k0) {   // scores of 64 keys from k0 on
+            tmem_ld32(s_at + 64 * half, reinterpret_cast<uint32_t*>(s));
+            tmem_ld32(s_at + 64 * half + 32, reinterpret_cast<uint32_t*>(s) + 32);
+            tmem_wait_ld();
+            if (k0 + 63 > pos_first) {   // some row of the warp does not see all of them
+#pragma unroll
+                for (int e = 0; e < 32; ++e) s[e] = make_float2(k0 + 2 * e <= pos ? s[e].x : -INFINITY, k0 + 2 * e + 1 <= pos ? s[e].y : -INFINITY);
+            }
+        };
+        const auto largest = [&] {
+            float mx[4] = {s[0].x, s[0].y, s[1].x, s[1].y};
+#pragma unroll
+            for (int e = 2; e < 32; ++e) {
+                mx[2 * (e & 1)] = fmaxf(mx[2 * (e & 1)], s[e].x);
+                mx[2 * (e & 1) + 1] = fmaxf(mx[2 * (e & 1) + 1], s[e].y);
+            }
+            return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        };
+        const auto exponentials = [&](int half) {
+            if (__any_sync(0xffffffffu, large)) {
+                const float base = large ? m : 0.0f;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) s[e] = make_float2(s[e].x - base, s[e].y - base);
+            }
+            const float off = large ? -SHIFT : oh;
+            const float2 c2 = make_float2(c, c), off2 = make_float2(-off, -off);
+            float2 ls[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float2 x = fma2(s[16 * h + e], c2, off2), a = make_float2(pk_ex2(x.x), pk_ex2(x.y));
+                    ls[e & 1] = add2(ls[e & 1], a);
+                    w[e] = R::pack(a.x, a.y);
+                }
+                tmem_st16(p_at + 32 * half + 16 * h, w);
+            }
+            l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 16 * t + 8 * half);
+        };
         for (int j = 0; j < n_tiles && ok; ++j) {
-            const int b = j & 1;
-            ok = __all_sync(0xffffffffu, *s_dead == 0 && mbar_wait(s_full + 16 * t + 8 * b, (uint32_t)(j >> 1) & 1u));
+            const bool both = j < n_tiles - 1 || !short_last;
+            const int k0 = j * PK_KEYS;
+            // the scores, and with them the products of the tile before, which were issued earlier
+            ok = __all_sync(0xffffffffu, *s_dead == 0 && mbar_wait(s_full + 8 * t, (uint32_t)j & 1u));
             if (!ok) break;
             tc_fence_after();
-            uint32_t sr[64];
-            float s[64];
-            tmem_ld32(s_at + 64 * b, sr);
-            tmem_ld32(s_at + 64 * b + 32, sr + 32);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 64; ++e) s[e] = __uint_as_float(sr[e]);
-            const int k0 = j * PK_KEYS;
-            if (k0 + PK_KEYS - 1 > pos_first) {   // some row of the warp does not see the whole tile
-#pragma unroll
-                for (int e = 0; e < 64; ++e) s[e] = k0 + e <= pos ? s[e] : -INFINITY;
+            load(0, k0);
+            float mt = largest();
+            if (both) {
+                load(1, k0 + 64);
+                mt = fmaxf(mt, largest());
             }
-            float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-            for (int e = 4; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
-            const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             if (__any_sync(0xffffffffu, (mt - m) * c > LAG || large)) {   // rare after the first tile
                 const float mn = fmaxf(m, mt), mc = mn == -INFINITY ? 0.0f : mn * c;
                 const bool nl = fabsf(mc) >= 1048576.0f;
                 const float nh = nl ? mc : mc - SHIFT, nlow = nl ? fmaf(mn, c, -mc) - SHIFT : 0.0f;
                 const float f = m == -INFINITY ? 0.0f : pk_ex2((oh - nh) + (ol - nlow));
                 if (j > 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(pv_done + 16 * t + 8 * (b ^ 1), (uint32_t)((j - 1) >> 1) & 1u));
-                    if (!ok) break;
-                    tc_fence_after();
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
                         uint32_t o[32];
@@ -366,34 +393,14 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 oh = nh;
                 ol = nlow;
                 large = nl;
-                if (__any_sync(0xffffffffu, large)) {
-                    const float base = large ? m : 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 64; ++e) s[e] -= base;
-                }
             }
-            const float off = large ? -SHIFT : oh;
-            float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t w[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float a0 = pk_ex2(fmaf(s[32 * h + 2 * e], c, -off)), a1 = pk_ex2(fmaf(s[32 * h + 2 * e + 1], c, -off));
-                    ls[(2 * e) & 3] += a0;
-                    ls[(2 * e + 1) & 3] += a1;
-                    w[e] = R::pack(a0, a1);
-                }
-                tmem_st16(s_at + 64 * b + 16 * h, w);
+            if (both) {
+                exponentials(1);
+                load(0, k0);
             }
-            l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full + 16 * t + 8 * b);
+            exponentials(0);
         }
-        for (int j = n_tiles < 2 ? 0 : n_tiles - 2; j < n_tiles && ok; ++j)
-            ok = __all_sync(0xffffffffu, mbar_wait(pv_done + 16 * t + 8 * (j & 1), (uint32_t)(j >> 1) & 1u));
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(o_full + 8 * t, 0));
         if (!ok && lane == 0) give_up(0x30043);
         __syncwarp();
         tc_fence_after();
