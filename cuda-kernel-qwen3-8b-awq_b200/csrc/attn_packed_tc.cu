@@ -37,6 +37,24 @@ __device__ __forceinline__ float pk_ex2(float x) {
     return r;
 }
 
+// 2^x for two x up to 30, on the FMA pipe: the exponential unit (16 results a clock and SM) is what the softmax waits for.  x = n + f with n the
+// nearest whole number, which 1.5 * 2^23 + x has in its last bits; 2^f by a polynomial of degree 4 that is 1 at 0 (minimax on [-1/2, 1/2] by
+// Remez' exchange: relative error 3.6e-6); n is added to the exponent.  Below -127, -Inf included, exactly 0.
+__device__ __forceinline__ float2 pk_ex2_fma(float2 x) {
+    constexpr float MAGIC = 12582912.0f;
+    x = make_float2(fmaxf(x.x, -127.0f), fmaxf(x.y, -127.0f));
+    const float2 t = add2(x, make_float2(MAGIC, MAGIC)), n = add2(t, make_float2(-MAGIC, -MAGIC)), f = add2(x, make_float2(-n.x, -n.y));
+    float2 p = fma2(make_float2(0.009782911186619846f, 0.009782911186619846f), f, make_float2(0.055976883149044095f, 0.055976883149044095f));
+    p = fma2(p, f, make_float2(0.24020711100517408f, 0.24020711100517408f));
+    p = fma2(p, f, make_float2(0.693113604482677f, 0.693113604482677f));
+    p = fma2(p, f, make_float2(1.0f, 1.0f));
+    return make_float2(__uint_as_float(__float_as_uint(t.x) * 8388608u + __float_as_uint(p.x)), __uint_as_float(__float_as_uint(t.y) * 8388608u + __float_as_uint(p.y)));
+}
+
+#ifndef POLYN
+#define POLYN 4
+#endif
+constexpr int PK_FMA = POLYN;   // of sixteen pairs of exponentials, those on the FMA pipe
 struct PackedParams {
     Qw3AttnPackedArgs a;
     float c;        // scale * log2(e)
@@ -347,7 +365,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 uint32_t w[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float2 x = fma2(s[16 * h + e], c2, off2), a = make_float2(pk_ex2(x.x), pk_ex2(x.y));
+                    const float2 x = fma2(s[16 * h + e], c2, off2), a = (e * PK_FMA) % 16 + PK_FMA >= 16 + (PK_FMA == 0) ? pk_ex2_fma(x) : make_float2(pk_ex2(x.x), pk_ex2(x.y));
                     ls[e & 1] = add2(ls[e & 1], a);
                     w[e] = R::pack(a.x, a.y);
                 }
