@@ -4,8 +4,11 @@
 // The queries of a sequence are its last rows: row i of nq sees keys 0 .. nk - nq + i.  One CTA takes 256 rows as two tiles of 128.  Where the
 // group's size has a factor `pack` of two, a row is a (token, head) pair of `pack` heads of the group: they read the same keys, so a tile
 // covers 128 / pack tokens, short sequences fill it, and less of the tiles on the diagonal is masked.  Both tiles read the same tiles of 128 keys.
+// One CTA an SM, which takes block after block (256 rows of a sequence and a group) from a counter, the blocks with the most keys of a
+// sequence first, so that the loads, the first scores and the next block's place are on their way during a block's epilogue.
 // Twelve warps:
-//   warp 0      TMA producer: the q rows once, then K and V tiles (128 keys x 128 dims, two 64-dim halves, 128-byte swizzle), five in a ring
+//   warp 0      takes and finds the blocks; TMA producer: the q rows, K and V tiles (128 keys x 128 dims, two 64-dim halves, 128-byte
+//               swizzle), five in a ring
 //   warp 1      MMA issuer: S = Q K^T (K-major operands from shared memory), O += P V with P from tensor memory and V MN-major as it lies
 //   warp 2      zeroes the V rows behind the sequence in the last tile: they are other sequences' or nobody's, and 0 * NaN is NaN
 //   warps 4..7, 8..11   one row a thread of the upper / lower tile: S from tensor memory, online softmax, P back in its place
@@ -51,15 +54,19 @@ __device__ __forceinline__ float2 pk_ex2_fma(float2 x) {
     return make_float2(__uint_as_float(__float_as_uint(t.x) * 8388608u + __float_as_uint(p.x)), __uint_as_float(__float_as_uint(t.y) * 8388608u + __float_as_uint(p.y)));
 }
 
-#ifndef POLYN
-#define POLYN 4
-#endif
-constexpr int PK_FMA = POLYN;   // of sixteen pairs of exponentials, those on the FMA pipe
+constexpr int PK_FMA = 4;   // of sixteen pairs of exponentials, those on the FMA pipe
 struct PackedParams {
     Qw3AttnPackedArgs a;
     float c;        // scale * log2(e)
     int pack;       // heads that share a tile
+    int* ticket;    // the next block to be taken, and the CTAs that are done; zero between launches
+    int* done;
     int* err;
+};
+// A block of rows: its sequence's first row and number of rows in q and in k, its number in the sequence (below 0: no more blocks), and
+// its first head.
+struct PackedBlock {
+    int q0, k0, nq, nk, block, head0;
 };
 
 // One row by a warp, from global memory and in 32-bit arithmetic: rows whose tile holds Inf or NaN in V behind the row.  The tensor
@@ -110,17 +117,18 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
 attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                    const PackedParams p) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ int s_place[4];   // the CTA's sequence: first row of q and of k, rows of q, of k; and its block of rows
-    __shared__ int s_block;
+    __shared__ PackedBlock s_block[2];
     using R = RowType<T>;
     constexpr bool HALF = R::FLOOR > 1e-9f;                        // fp16
     constexpr float SHIFT = HALF ? 8.0f : 0.0f, LAG = HALF ? 7.0f : 8.0f;
     uint8_t* q_s = smem;
-    uint8_t* kv_s = q_s + 2 * PK_Q_BYTES;   // tile 2j of the ring is K of key tile j, tile 2j + 1 V
+    uint8_t* kv_s = q_s + 2 * PK_Q_BYTES;   // a ring: K of a key tile, V of it, K of the next, ..
     uint64_t* bars = reinterpret_cast<uint64_t*>(kv_s + PK_STAGES * PK_KV_BYTES);
-    const uint32_t q_full = smem_u32(bars), full = q_full + 8, empty = full + 8 * PK_STAGES, s_full = empty + 8 * PK_STAGES /* [tile] */,
-                   p_full = s_full + 16 /* [tile][half] */, o_full = p_full + 32 /* [tile] */, drain = o_full + 16, v_last = drain + 8, v_clean = v_last + 8;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * PK_STAGES + 12);
+    // phases: of a block: q_*, o_* [tile]; of a key tile: s_full, p_full [tile][half]; of every second block: place_* [block & 1]
+    const uint32_t q_full = smem_u32(bars), q_empty = q_full + 8, full = q_empty + 8, empty = full + 8 * PK_STAGES, s_full = empty + 8 * PK_STAGES,
+                   p_full = s_full + 16, o_full = p_full + 32, o_empty = o_full + 16, place_full = o_empty + 16, place_empty = place_full + 16,
+                   drain = place_empty + 16, v_last = drain + 8, v_clean = v_last + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * PK_STAGES + 19);
     volatile int* s_dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const auto give_up = [&](int code) {
@@ -130,48 +138,11 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
     const int pack = p.pack, block_tokens = 2 * PK_ROWS / pack, tile_tokens = PK_ROWS / pack;
     const int groups = p.a.heads / pack;
-    const int head0 = (int)(blockIdx.x % groups) * pack;
     pdl_launch_dependents();
-    pdl_wait();
 
-    // the block of rows: the last sequence's last block comes first (the blocks with the most keys of a sequence start first)
-    if (warp == 0) {
-        int left = (int)(blockIdx.x / groups), found = -1;
-        for (int b0 = p.a.n_seq; b0 > 0 && found < 0; b0 -= 32) {
-            const int b = b0 - 1 - lane;
-            int q0 = 0, nq = 0, k0 = 0, nk = 0, bad = 0;
-            if (b >= 0) {
-                const int qa = p.a.d_cu_q[b], qb = p.a.d_cu_q[b + 1], ka = p.a.d_cu_k[b], kb = p.a.d_cu_k[b + 1];
-                bad = qa < 0 || qb < qa || (long long)qb > p.a.q_rows || ka < 0 || kb < ka || (long long)kb > p.a.k_rows;
-                if (!bad) { q0 = qa; nq = qb - qa; k0 = ka; nk = kb - ka; }
-            }
-            const int blocks = (nq + block_tokens - 1) / block_tokens;
-            int sum = blocks;
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const int x = __shfl_up_sync(0xffffffffu, sum, d);
-                if (lane >= d) sum += x;
-            }
-            const uint32_t hit = __ballot_sync(0xffffffffu, left < sum);
-            if (hit != 0) {
-                found = __ffs(hit) - 1;
-                if (lane == found) {
-                    s_place[0] = q0; s_place[1] = k0; s_place[2] = nq; s_place[3] = nk;
-                    s_block = blocks - 1 - (left - (sum - blocks));
-                }
-            }
-            left -= __shfl_sync(0xffffffffu, sum, 31);
-        }
-        if (found < 0 && lane == 0) s_block = -1;
-        // CTA 0 looks at all sequences, for their reports
-        if (blockIdx.x == 0)
-            for (int b = lane; b < p.a.n_seq; b += 32) {
-                const int qa = p.a.d_cu_q[b], qb = p.a.d_cu_q[b + 1], ka = p.a.d_cu_k[b], kb = p.a.d_cu_k[b + 1];
-                if (qa < 0 || qb < qa || (long long)qb > p.a.q_rows || ka < 0 || kb < ka || (long long)kb > p.a.k_rows) kv4_error(p.err, KV4_ERR_PACKED_CU);
-            }
-    }
     if (tid == 0) {
         mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
         mbar_init(drain, 1);
         mbar_init(v_last, 1);
         mbar_init(v_clean, 1);
@@ -182,26 +153,14 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + 8 * i, 1);
             mbar_init(o_full + 8 * i, 1);
+            mbar_init(o_empty + 8 * i, 4);   // the four warps of the tile
+            mbar_init(place_full + 8 * i, 1);
+            mbar_init(place_empty + 8 * i, 10);   // warps 1, 2 and the eight of the softmax
         }
-        for (int i = 0; i < 4; ++i) mbar_init(p_full + 8 * i, 4);   // the four warps of the tile
+        for (int i = 0; i < 4; ++i) mbar_init(p_full + 8 * i, 4);
         *s_dead = 0;
         mbar_fence_init();
     }
-    __syncthreads();
-    if (s_block < 0) return;
-    const int seq_q0 = s_place[0], seq_k0 = s_place[1], nq = s_place[2], nk = s_place[3];
-    const int t0 = s_block * block_tokens, past = nk - nq;   // token i of the block is t0 + i; it sees keys 0 .. past + t0 + i
-    const int n_keys = min(nk, past + min(t0 + block_tokens, nq));
-    T* const out = static_cast<T*>(p.a.d_out) + (size_t)(seq_q0 + t0) * p.a.heads * 128 + (size_t)head0 * 128;
-    if (n_keys <= 0) {   // no row of the block sees a key
-        const int rows = min(block_tokens, nq - t0) * pack;
-        for (int i = tid; i < rows * 16; i += PK_THREADS)
-            reinterpret_cast<uint4*>(out + ((size_t)(i / 16 / pack) * p.a.heads + i / 16 % pack) * 128)[i & 15] = make_uint4(0, 0, 0, 0);
-        return;
-    }
-    const int n_tiles = (n_keys + PK_KEYS - 1) / PK_KEYS;
-    const bool short_last = n_keys - (n_tiles - 1) * PK_KEYS <= PK_KEYS / 2;   // of the last tile only the first half has keys
-    const bool ragged = n_keys % (PK_KEYS / 2) != 0;
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -210,48 +169,129 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;   // O of the tiles at columns 0 and 128, S at 256 + 128 tile, P at 64 columns of that + 32 half
+    pdl_wait();
+
+    // what follows from a block's place
+    struct Shape {
+        int t0, past, n_keys, n_tiles;   // token i of the block is t0 + i of the sequence's queries; it sees keys 0 .. past + t0 + i
+        bool short_last, ragged;         // of the last key tile only the first half has keys; its V has rows that are not the sequence's
+    };
+    const auto shape_of = [&](const PackedBlock& b) {
+        Shape s;
+        s.t0 = b.block * block_tokens;
+        s.past = b.nk - b.nq;
+        s.n_keys = max(0, min(b.nk, s.past + min(s.t0 + block_tokens, b.nq)));
+        s.n_tiles = (s.n_keys + PK_KEYS - 1) / PK_KEYS;
+        s.short_last = s.n_keys - (s.n_tiles - 1) * PK_KEYS <= PK_KEYS / 2;
+        s.ragged = s.n_keys % (PK_KEYS / 2) != 0;
+        return s;
+    };
 
     if (warp == 0) {
-        if (elect_one()) {
-            bool ok = true;
-            const int kv_head = head0 / (p.a.heads / p.a.kv_heads);
-            mbar_expect_tx(q_full, 2 * PK_Q_BYTES);
-            for (int t = 0; t < 2; ++t)
-                for (int h = 0; h < 2; ++h)
-                    tma_load_3d(smem_u32(q_s + t * PK_Q_BYTES + h * (PK_Q_BYTES / 2)), &tm_q, 64 * h, head0, seq_q0 + t0 + tile_tokens * t, q_full);
-            int i = 0;
-            for (; i < 2 * n_tiles; ++i) {
-                const int s = i % PK_STAGES, j = i / 2, v = i & 1;
-                if (i >= PK_STAGES) ok = mbar_wait(empty + 8 * s, (uint32_t)(i / PK_STAGES - 1) & 1u);
-                if (*s_dead != 0) ok = false;
-                if (!ok) break;
-                mbar_expect_tx(full + 8 * s, PK_KV_BYTES);
-                for (int h = 0; h < 2; ++h)
-                    tma_load_3d(smem_u32(kv_s + s * PK_KV_BYTES + h * (PK_KV_BYTES / 2)), v ? &tm_v : &tm_k, 64 * h, seq_k0 + j * PK_KEYS, kv_head, full + 8 * s);
+        int i = 0, used = 0;   // tiles asked for, blocks with keys
+        for (int k = 0;; ++k) {
+            PackedBlock b = {0, 0, 0, 0, -1, 0};
+            if (*s_dead == 0) {
+                const int ticket = __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(p.ticket, 1) : 0, 0);
+                int left = ticket / groups;
+                b.head0 = (ticket - left * groups) * pack;
+                // the last sequence's last block comes first
+                for (int b0 = p.a.n_seq; b0 > 0; b0 -= 32) {
+                    const int seq = b0 - 1 - lane;
+                    int q0 = 0, nq = 0, k0 = 0, nk = 0;
+                    if (seq >= 0) {
+                        const int qa = p.a.d_cu_q[seq], qb = p.a.d_cu_q[seq + 1], ka = p.a.d_cu_k[seq], kb = p.a.d_cu_k[seq + 1];
+                        if (qa >= 0 && qb >= qa && (long long)qb <= p.a.q_rows && ka >= 0 && kb >= ka && (long long)kb <= p.a.k_rows) {
+                            q0 = qa; nq = qb - qa; k0 = ka; nk = kb - ka;
+                        } else if (ticket == 0) {
+                            kv4_error(p.err, KV4_ERR_PACKED_CU);
+                        }
+                    }
+                    const int blocks = (nq + block_tokens - 1) / block_tokens;
+                    int sum = blocks;
+#pragma unroll
+                    for (int d = 1; d < 32; d *= 2) {
+                        const int x = __shfl_up_sync(0xffffffffu, sum, d);
+                        if (lane >= d) sum += x;
+                    }
+                    const uint32_t hit = b.block >= 0 ? 0u : __ballot_sync(0xffffffffu, left < sum);
+                    if (hit != 0) {
+                        const int at = __ffs(hit) - 1;
+                        b.q0 = __shfl_sync(0xffffffffu, q0, at);
+                        b.k0 = __shfl_sync(0xffffffffu, k0, at);
+                        b.nq = __shfl_sync(0xffffffffu, nq, at);
+                        b.nk = __shfl_sync(0xffffffffu, nk, at);
+                        b.block = __shfl_sync(0xffffffffu, sum - 1 - left, at);
+                        if (ticket != 0) break;   // the first ticket looks at all sequences, for their reports
+                    }
+                    left -= __shfl_sync(0xffffffffu, sum, 31);
+                }
             }
-            if (ok && ragged) {   // this thread knows the lap that the barrier is in; warp 2 does not
-                ok = mbar_wait(full + 8 * ((2 * n_tiles - 1) % PK_STAGES), (uint32_t)((2 * n_tiles - 1) / PK_STAGES) & 1u);
-                mbar_arrive(v_last);
+            const uint32_t at = 8 * (k & 1);
+            if (k > 1 && !__all_sync(0xffffffffu, mbar_wait(place_empty + at, (uint32_t)((k >> 1) - 1) & 1u))) {
+                if (lane == 0) give_up(0x30045);
+                break;
             }
-            // drain: the last release arrivals land before the CTA may leave
-            for (int k = max(2 * n_tiles - PK_STAGES, 0); k < 2 * n_tiles && ok; ++k) ok = mbar_wait(empty + 8 * (k % PK_STAGES), (uint32_t)(k / PK_STAGES) & 1u);
-            if (!ok) {
-                give_up(0x30041);
-                mbar_wait(q_full, 0);   // the copies in flight
-                for (int k = max(i - PK_STAGES, 0); k < i; ++k) mbar_wait(full + 8 * (k % PK_STAGES), (uint32_t)(k / PK_STAGES) & 1u);
+            if (lane == 0) {
+                s_block[k & 1] = b;
+                mbar_arrive(place_full + at);
             }
+            if (b.block < 0) break;
+            const Shape sh = shape_of(b);
+            if (sh.n_tiles > 0 && elect_one()) {
+                const int kv_head = b.head0 / (p.a.heads / p.a.kv_heads), end = i + 2 * sh.n_tiles;
+                bool ok = used == 0 || mbar_wait(q_empty, (uint32_t)(used - 1) & 1u);
+                const bool q_asked = ok;
+                if (ok) {
+                    mbar_expect_tx(q_full, 2 * PK_Q_BYTES);
+                    for (int t = 0; t < 2; ++t)
+                        for (int h = 0; h < 2; ++h)
+                            tma_load_3d(smem_u32(q_s + t * PK_Q_BYTES + h * (PK_Q_BYTES / 2)), &tm_q, 64 * h, b.head0, b.q0 + sh.t0 + tile_tokens * t, q_full);
+                }
+                int n = i;
+                for (int j = 0; ok && n < end; ++n) {
+                    const int s = n % PK_STAGES, v = (n - i) & 1;
+                    if (n >= PK_STAGES) ok = mbar_wait(empty + 8 * s, (uint32_t)(n / PK_STAGES - 1) & 1u);
+                    if (*s_dead != 0) ok = false;
+                    if (!ok) break;
+                    mbar_expect_tx(full + 8 * s, PK_KV_BYTES);
+                    for (int h = 0; h < 2; ++h)
+                        tma_load_3d(smem_u32(kv_s + s * PK_KV_BYTES + h * (PK_KV_BYTES / 2)), v ? &tm_v : &tm_k, 64 * h, b.k0 + j * PK_KEYS, kv_head, full + 8 * s);
+                    j += v;
+                }
+                if (!ok) {
+                    give_up(0x30041);
+                    if (q_asked) mbar_wait(q_full, (uint32_t)used & 1u);   // the copies in flight
+                    for (int m = max(n - PK_STAGES, 0); m < n; ++m) mbar_wait(full + 8 * (m % PK_STAGES), (uint32_t)(m / PK_STAGES) & 1u);
+                }
+            }
+            __syncwarp();
+            if (sh.n_tiles > 0) {
+                i += 2 * sh.n_tiles;
+                ++used;
+            }
+        }
+        // drain: the last release arrivals land before the CTA may leave
+        if (*s_dead == 0 && used > 0) {
+            bool ok = mbar_wait(q_empty, (uint32_t)(used - 1) & 1u);
+            for (int m = max(i - PK_STAGES, 0); m < i && ok; ++m) ok = mbar_wait(empty + 8 * (m % PK_STAGES), (uint32_t)(m / PK_STAGES) & 1u);
+            if (!ok && lane == 0) give_up(0x30046);
+        }
+        if (lane == 0 && atomicAdd(p.done, 1) == (int)gridDim.x - 1) {   // all CTAs have taken their last ticket
+            atomicExch(p.ticket, 0);
+            atomicExch(p.done, 0);
         }
         __syncwarp();
     } else if (warp == 1) {
         if (elect_one()) {
-            // D = f32, A and B of the rows' type.  S: N = 64 keys, both K-major.  P V: N = 128 dims, V MN-major (bit 16).
+            // D = f32, A and B of the rows' type.  S: N = keys, both K-major.  P V: N = 128 dims, V MN-major (bit 16).
             const uint32_t types = (1u << 4) | (HALF ? 0u : (1u << 7) | (1u << 10));
             const uint32_t rows = (uint32_t)(PK_ROWS >> 4) << 24, idesc_o = types | (1u << 16) | ((uint32_t)(128 >> 3) << 17) | rows;
             const uint64_t qd = make_smem_desc(smem_u32(q_s), 16, 1024), kd = make_smem_desc(smem_u32(kv_s), 16, 1024);
             const uint64_t vd = make_smem_desc(smem_u32(kv_s), PK_KV_BYTES / 2, 1024);   // 64-dim halves, 8-key groups
-            const auto scores = [&](int t, int j) {   // S of tile t against key tile j
-                const int s = 2 * j % PK_STAGES;
-                const uint32_t keys = j == n_tiles - 1 && short_last ? PK_KEYS / 2 : PK_KEYS, idesc = types | (keys >> 3) << 17 | rows;
+            const auto scores = [&](int t, int i, uint32_t keys, bool last) {   // S of tile t against tile i of the ring
+                const int s = i % PK_STAGES;
+                const uint32_t idesc = types | (keys >> 3) << 17 | rows;
                 const uint64_t a = qd + (uint64_t)(t * (PK_Q_BYTES >> 4)), b = kd + (uint64_t)(s * (PK_KV_BYTES >> 4));
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks)
@@ -259,42 +299,65 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                              b + (uint64_t)((ks >> 2) * (PK_KV_BYTES >> 5) + (ks & 3) * 2), idesc, ks > 0 ? 1u : 0u);
                 umma_commit(s_full + 8 * t);
                 if (t == 1) umma_commit(empty + 8 * s);
+                if (t == 1 && last) umma_commit(q_empty);
             };
-            const auto products = [&](int t, int j, int half, bool first) {   // O of tile t += P V of 64 keys
-                const uint64_t v = vd + (uint64_t)((2 * j + 1) % PK_STAGES * (PK_KV_BYTES >> 4) + half * (64 * 128 >> 4));
+            const auto products = [&](int t, int i, int half, bool first) {   // O of tile t += P V of 64 keys
+                const uint64_t v = vd + (uint64_t)(i % PK_STAGES * (PK_KV_BYTES >> 4) + half * (64 * 128 >> 4));
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks)
                     umma_f16_ts(tmem + 128 * t, tmem + 256 + 128 * t + 64 + 32 * half + 8 * ks, v + (uint64_t)(ks * (2048 >> 4)), idesc_o, first && ks == 0 ? 0u : 1u);
             };
-            bool ok = mbar_wait(q_full, 0) && mbar_wait(full, 0);
-            if (ok) {
-                scores(0, 0);
-                scores(1, 0);
-            }
-            for (int j = 0; j < n_tiles && ok; ++j) {
-                const int iv = 2 * j + 1, ik = 2 * j + 2;   // tiles of the ring
-                const bool last = j == n_tiles - 1, both = !last || !short_last;
-                ok = *s_dead == 0 && (last && ragged ? mbar_wait(v_clean, 0) : mbar_wait(full + 8 * (iv % PK_STAGES), (uint32_t)(iv / PK_STAGES) & 1u));
-                for (int t = 0; t < 2 && ok; ++t) {
-                    if (both) {
-                        ok = mbar_wait(p_full + 16 * t + 8, (uint32_t)j & 1u);
+            bool ok = true;
+            int i = 0, used = 0, n_a = 0, n_b = 0, n_v = 0;   // tiles of the ring, blocks with keys, halves of P, cleaned tiles so far
+            for (int k = 0;; ++k) {
+                if (!mbar_wait(place_full + 8 * (k & 1), (uint32_t)(k >> 1) & 1u)) {
+                    ok = false;
+                    break;
+                }
+                const PackedBlock b = s_block[k & 1];
+                mbar_arrive(place_empty + 8 * (k & 1));
+                if (b.block < 0) break;
+                const Shape sh = shape_of(b);
+                if (sh.n_tiles == 0 || !ok) continue;
+                const auto tile_wait = [&](int at) { return mbar_wait(full + 8 * (at % PK_STAGES), (uint32_t)(at / PK_STAGES) & 1u); };
+                const auto keys_of = [&](int j) { return (uint32_t)(j == sh.n_tiles - 1 && sh.short_last ? PK_KEYS / 2 : PK_KEYS); };
+                ok = *s_dead == 0 && mbar_wait(q_full, (uint32_t)used & 1u) && tile_wait(i);
+                if (ok)
+                    for (int t = 0; t < 2; ++t) scores(t, i, keys_of(0), sh.n_tiles == 1);
+                for (int j = 0; j < sh.n_tiles && ok; ++j) {
+                    const bool last = j == sh.n_tiles - 1, both = !last || !sh.short_last, clean = last && sh.ragged;
+                    ok = *s_dead == 0 && tile_wait(i + 2 * j + 1);
+                    if (ok && clean) mbar_arrive(v_last);
+                    for (int t = 0; t < 2 && ok; ++t) {
+                        if (j == 0 && used > 0) ok = mbar_wait(o_empty + 8 * t, (uint32_t)(used - 1) & 1u);   // the block before has left
+                        if (ok && both) {
+                            ok = mbar_wait(p_full + 16 * t + 8, (uint32_t)n_b & 1u);
+                            if (ok && clean && t == 0) ok = mbar_wait(v_clean, (uint32_t)n_v & 1u);
+                            if (!ok) break;
+                            tc_fence_after();
+                            products(t, i + 2 * j + 1, 1, j == 0);
+                        }
+                        if (ok) ok = mbar_wait(p_full + 16 * t, (uint32_t)n_a & 1u);
+                        if (ok && clean && t == 0 && !both) ok = mbar_wait(v_clean, (uint32_t)n_v & 1u);
                         if (!ok) break;
                         tc_fence_after();
-                        products(t, j, 1, j == 0);
+                        products(t, i + 2 * j + 1, 0, j == 0 && !both);
+                        if (last) umma_commit(o_full + 8 * t);
+                        if (t == 1) umma_commit(empty + 8 * ((i + 2 * j + 1) % PK_STAGES));
+                        // the next scores: issued after, and so executed after, the products that read P there
+                        if (!last) {
+                            if (t == 0) ok = tile_wait(i + 2 * j + 2);
+                            if (!ok) break;
+                            scores(t, i + 2 * j + 2, keys_of(j + 1), j + 2 == sh.n_tiles);
+                        }
                     }
-                    ok = mbar_wait(p_full + 16 * t, (uint32_t)j & 1u);
-                    if (!ok) break;
-                    tc_fence_after();
-                    products(t, j, 0, j == 0 && !both);
-                    if (last) umma_commit(o_full + 8 * t);
-                    if (t == 1) umma_commit(empty + 8 * (iv % PK_STAGES));
-                    // the next scores: issued after, and so executed after, the products that read P there
-                    if (!last) {
-                        if (t == 0) ok = mbar_wait(full + 8 * (ik % PK_STAGES), (uint32_t)(ik / PK_STAGES) & 1u);
-                        if (!ok) break;
-                        scores(t, j + 1);
-                    }
+                    ++n_a;
+                    n_b += both;
+                    n_v += clean;
                 }
+                if (!ok) give_up(0x30042);
+                i += 2 * sh.n_tiles;
+                ++used;
             }
             if (!ok) give_up(0x30042);
             if (!ok || *s_dead != 0) {   // the MMAs in flight
@@ -304,13 +367,26 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         }
         __syncwarp();
     } else if (warp == 2) {
-        if (ragged) {
-            uint8_t* const tile = kv_s + (2 * n_tiles - 1) % PK_STAGES * PK_KV_BYTES;
-            const int from = n_keys - (n_tiles - 1) * PK_KEYS, n = (short_last ? PK_KEYS / 2 : PK_KEYS) - from;
-            const bool ok = __all_sync(0xffffffffu, mbar_wait(v_last, 0));
+        int i = 0, n_v = 0;
+        for (int k = 0;; ++k) {
+            if (!__all_sync(0xffffffffu, mbar_wait(place_full + 8 * (k & 1), (uint32_t)(k >> 1) & 1u))) {
+                if (lane == 0) give_up(0x30044);
+                break;
+            }
+            const PackedBlock b = s_block[k & 1];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(place_empty + 8 * (k & 1));
+            if (b.block < 0) break;
+            const Shape sh = shape_of(b);
+            i += 2 * sh.n_tiles;
+            if (!sh.ragged || *s_dead != 0) continue;
+            const bool ok = __all_sync(0xffffffffu, mbar_wait(v_last, (uint32_t)n_v & 1u));   // the issuer has seen the tile land
+            ++n_v;
             if (ok) {
-                for (int i = lane; i < n * 16; i += 32) {   // rows of 128 bytes in either half
-                    const int h = i / (n * 8), in = i - h * n * 8;
+                uint8_t* const tile = kv_s + (i - 1) % PK_STAGES * PK_KV_BYTES;
+                const int from = sh.n_keys - (sh.n_tiles - 1) * PK_KEYS, n = (sh.short_last ? PK_KEYS / 2 : PK_KEYS) - from;
+                for (int e = lane; e < n * 16; e += 32) {   // rows of 128 bytes in either half
+                    const int h = e / (n * 8), in = e - h * n * 8;
                     *reinterpret_cast<uint4*>(tile + h * (PK_KV_BYTES / 2) + from * 128 + in * 16) = make_uint4(0, 0, 0, 0);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -325,135 +401,159 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16);
         const uint32_t o_at = lane_base + 128 * t, s_at = lane_base + 256 + 128 * t, p_at = s_at + 64;
         const int row = 32 * q + lane, token = tile_tokens * t + row / pack;   // of the block
-        const int pos = min(past + t0 + token, n_keys - 1);                    // last key the row sees
-        const int pos_first = min(past + t0 + tile_tokens * t + 32 * q / pack, n_keys - 1);   // of the warp's first row
+        const int warp_token = tile_tokens * t + 32 * q / pack;                // of the warp's first row
         const float c = p.c;
-        float m = -INFINITY, l = 0.0f;           // m: maximum in use (raw scores)
-        float oh = -SHIFT, ol = 0.0f;            // P = 2^(s c - oh - ol)
-        bool large = false;                      // m c has no fraction left in fp32: then oh = m c, ol its rounding error, and m is taken off s first
         bool ok = true;
-        float2 s[32];
-        const auto load = [&](int half, int k0) {   // scores of 64 keys from k0 on
-            tmem_ld32(s_at + 64 * half, reinterpret_cast<uint32_t*>(s));
-            tmem_ld32(s_at + 64 * half + 32, reinterpret_cast<uint32_t*>(s) + 32);
-            tmem_wait_ld();
-            if (k0 + 63 > pos_first) {   // some row of the warp does not see all of them
-#pragma unroll
-                for (int e = 0; e < 32; ++e) s[e] = make_float2(k0 + 2 * e <= pos ? s[e].x : -INFINITY, k0 + 2 * e + 1 <= pos ? s[e].y : -INFINITY);
+        int used = 0, n_a = 0;   // blocks with keys, key tiles so far
+        for (int k = 0;; ++k) {
+            if (!__all_sync(0xffffffffu, mbar_wait(place_full + 8 * (k & 1), (uint32_t)(k >> 1) & 1u))) {
+                if (lane == 0) give_up(0x30043);
+                break;
             }
-        };
-        const auto largest = [&] {
-            float mx[4] = {s[0].x, s[0].y, s[1].x, s[1].y};
-#pragma unroll
-            for (int e = 2; e < 32; ++e) {
-                mx[2 * (e & 1)] = fmaxf(mx[2 * (e & 1)], s[e].x);
-                mx[2 * (e & 1) + 1] = fmaxf(mx[2 * (e & 1) + 1], s[e].y);
-            }
-            return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        };
-        const auto exponentials = [&](int half) {
-            if (__any_sync(0xffffffffu, large)) {
-                const float base = large ? m : 0.0f;
-#pragma unroll
-                for (int e = 0; e < 32; ++e) s[e] = make_float2(s[e].x - base, s[e].y - base);
-            }
-            const float off = large ? -SHIFT : oh;
-            const float2 c2 = make_float2(c, c), off2 = make_float2(-off, -off);
-            float2 ls[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t w[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float2 x = fma2(s[16 * h + e], c2, off2), a = (e * PK_FMA) % 16 + PK_FMA >= 16 + (PK_FMA == 0) ? pk_ex2_fma(x) : make_float2(pk_ex2(x.x), pk_ex2(x.y));
-                    ls[e & 1] = add2(ls[e & 1], a);
-                    w[e] = R::pack(a.x, a.y);
-                }
-                tmem_st16(p_at + 32 * half + 16 * h, w);
-            }
-            l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
-            tmem_wait_st();
-            tc_fence_before();
+            const PackedBlock b = s_block[k & 1];
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full + 16 * t + 8 * half);
-        };
-        for (int j = 0; j < n_tiles && ok; ++j) {
-            const bool both = j < n_tiles - 1 || !short_last;
-            const int k0 = j * PK_KEYS;
-            // the scores, and with them the products of the tile before, which were issued earlier
-            ok = __all_sync(0xffffffffu, *s_dead == 0 && mbar_wait(s_full + 8 * t, (uint32_t)j & 1u));
-            if (!ok) break;
-            tc_fence_after();
-            load(0, k0);
-            float mt = largest();
-            if (both) {
-                load(1, k0 + 64);
-                mt = fmaxf(mt, largest());
-            }
-            if (__any_sync(0xffffffffu, (mt - m) * c > LAG || large)) {   // rare after the first tile
-                const float mn = fmaxf(m, mt), mc = mn == -INFINITY ? 0.0f : mn * c;
-                const bool nl = fabsf(mc) >= 1048576.0f;
-                const float nh = nl ? mc : mc - SHIFT, nlow = nl ? fmaf(mn, c, -mc) - SHIFT : 0.0f;
-                const float f = m == -INFINITY ? 0.0f : pk_ex2((oh - nh) + (ol - nlow));
-                if (j > 0) {
+            if (lane == 0) mbar_arrive(place_empty + 8 * (k & 1));
+            if (b.block < 0) break;
+            const Shape sh = shape_of(b);
+            const int pos = min(sh.past + sh.t0 + token, sh.n_keys - 1);                // last key the row sees
+            const int pos_first = min(sh.past + sh.t0 + warp_token, sh.n_keys - 1);
+            const bool mine = sh.t0 + token < b.nq;
+            T* const out = static_cast<T*>(p.a.d_out) + ((size_t)(b.q0 + sh.t0) * p.a.heads + b.head0) * 128;
+            T* const dst = out + ((size_t)token * p.a.heads + row % pack) * 128;
+            float m = -INFINITY, l = 0.0f;           // m: maximum in use (raw scores)
+            float oh = -SHIFT, ol = 0.0f;            // P = 2^(s c - oh - ol)
+            bool large = false;                      // m c has no fraction left in fp32: then oh = m c, ol its rounding error, and m is taken off s first
+            float2 s[32];
+            const auto load = [&](int half, int k0) {   // scores of 64 keys from k0 on
+                tmem_ld32(s_at + 64 * half, reinterpret_cast<uint32_t*>(s));
+                tmem_ld32(s_at + 64 * half + 32, reinterpret_cast<uint32_t*>(s) + 32);
+                tmem_wait_ld();
+                if (k0 + 63 > pos_first) {   // some row of the warp does not see all of them
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        uint32_t o[32];
-                        tmem_ld32(o_at + 32 * h, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tmem_st32(o_at + 32 * h, o);
-                    }
+                    for (int e = 0; e < 32; ++e) s[e] = make_float2(k0 + 2 * e <= pos ? s[e].x : -INFINITY, k0 + 2 * e + 1 <= pos ? s[e].y : -INFINITY);
                 }
-                l *= f;
-                m = mn;
-                oh = nh;
-                ol = nlow;
-                large = nl;
-            }
-            if (both) {
-                exponentials(1);
+            };
+            const auto largest = [&] {
+                float mx[4] = {s[0].x, s[0].y, s[1].x, s[1].y};
+#pragma unroll
+                for (int e = 2; e < 32; ++e) {
+                    mx[2 * (e & 1)] = fmaxf(mx[2 * (e & 1)], s[e].x);
+                    mx[2 * (e & 1) + 1] = fmaxf(mx[2 * (e & 1) + 1], s[e].y);
+                }
+                return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            };
+            const auto exponentials = [&](int half) {
+                if (__any_sync(0xffffffffu, large)) {
+                    const float base = large ? m : 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) s[e] = make_float2(s[e].x - base, s[e].y - base);
+                }
+                const float off = large ? -SHIFT : oh;
+                const float2 c2 = make_float2(c, c), off2 = make_float2(-off, -off);
+                float2 ls[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float2 x = fma2(s[16 * h + e], c2, off2);
+                        const float2 a = (e * PK_FMA) % 16 + PK_FMA >= 16 ? pk_ex2_fma(x) : make_float2(pk_ex2(x.x), pk_ex2(x.y));
+                        ls[e & 1] = add2(ls[e & 1], a);
+                        w[e] = R::pack(a.x, a.y);
+                    }
+                    tmem_st16(p_at + 32 * half + 16 * h, w);
+                }
+                l += (ls[0].x + ls[0].y) + (ls[1].x + ls[1].y);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + 16 * t + 8 * half);
+            };
+            for (int j = 0; j < sh.n_tiles && ok; ++j) {
+                const bool both = j < sh.n_tiles - 1 || !sh.short_last;
+                const int k0 = j * PK_KEYS;
+                // the scores, and with them the products of the tile before, which were issued earlier
+                ok = __all_sync(0xffffffffu, *s_dead == 0 && mbar_wait(s_full + 8 * t, (uint32_t)(n_a + j) & 1u));
+                if (!ok) break;
+                tc_fence_after();
                 load(0, k0);
-            }
-            exponentials(0);
-        }
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(o_full + 8 * t, 0));
-        if (!ok && lane == 0) give_up(0x30043);
-        __syncwarp();
-        tc_fence_after();
-        const bool mine = t0 + token < nq;
-        T* const dst = out + ((size_t)token * p.a.heads + row % pack) * 128;
-        const float r = pos < 0 ? 0.0f : 1.0f / l;   // a row that sees no key is zeros
-        float finite = 0.0f;   // NaN as soon as an output is NaN or Inf
+                float mt = largest();
+                if (both) {
+                    load(1, k0 + 64);
+                    mt = fmaxf(mt, largest());
+                }
+                if (__any_sync(0xffffffffu, (mt - m) * c > LAG || large)) {   // rare after the first tile
+                    const float mn = fmaxf(m, mt), mc = mn == -INFINITY ? 0.0f : mn * c;
+                    const bool nl = fabsf(mc) >= 1048576.0f;
+                    const float nh = nl ? mc : mc - SHIFT, nlow = nl ? fmaf(mn, c, -mc) - SHIFT : 0.0f;
+                    const float f = m == -INFINITY ? 0.0f : pk_ex2((oh - nh) + (ol - nlow));
+                    if (j > 0) {
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            uint32_t o[32];
-            __syncwarp();
-            tmem_ld32(o_at + 32 * h, o);
-            tmem_wait_ld();
-            if (mine) {
+                        for (int h = 0; h < 4; ++h) {
+                            uint32_t o[32];
+                            tmem_ld32(o_at + 32 * h, o);
+                            tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float x = __uint_as_float(o[e + 2 * k]) * r, y = __uint_as_float(o[e + 2 * k + 1]) * r;
-                        finite = fmaf(x, 0.0f, fmaf(y, 0.0f, finite));
-                        w[k] = !ok ? 0x7fff7fffu : pos < 0 ? 0u : R::pack(x, y);
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st32(o_at + 32 * h, o);
+                        }
                     }
-                    *reinterpret_cast<uint4*>(dst + 32 * h + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    l *= f;
+                    m = mn;
+                    oh = nh;
+                    ol = nlow;
+                    large = nl;
+                }
+                if (both) {
+                    exponentials(1);
+                    load(0, k0);
+                }
+                exponentials(0);
+            }
+            n_a += sh.n_tiles;
+            if (sh.n_tiles > 0) {
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(o_full + 8 * t, (uint32_t)used & 1u));
+                ++used;
+                if (!ok && lane == 0) give_up(0x30043);
+            }
+            __syncwarp();
+            tc_fence_after();
+            const float r = pos < 0 ? 0.0f : 1.0f / l;   // a row that sees no key is zeros
+            float finite = 0.0f;   // NaN as soon as an output is NaN or Inf
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                uint32_t o[32];
+                __syncwarp();
+                tmem_ld32(o_at + 32 * h, o);   // of a block without keys: not used
+                tmem_wait_ld();
+                if (h == 3 && sh.n_tiles > 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(o_empty + 8 * t);
+                }
+                if (mine) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = __uint_as_float(o[e + 2 * i]) * r, y = __uint_as_float(o[e + 2 * i + 1]) * r;
+                            finite = fmaf(x, 0.0f, fmaf(y, 0.0f, finite));
+                            w[i] = !ok ? 0x7fff7fffu : pos < 0 ? 0u : R::pack(x, y);
+                        }
+                        *reinterpret_cast<uint4*>(dst + 32 * h + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
                 }
             }
-        }
-        __syncwarp();   // a row that is done again has been stored
-        for (uint32_t redo = ok ? __ballot_sync(0xffffffffu, mine && pos >= 0 && finite != 0.0f) : 0u; redo != 0; redo &= redo - 1) {
-            const int rr = 32 * q + __ffs(redo) - 1, tok = tile_tokens * t + rr / pack, head = head0 + rr % pack;
-            const int kv_head = head / (p.a.heads / p.a.kv_heads);
-            packed_row<T>(static_cast<const T*>(p.a.d_q) + (seq_q0 + t0 + tok) * p.a.q_stride + head * 128,
-                          static_cast<const T*>(p.a.d_k) + seq_k0 * p.a.k_stride + kv_head * 128, p.a.k_stride,
-                          static_cast<const T*>(p.a.d_v) + seq_k0 * p.a.v_stride + kv_head * 128, p.a.v_stride, past + t0 + tok + 1, c,
-                          out + ((size_t)tok * p.a.heads + rr % pack) * 128, lane);
+            __syncwarp();   // a row that is done again has been stored
+            for (uint32_t redo = ok ? __ballot_sync(0xffffffffu, mine && pos >= 0 && finite != 0.0f) : 0u; redo != 0; redo &= redo - 1) {
+                const int rr = 32 * q + __ffs(redo) - 1, tok = tile_tokens * t + rr / pack, head = b.head0 + rr % pack;
+                const int kv_head = head / (p.a.heads / p.a.kv_heads);
+                packed_row<T>(static_cast<const T*>(p.a.d_q) + (b.q0 + sh.t0 + tok) * p.a.q_stride + head * 128,
+                              static_cast<const T*>(p.a.d_k) + b.k0 * p.a.k_stride + kv_head * 128, p.a.k_stride,
+                              static_cast<const T*>(p.a.d_v) + b.k0 * p.a.v_stride + kv_head * 128, p.a.v_stride, sh.past + sh.t0 + tok + 1, c,
+                              out + ((size_t)tok * p.a.heads + rr % pack) * 128, lane);
+            }
         }
     }
     tc_fence_before();
@@ -472,6 +572,8 @@ static int packed_launch(const Qw3AttnPackedArgs& a, const Workspace* ws, bool p
     const int group = a.heads / a.kv_heads;
     p.pack = group & -group;
     if (p.pack > 16) p.pack = 16;
+    p.ticket = ws->counters;
+    p.done = ws->counters + 1;
     p.err = ws->err;
     CUtensorMap tm_q, tm_k, tm_v;
     const uint64_t qd[3] = {128, (uint64_t)a.heads, (uint64_t)a.q_rows}, qs[2] = {256, (uint64_t)a.q_stride * 2};
@@ -494,8 +596,8 @@ static int packed_launch(const Qw3AttnPackedArgs& a, const Workspace* ws, bool p
     }
     // every sequence ends with one block that may not be full
     const int64_t block_tokens = 2 * PK_ROWS / p.pack, blocks = (a.q_rows / block_tokens + a.n_seq) * (a.heads / p.pack);
-    QW3_REQUIRE(blocks <= 0x7fffffff, "qw3_attn_packed: too many rows");
-    QW3_CUDA(kv4_launch(attn_packed_kernel<T>, dim3((unsigned)blocks), dim3(PK_THREADS), PK_SMEM, st, pdl, 1, tm_q, tm_k, tm_v, p));
+    QW3_REQUIRE(blocks <= 0x7fffffff - ws->sm_count, "qw3_attn_packed: too many rows");
+    QW3_CUDA(kv4_launch(attn_packed_kernel<T>, dim3((unsigned)(blocks < ws->sm_count ? blocks : ws->sm_count)), dim3(PK_THREADS), PK_SMEM, st, pdl, 1, tm_q, tm_k, tm_v, p));
     return QW3_OK;
 }
 

@@ -133,6 +133,7 @@ def argmax_f16(logits, ws):
 # Tensors may live on any CUDA device (all of a call, and its workspace, on the same one); the call goes to that device's current
 # stream.  What the device finds out of range is left out and reported by Workspace.check().
 
+_I32 = torch.int32
 _DTYPES = {torch.float16: cabi.F16, torch.bfloat16: cabi.BF16}
 
 
@@ -160,9 +161,9 @@ def _rows128(t, heads, what, device, dtype):
 
 
 def _ints(t, n, what, device):
-    if t.dtype != torch.int32 or t.device != device or t.shape != (n,) or not t.is_contiguous():
-        raise ValueError(f"{what}: contiguous int32 [{n}] on {device} expected")
-    return t.data_ptr()
+    if t.dtype is _I32 and t.device == device and t.shape == (n,) and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{what}: contiguous int32 [{n}] on {device} expected")
 
 
 def _table(t, rows, device):
@@ -213,16 +214,17 @@ def page_slots(ctx_len, new_len, page_size, block_table, free_pages, n_free, max
     dev, n = ctx_len.device, ctx_len.shape[0]
     d_ctx = _ints(ctx_len, n, "ctx_len", dev)
     d_new = _ints(new_len, n, "new_len", dev)
-    _want(free_pages.dim() == 1, "free_pages: one dimension expected")
-    d_free = _ints(free_pages, free_pages.shape[0], "free_pages", dev)
+    capacity = free_pages.numel()
+    d_free = _ints(free_pages, capacity, "free_pages", dev)
     d_n_free = _ints(n_free, 1, "n_free", dev)
     stride = _table(block_table, n, dev)
-    _want(0 <= max_tokens < 2 ** 31, "max_tokens: out of range")
+    if not 0 <= max_tokens < 2 ** 31:
+        raise ValueError("max_tokens: out of range")
     cu, pos, slots, own_len, own_free = torch.empty(2 * n + 2 + 2 * max_tokens, dtype=torch.int32, device=dev).split_with_sizes(
         (n + 1, max_tokens, max_tokens, n, 1))
     kv_len = own_len if kv_len is None else kv_len
     n_free_out = own_free if n_free_out is None else n_free_out
-    a = cabi.PageArgs(d_ctx, d_new, n, page_size, block_table.data_ptr(), stride, block_table.shape[1], free_pages.shape[0], d_free, d_n_free,
+    a = cabi.PageArgs(d_ctx, d_new, n, page_size, block_table.data_ptr(), stride, block_table.shape[1], capacity, d_free, d_n_free,
                       _ints(n_free_out, 1, "n_free_out", dev), cu.data_ptr(), _ints(kv_len, n, "kv_len", dev), pos.data_ptr(), slots.data_ptr(), max_tokens)
     _on(dev, "qw3_page_slots", C.byref(a), ws.h)
     return cu, pos, slots, kv_len, n_free_out
@@ -247,20 +249,20 @@ def rope_kv4_append(qkv, cache, slots, pos, cos, sin, heads, ws, pairs=False):
         rot *= 2
         _want(max_pos > 0 and rot > 0, "cos: [max_pos][rot_dim / 2] expected")
         d_cos, d_sin = cos.data_ptr(), sin.data_ptr()
-    q, k = torch.empty((heads + kv) * tokens, 128, dtype=dtype, device=dev).split_with_sizes((heads * tokens, kv * tokens))
+    q, k = torch.empty((tokens, heads, 128), dtype=dtype, device=dev), torch.empty((tokens, kv, 128), dtype=dtype, device=dev)
     a = cabi.Kv4AppendArgs(qkv.data_ptr(), stride, tokens, heads, cabi.ROPE_PAIRS if pairs else cabi.ROPE_HALVES, rot, 0, d_slots, d_pos, d_cos, d_sin, max_pos,
                            q.data_ptr(), k.data_ptr())
     _on(dev, "qw3_rope_kv4_append", cache.ref, C.byref(a), ws.h)
-    return q.view(tokens, heads, 128), k.view(tokens, kv, 128)
+    return q, k
 
 
 def kv4_read(cache, slots, ws):
     """The rows of the slots as dense K and V, [tokens][kv_heads][128] each; zeros for a slot below 0."""
     dev = cache.device
-    _want(slots.dim() == 1, "slots: one dimension expected")
-    tokens = slots.shape[0]
+    tokens = slots.numel()
     d_slots = _ints(slots, tokens, "slots", dev)
-    k, v = torch.empty(2, tokens, cache.kv_heads, 128, dtype=cache.dtype, device=dev).unbind()
+    shape = (tokens, cache.kv_heads, 128)
+    k, v = torch.empty(shape, dtype=cache.dtype, device=dev), torch.empty(shape, dtype=cache.dtype, device=dev)
     _on(dev, "qw3_kv4_read", cache.ref, d_slots, tokens, k.data_ptr(), v.data_ptr(), ws.h)
     return k, v
 
