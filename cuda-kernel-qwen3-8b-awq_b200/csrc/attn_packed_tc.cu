@@ -54,7 +54,7 @@ __device__ __forceinline__ float2 pk_ex2_fma(float2 x) {
     return make_float2(__uint_as_float(__float_as_uint(t.x) * 8388608u + __float_as_uint(p.x)), __uint_as_float(__float_as_uint(t.y) * 8388608u + __float_as_uint(p.y)));
 }
 
-constexpr int PK_FMA = 4;   // of sixteen pairs of exponentials, those on the FMA pipe
+constexpr int PK_FMA = 5;   // of sixteen pairs of exponentials, those on the FMA pipe
 struct PackedParams {
     Qw3AttnPackedArgs a;
     float c;        // scale * log2(e)
@@ -533,15 +533,17 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 }
                 if (mine) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        uint32_t w[4];
+                    for (int e = 0; e < 32; e += 16) {
+                        uint32_t w[8];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
+                        for (int i = 0; i < 8; ++i) {
                             const float x = __uint_as_float(o[e + 2 * i]) * r, y = __uint_as_float(o[e + 2 * i + 1]) * r;
                             finite = fmaf(x, 0.0f, fmaf(y, 0.0f, finite));
                             w[i] = !ok ? 0x7fff7fffu : pos < 0 ? 0u : R::pack(x, y);
                         }
-                        *reinterpret_cast<uint4*>(dst + 32 * h + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                        // 32 bytes a lane: every lane writes a row of its own, and a store takes a cycle a row
+                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 32 * h + e), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                                     "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
                     }
                 }
             }
@@ -620,6 +622,7 @@ extern "C" int qw3_attn_packed(const Qw3AttnPackedArgs* a, qw3_ws_t ws, void* st
                 "%s: strides must be multiples of 8 and hold the heads", who);
     QW3_REQUIRE(((reinterpret_cast<uintptr_t>(a->d_q) | reinterpret_cast<uintptr_t>(a->d_out) | reinterpret_cast<uintptr_t>(a->d_k) | reinterpret_cast<uintptr_t>(a->d_v)) & 15) == 0,
                 "%s: rows must be 16-byte aligned", who);
+    QW3_REQUIRE((reinterpret_cast<uintptr_t>(a->d_out) & 31) == 0, "%s: out must be 32-byte aligned", who);
     const int rc = ws_on_device(who, ws);
     if (rc != QW3_OK) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -287,7 +287,7 @@ typedef struct Qw3AttnPackedArgs {
     int32_t  head_dim;        /* 128 */
     int32_t  dtype;           /* enum Qw3Dtype */
     float    scale;           /* of the scores, above 0; 0: 1 / sqrt(128) */
-    void*    d_out;           /* [q_rows][heads][128] */
+    void*    d_out;           /* [q_rows][heads][128], 32-byte aligned */
 } Qw3AttnPackedArgs;
 
 /* Causal attention of packed sequences (attentionKernel, Inference.cu:182-266, intended math; the reference has one sequence and as
