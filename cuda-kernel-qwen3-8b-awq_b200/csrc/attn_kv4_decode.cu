@@ -36,6 +36,8 @@ static_assert(2 * (size_t)KD_MAX_GRID * KD_PART <= WS_PARTIALS && KD_MAX_GRID <=
 struct KdSmem {
     uint8_t ring[KD_WARPS][KD_STAGES][KD_STAGE_BYTES];
     float4 o[KD_WARPS][8][32];        // sums of a warp, in the order of its fragments
+    struct { const uint8_t* at[2]; } src[KD_WARPS][32];   // tiles of the chunks that are looked up, and of each the tokens in them: 16 bits a tile
+    int tokens[KD_WARPS][32];
     float4 token[KD_WARPS][KD_CHUNK];  // of the chunk's tokens: scale of K * 2^24, minimum of K, log2 of V's scale, 1 / V's scale
     float mid[KD_WARPS][KD_CHUNK];     // and V's minimum + 8 * scale
     float stat[KD_WARPS][8][3];
@@ -199,8 +201,6 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
     const int my_chunks = (n_mine - warp + KD_WARPS - 1) / KD_WARPS;
     KdPlace ahead = place;
     int ahead_at = 0, issued = 0;   // `ahead` is the place of the CTA's chunk number ahead_at; chunks issued
-    int tokens = 0;                 // of the lane's chunk, in its two tiles: 16 bits each
-    const uint8_t *src0 = nullptr, *src1 = nullptr;
     const auto tile_at = [&](const KdPlace& q, int tile) -> const uint8_t* {   // null where the page is outside the pool
         const int in = tile / tiles_page, page = p.a.d_block_table[q.b * p.a.table_stride + in];
         if (page < 0 || page >= p.pool.n_pages) {
@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
     };
     const auto look_up = [&]() {
         const int k = issued + lane, at = warp + KD_WARPS * k;
-        tokens = 0;
+        int tokens = 0;
+        const uint8_t *src0 = nullptr, *src1 = nullptr;
         KdPlace q = ahead;
         if (k < my_chunks) {
             int left = at - ahead_at;
@@ -232,6 +233,9 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
                 if (src1 != nullptr) tokens |= min(n1, 16) << 16;
             }
         }
+        sm.src[warp][lane].at[0] = src0;
+        sm.src[warp][lane].at[1] = src1;
+        sm.tokens[warp][lane] = tokens;
         __syncwarp();
         // the next thirty-two are found from the last of these (used only where there is one)
         ahead.ht = __shfl_sync(0xffffffffu, q.ht, 31);
@@ -241,20 +245,20 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
         ahead_at = warp + KD_WARPS * (issued + 31);
     };
     const auto issue = [&]() {
-        const int turn = issued & 31;
+        const int turn = issued & 31, s = issued % KD_STAGES;
         if (turn == 0) look_up();
-        const int s = issued % KD_STAGES, n = __shfl_sync(0xffffffffu, tokens, turn);
-        const unsigned long long a = __shfl_sync(0xffffffffu, (unsigned long long)src0, turn), b = __shfl_sync(0xffffffffu, (unsigned long long)src1, turn);
         if (elect_one()) {
             const uint32_t bar = smem_u32(&sm.bar[warp][s]), to = smem_u32(sm.ring[warp][s]);
+            const int n = sm.tokens[warp][turn];
+            const uint8_t *const a = sm.src[warp][turn].at[0], *const b = sm.src[warp][turn].at[1];
             const bool n0 = (n & 0xffff) != 0, n1 = n >> 16 != 0;
             sm.valid[warp][s] = n;
             mbar_expect_tx(bar, (n0 ? KV4_TILE_BYTES : 0) + (n1 ? KV4_TILE_BYTES : 0));
             if (n0 && n1 && b - a == KV4_TILE_BYTES) {   // of one page
-                bulk_load(to, reinterpret_cast<const void*>(a), 2 * KV4_TILE_BYTES, bar);
+                bulk_load(to, a, 2 * KV4_TILE_BYTES, bar);
             } else {
-                if (n0) bulk_load(to, reinterpret_cast<const void*>(a), KV4_TILE_BYTES, bar);
-                if (n1) bulk_load(to + KV4_TILE_BYTES, reinterpret_cast<const void*>(b), KV4_TILE_BYTES, bar);
+                if (n0) bulk_load(to, a, KV4_TILE_BYTES, bar);
+                if (n1) bulk_load(to + KV4_TILE_BYTES, b, KV4_TILE_BYTES, bar);
             }
         }
         __syncwarp();
@@ -356,8 +360,11 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
 
         for (; warp + KD_WARPS * used < part_end; ++used) {
             const int s = used % KD_STAGES;
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sm.bar[warp][s]), (uint32_t)(used / KD_STAGES) & 1u));
-            if (!ok) continue;   // reported below
+            const uint32_t bar = smem_u32(&sm.bar[warp][s]), parity = (uint32_t)(used / KD_STAGES) & 1u;
+            if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity));
+                if (!ok) continue;   // reported below
+            }
             const uint8_t* const stage = sm.ring[warp][s];
             {   // lane i: what belongs to token i of the chunk; behind the last one nothing is left but codes, which are finite, times zero
                 const uint8_t* const tile = stage + (lane >> 4) * KV4_TILE_BYTES + 4 * (lane & 15);
