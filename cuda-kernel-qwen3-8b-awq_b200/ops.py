@@ -173,16 +173,19 @@ def _table(t, rows, device):
     return t.stride(0) if rows > 1 else shape[1]
 
 
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _on(device, name, *args):
     """Calls entry point `name` on the device's current stream."""
-    if device.type != "cuda":
+    index = device.index
+    if index is None or device.type != "cuda":
         raise ValueError(f"{name}: CUDA tensors expected")
-    fn, stream = getattr(cabi.lib(), name), torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch._C._cuda_getDevice():
-        status = fn(*args, stream)
+    if index == _current_device():
+        status = getattr(cabi.lib(), name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, stream)
+            status = getattr(cabi.lib(), name)(*args, _raw_stream(index))
     if status:
         cabi.check(status, name)
 
@@ -220,8 +223,7 @@ def page_slots(ctx_len, new_len, page_size, block_table, free_pages, n_free, max
     stride = _table(block_table, n, dev)
     if not 0 <= max_tokens < 2 ** 31:
         raise ValueError("max_tokens: out of range")
-    cu, pos, slots, own_len, own_free = torch.empty(2 * n + 2 + 2 * max_tokens, dtype=torch.int32, device=dev).split_with_sizes(
-        (n + 1, max_tokens, max_tokens, n, 1))
+    cu, pos, slots, own_len, own_free = ctx_len.new_empty(2 * n + 2 + 2 * max_tokens).split_with_sizes((n + 1, max_tokens, max_tokens, n, 1))
     kv_len = own_len if kv_len is None else kv_len
     n_free_out = own_free if n_free_out is None else n_free_out
     a = cabi.PageArgs(d_ctx, d_new, n, page_size, block_table.data_ptr(), stride, block_table.shape[1], capacity, d_free, d_n_free,
@@ -249,7 +251,7 @@ def rope_kv4_append(qkv, cache, slots, pos, cos, sin, heads, ws, pairs=False):
         rot *= 2
         _want(max_pos > 0 and rot > 0, "cos: [max_pos][rot_dim / 2] expected")
         d_cos, d_sin = cos.data_ptr(), sin.data_ptr()
-    q, k = torch.empty((tokens, heads, 128), dtype=dtype, device=dev), torch.empty((tokens, kv, 128), dtype=dtype, device=dev)
+    q, k = qkv.new_empty((tokens, heads, 128)), qkv.new_empty((tokens, kv, 128))
     a = cabi.Kv4AppendArgs(qkv.data_ptr(), stride, tokens, heads, cabi.ROPE_PAIRS if pairs else cabi.ROPE_HALVES, rot, 0, d_slots, d_pos, d_cos, d_sin, max_pos,
                            q.data_ptr(), k.data_ptr())
     _on(dev, "qw3_rope_kv4_append", cache.ref, C.byref(a), ws.h)
@@ -261,8 +263,8 @@ def kv4_read(cache, slots, ws):
     dev = cache.device
     tokens = slots.numel()
     d_slots = _ints(slots, tokens, "slots", dev)
-    shape = (tokens, cache.kv_heads, 128)
-    k, v = torch.empty(shape, dtype=cache.dtype, device=dev), torch.empty(shape, dtype=cache.dtype, device=dev)
+    k = torch.empty((tokens, cache.kv_heads, 128), dtype=cache.dtype, device=dev)
+    v = torch.empty_like(k)
     _on(dev, "qw3_kv4_read", cache.ref, d_slots, tokens, k.data_ptr(), v.data_ptr(), ws.h)
     return k, v
 
@@ -277,7 +279,7 @@ def attn_kv4_decode(q, cache, block_table, kv_len, ws, scale=None):
     n = q.shape[0]
     d_len = _ints(kv_len, n, "kv_len", dev)
     table_stride = _table(block_table, n, dev)
-    out = torch.empty(n, heads, 128, dtype=dtype, device=dev)
+    out = torch.empty_like(q) if q.dim() == 3 and q.is_contiguous() else q.new_empty((n, heads, 128))
     a = cabi.AttnKv4Args(q.data_ptr(), stride, n, heads, block_table.data_ptr(), table_stride, block_table.shape[1], scale or 0.0, d_len, out.data_ptr())
     _on(dev, "qw3_attn_kv4_decode", cache.ref, C.byref(a), ws.h)
     return out
@@ -298,7 +300,7 @@ def attn_packed(q, k, v, cu_q, cu_k, ws, scale=None, out=None):
     _want(n >= 0, "cu_q: [sequences + 1] expected")
     d_cu_q, d_cu_k = _ints(cu_q, n + 1, "cu_q", dev), _ints(cu_k, n + 1, "cu_k", dev)
     if out is None:
-        out = torch.empty(q.shape[0], heads, 128, dtype=dtype, device=dev)
+        out = torch.empty_like(q) if q.dim() == 3 and q.is_contiguous() else q.new_empty((q.shape[0], heads, 128))
     else:
         _want(out.device == dev and out.dtype == dtype and out.is_contiguous() and out.numel() == q.shape[0] * heads * 128,
               "out: contiguous [q_rows][heads][128] expected")
