@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
             found[e] = w == total;
             x[e] = found[e] ? chunks : ht[e] * per_head;
         }
-        int before = 0;             // chunks of the requests before the thirty-two
+        long long before = 0;       // chunks of the requests before the thirty-two
         for (int b0 = 0; b0 < B && !(found[0] && found[1]); b0 += 32) {
             const int n = b0 + lane < B ? (length(b0 + lane) + KD_CHUNK - 1) / KD_CHUNK : 0;
             int s = n;

@@ -42,7 +42,8 @@ __device__ __forceinline__ float pk_ex2(float x) {
 
 // 2^x for two x up to 30, on the FMA pipe: the exponential unit (16 results a clock and SM) is what the softmax waits for.  x = n + f with n the
 // nearest whole number, which 1.5 * 2^23 + x has in its last bits; 2^f by a polynomial of degree 4 that is 1 at 0 (minimax on [-1/2, 1/2] by
-// Remez' exchange: relative error 3.6e-6); n is added to the exponent.  Below -127, -Inf included, exactly 0.
+// Remez' exchange: relative error 3.6e-6); n is added to the exponent.  Below -127, -Inf included, exactly 0.  Not for NaN:
+// a row that sees one has it in its maximum.
 __device__ __forceinline__ float2 pk_ex2_fma(float2 x) {
     constexpr float MAGIC = 12582912.0f;
     x = make_float2(fmaxf(x.x, -127.0f), fmaxf(x.y, -127.0f));
@@ -54,6 +55,12 @@ __device__ __forceinline__ float2 pk_ex2_fma(float2 x) {
     return make_float2(__uint_as_float(__float_as_uint(t.x) * 8388608u + __float_as_uint(p.x)), __uint_as_float(__float_as_uint(t.y) * 8388608u + __float_as_uint(p.y)));
 }
 
+// the largest of three, NaN where one is
+__device__ __forceinline__ float pk_max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 constexpr int PK_FMA = 5;   // of sixteen pairs of exponentials, those on the FMA pipe
 struct PackedParams {
     Qw3AttnPackedArgs a;
@@ -188,25 +195,31 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     };
 
     if (warp == 0) {
-        int i = 0, used = 0;   // tiles asked for, blocks with keys
+        const auto sequence = [&](int s, int& q0, int& nq, int& k0, int& nk) {   // false where it is not inside the buffers, which leaves it without rows
+            q0 = nq = k0 = nk = 0;
+            if (s < 0) return true;
+            const int qa = p.a.d_cu_q[s], qb = p.a.d_cu_q[s + 1], ka = p.a.d_cu_k[s], kb = p.a.d_cu_k[s + 1];
+            if (qa < 0 || qb < qa || (long long)qb > p.a.q_rows || ka < 0 || kb < ka || (long long)kb > p.a.k_rows) return false;
+            q0 = qa; nq = qb - qa; k0 = ka; nk = kb - ka;
+            return true;
+        };
+        if (blockIdx.x == 0)   // the reports
+            for (int s = lane; s < p.a.n_seq; s += 32) {
+                int q0, nq, k0, nk;
+                if (!sequence(s, q0, nq, k0, nk)) kv4_error(p.err, KV4_ERR_PACKED_CU);
+            }
+        __syncwarp();
+        int i = 0, used = 0;                  // tiles asked for, blocks with keys
+        int seq0 = p.a.n_seq, passed = 0;     // the search for the next block: sequences below seq0 are left, the others have `passed` blocks
         for (int k = 0;; ++k) {
             PackedBlock b = {0, 0, 0, 0, -1, 0};
             if (*s_dead == 0) {
-                const int ticket = __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(p.ticket, 1) : 0, 0);
-                int left = ticket / groups;
-                b.head0 = (ticket - left * groups) * pack;
-                // the last sequence's last block comes first
-                for (int b0 = p.a.n_seq; b0 > 0; b0 -= 32) {
-                    const int seq = b0 - 1 - lane;
-                    int q0 = 0, nq = 0, k0 = 0, nk = 0;
-                    if (seq >= 0) {
-                        const int qa = p.a.d_cu_q[seq], qb = p.a.d_cu_q[seq + 1], ka = p.a.d_cu_k[seq], kb = p.a.d_cu_k[seq + 1];
-                        if (qa >= 0 && qb >= qa && (long long)qb <= p.a.q_rows && ka >= 0 && kb >= ka && (long long)kb <= p.a.k_rows) {
-                            q0 = qa; nq = qb - qa; k0 = ka; nk = kb - ka;
-                        } else if (ticket == 0) {
-                            kv4_error(p.err, KV4_ERR_PACKED_CU);
-                        }
-                    }
+                const int ticket = __shfl_sync(0xffffffffu, lane == 0 ? atomicAdd(p.ticket, 1) : 0, 0), number = ticket / groups;
+                b.head0 = (ticket - number * groups) * pack;
+                // the last sequence's last block comes first; the numbers of a CTA grow, so the search goes on where it was
+                while (seq0 > 0 && b.block < 0) {
+                    int q0, nq, k0, nk;
+                    sequence(seq0 - 1 - lane, q0, nq, k0, nk);
                     const int blocks = (nq + block_tokens - 1) / block_tokens;
                     int sum = blocks;
 #pragma unroll
@@ -214,17 +227,18 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                         const int x = __shfl_up_sync(0xffffffffu, sum, d);
                         if (lane >= d) sum += x;
                     }
-                    const uint32_t hit = b.block >= 0 ? 0u : __ballot_sync(0xffffffffu, left < sum);
+                    const uint32_t hit = __ballot_sync(0xffffffffu, number - passed < sum);
                     if (hit != 0) {
-                        const int at = __ffs(hit) - 1;
-                        b.q0 = __shfl_sync(0xffffffffu, q0, at);
-                        b.k0 = __shfl_sync(0xffffffffu, k0, at);
-                        b.nq = __shfl_sync(0xffffffffu, nq, at);
-                        b.nk = __shfl_sync(0xffffffffu, nk, at);
-                        b.block = __shfl_sync(0xffffffffu, sum - 1 - left, at);
-                        if (ticket != 0) break;   // the first ticket looks at all sequences, for their reports
+                        const int from = __ffs(hit) - 1;
+                        b.q0 = __shfl_sync(0xffffffffu, q0, from);
+                        b.k0 = __shfl_sync(0xffffffffu, k0, from);
+                        b.nq = __shfl_sync(0xffffffffu, nq, from);
+                        b.nk = __shfl_sync(0xffffffffu, nk, from);
+                        b.block = __shfl_sync(0xffffffffu, sum - 1 - (number - passed), from);
+                    } else {
+                        passed += __shfl_sync(0xffffffffu, sum, 31);
+                        seq0 -= 32;
                     }
-                    left -= __shfl_sync(0xffffffffu, sum, 31);
                 }
             }
             const uint32_t at = 8 * (k & 1);
@@ -436,11 +450,8 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             const auto largest = [&] {
                 float mx[4] = {s[0].x, s[0].y, s[1].x, s[1].y};
 #pragma unroll
-                for (int e = 2; e < 32; ++e) {
-                    mx[2 * (e & 1)] = fmaxf(mx[2 * (e & 1)], s[e].x);
-                    mx[2 * (e & 1) + 1] = fmaxf(mx[2 * (e & 1) + 1], s[e].y);
-                }
-                return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                for (int e = 2; e < 32; ++e) mx[e & 3] = pk_max3(mx[e & 3], s[e].x, s[e].y);
+                return max_nan(pk_max3(mx[0], mx[1], mx[2]), mx[3]);
             };
             const auto exponentials = [&](int half) {
                 if (__any_sync(0xffffffffu, large)) {
@@ -480,10 +491,10 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 float mt = largest();
                 if (both) {
                     load(1, k0 + 64);
-                    mt = fmaxf(mt, largest());
+                    mt = max_nan(mt, largest());
                 }
-                if (__any_sync(0xffffffffu, (mt - m) * c > LAG || large)) {   // rare after the first tile
-                    const float mn = fmaxf(m, mt), mc = mn == -INFINITY ? 0.0f : mn * c;
+                if (__any_sync(0xffffffffu, !((mt - m) * c <= LAG) || large)) {   // rare after the first tile; NaN goes this way too
+                    const float mn = max_nan(m, mt), mc = mn == -INFINITY ? 0.0f : mn * c;
                     const bool nl = fabsf(mc) >= 1048576.0f;
                     const float nh = nl ? mc : mc - SHIFT, nlow = nl ? fmaf(mn, c, -mc) - SHIFT : 0.0f;
                     const float f = m == -INFINITY ? 0.0f : pk_ex2((oh - nh) + (ol - nlow));

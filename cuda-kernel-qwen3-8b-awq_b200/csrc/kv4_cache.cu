@@ -135,16 +135,6 @@ __global__ void __launch_bounds__(PS_THREADS) page_slots_kernel(const Qw3PageArg
 // heads, bf16, 181 MB: 43 us, 4.2 TB/s.
 constexpr int AP_THREADS = 256, AP_WARPS = AP_THREADS / 32, AP_MAX_ROWS = 96;
 
-__device__ __forceinline__ float min_nan(float a, float b) {   // NaN where either is
-    float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 // Over the lanes of either half-warp.  Two reductions over the whole warp: one with a mask a half would be run half after half.
 template <bool MAX>
 __device__ __forceinline__ float reduce_half(float a, bool upper) {
@@ -375,7 +365,7 @@ extern "C" {
 int qw3_page_slots(const Qw3PageArgs* a, qw3_ws_t ws, void* stream) {
     const char* who = "qw3_page_slots";
     QW3_REQUIRE(a && ws, "%s: null argument", who);
-    QW3_REQUIRE(a->d_ctx_len && a->d_new_len && a->d_block_table && a->d_free && a->d_n_free && a->d_n_free_out && a->d_cu && a->d_kv_len, "%s: null pointer", who);
+    QW3_REQUIRE(a->d_ctx_len && a->d_new_len && a->d_block_table && (a->d_free || a->free_capacity == 0) && a->d_n_free && a->d_n_free_out && a->d_cu && a->d_kv_len, "%s: null pointer", who);
     QW3_REQUIRE(a->max_tokens >= 0 && (a->max_tokens == 0 || (a->d_pos && a->d_slot)), "%s: null pointer or max_tokens out of range", who);
     QW3_REQUIRE(a->max_tokens <= 0x7fffffff - 65536, "%s: max_tokens out of range", who);
     QW3_REQUIRE(a->n_req > 0 && a->n_req <= PS_MAX_REQ, "%s: n_req must be 1 to %d", who, PS_MAX_REQ);

@@ -244,3 +244,36 @@ def test_prompt_then_tokens_through_the_cache(ops, cuda, dtype):
             out = ops.attn_packed(q, kk, vv, cu, _cu(held, cuda), ws)
             _check(out, q, kk, vv, new, held)
     ws.check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_packed_a_key_that_is_not_finite_reaches_every_row_that_sees_it(ops, cuda, dtype, value):
+    """NaN or Inf in key i of sequence i, for every place in two tiles of keys (the exponentials of a tile are computed in two ways): the rows that
+    see it are NaN, the ones before it are not."""
+    n = 260
+    lens = [n] * n
+    g = torch.Generator(device=cuda).manual_seed(12)
+    q = torch.randn(2 * n, 4, 128, device=cuda, generator=g).abs().to(dtype)
+    k = torch.randn(n, n, 1, 128, device=cuda, generator=g).to(dtype)
+    v = torch.randn(n * n, 1, 128, device=cuda, generator=g).to(dtype)
+    i = torch.arange(n, device=cuda)
+    k[i, i, 0, 7] = value
+    ws = ops.Workspace()
+    # two queries a sequence: its last rows, which see all keys but the last one, and all
+    got = ops.attn_packed(q, k.flatten(0, 1), v, _cu([2] * n, cuda), _cu(lens, cuda), ws).view(n, 2, 4, 128)
+    ws.check()
+    bad = got.isnan().all(-1).all(-1)
+    want = torch.ones(n, 2, dtype=torch.bool, device=cuda)
+    want[n - 1, 0] = False
+    assert torch.equal(bad, want) and got[n - 1, 0].isfinite().all()
+
+
+def test_packed_many_sequences(ops, cuda):
+    """More sequences than a CTA looks at in one step, of lengths that make blocks of every size."""
+    lens = [(7 * b) % 19 for b in range(1500)]
+    q, k, v = _rows(lens, lens, 2, 1, torch.float16, cuda, seed=13)
+    ws = ops.Workspace()
+    got = ops.attn_packed(q, k, v, _cu(lens, cuda), _cu(lens, cuda), ws)
+    ws.check()
+    _check(got, q, k, v, lens, lens)

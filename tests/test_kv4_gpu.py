@@ -173,6 +173,28 @@ def test_append_and_read(ops, cuda, dtype, pairs, tokens, heads, kv, page, rot, 
         assert ((want - rows.double()).abs() <= step * (0.5 + 2.0 ** -20) + ref.HALF[dtype] * (1.01 * lo.abs() + 1.01 * (hi - lo)) + tiny * 8).all()
 
 
+def test_append_without_the_rotated_k_and_empty_calls(ops, cuda):
+    """Through the C entry point: no buffer for k; and calls without tokens, requests or new tokens, which do nothing."""
+    cabi = ops.cabi
+    L, ws, st = cabi.lib(), ops.Workspace(), ops._stream()
+    qkv = torch.randn(3, 8 * 128, generator=_gen(16)).half().to(cuda)
+    caches = [ops.Kv4Cache.alloc(2, 16, 2, torch.float16, cuda) for _ in range(2)]
+    slots = _i32([4, 31, 0], cuda)
+    want, _ = ops.rope_kv4_append(qkv, caches[0], slots, None, None, None, 4, ws)
+    q = torch.zeros_like(want)
+    a = cabi.Kv4AppendArgs(qkv.data_ptr(), 8 * 128, 3, 4, cabi.ROPE_HALVES, 0, 0, slots.data_ptr(), None, None, None, 0, q.data_ptr(), None)
+    cabi.check(L.qw3_rope_kv4_append(caches[1].ref, C.byref(a), ws.h, st), "qw3_rope_kv4_append")
+    assert torch.equal(q, want) and torch.equal(caches[0].pages, caches[1].pages)
+    none = torch.empty(0, dtype=torch.int32, device=cuda)
+    assert ops.rope_kv4_append(qkv[:0], caches[0], none, None, None, None, 4, ws)[0].shape == (0, 4, 128)
+    assert ops.kv4_read(caches[0], none, ws)[1].shape == (0, 2, 128)
+    assert ops.attn_kv4_decode(q[:0], caches[0], torch.empty(0, 1, dtype=torch.int32, device=cuda), none, ws).shape == (0, 4, 128)
+    table = torch.full((2, 3), -1, dtype=torch.int32, device=cuda)
+    got = ops.page_slots(_i32([0, 0], cuda), _i32([0, 0], cuda), 16, table, none, _i32([0], cuda), 0, ws)
+    ws.check()
+    assert got[0].tolist() == [0, 0, 0] and got[1].numel() == got[2].numel() == 0 and got[3].tolist() == [0, 0] and (table == -1).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_append_of_halfway_values_rounds_to_even(ops, cuda, dtype):
     """Rows 0, 0.5, 1, .. 15: scale 1, and every second value halfway between two codes."""
