@@ -90,8 +90,10 @@ struct KdPlace {
     int ht, b, c, n;
 };
 
-template <class T>
-__global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(const KdParams p) {
+// NARROW: groups of four heads at most, which leave half of a fragment's columns empty.  The lanes of the empty columns take the scores of the
+// second tile, so that each has half as many exponentials; what they put into the products' empty columns is read by nobody.
+template <class T, bool NARROW>
+__global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(KdParams p) {
     extern __shared__ __align__(128) uint8_t kd_smem[];
     KdSmem& sm = *reinterpret_cast<KdSmem*>(kd_smem);
     using R = RowType<T>;
@@ -327,10 +329,11 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
                 qf[j][2] = __byte_perm(w[j].x, w[j].z, 0x7632);
                 qf[j][3] = __byte_perm(w[j].y, w[j].w, 0x7632);
             }
-            f0 = __shfl_sync(0xffffffffu, f, 8 * t);
-            f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
-            qs0 = __shfl_sync(0xffffffffu, sum, 8 * t);
-            qs1 = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+            const int from = 4 * (NARROW ? 2 * (t & 1) : 2 * t);   // of the lane's two heads
+            f0 = __shfl_sync(0xffffffffu, f, from);
+            f1 = __shfl_sync(0xffffffffu, f, from + 4);
+            qs0 = __shfl_sync(0xffffffffu, sum, from);
+            qs1 = __shfl_sync(0xffffffffu, sum, from + 4);
         }
 
         int unflushed = 0;      // chunks in the accumulators
@@ -374,8 +377,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
                 sm.mid[warp][lane] = in ? fmaf(8.0f, vs.x, vs.y) : 0.0f;
             }
             __syncwarp();
-            float u[2][4];       // tokens row0, row0 + 8 x heads 2t, 2t + 1
-            float inv[2][2];
+            float sum[2][4];     // of a tile: tokens row0, row0 + 8 x heads 2t, 2t + 1
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const uint8_t* const tile = stage + e * KV4_TILE_BYTES;
@@ -394,18 +396,32 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
                     }
                 }
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {   // token row0 + 8 h
-                    const float4 k = sm.token[warp][16 * e + row0 + 8 * h];
-                    const float s0 = fmaf(k.x, fmaf(hi[2 * h], 0.0625f, lo[2 * h]), k.y * qs0), s1 = fmaf(k.x, fmaf(hi[2 * h + 1], 0.0625f, lo[2 * h + 1]), k.y * qs1);
-                    u[e][2 * h] = fmaf(f0, s0, k.z);
-                    u[e][2 * h + 1] = fmaf(f1, s1, k.z);
-                    inv[e][h] = k.w;
+                for (int i = 0; i < 4; ++i) sum[e][i] = fmaf(hi[i], 0.0625f, lo[i]);
+            }
+            if (NARROW) {        // lanes of t = 2, 3: the second tile's, of the heads of t = 0, 1
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float other = __shfl_xor_sync(0xffffffffu, sum[1][i], 2);
+                    sum[0][i] = t < 2 ? sum[0][i] : other;
                 }
             }
-            float x0m = fmaxf(fmaxf(u[0][0], u[0][2]), fmaxf(u[1][0], u[1][2])), x1m = fmaxf(fmaxf(u[0][1], u[0][3]), fmaxf(u[1][1], u[1][3]));
+            constexpr int TILES = NARROW ? 1 : 2;   // that the lane has values of
+            float u[TILES][4], inv[TILES][2];
+            float x0m = -INFINITY, x1m = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < TILES; ++e)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {   // token row0 + 8 h
+                    const float4 k = sm.token[warp][16 * (NARROW ? t >> 1 : e) + row0 + 8 * h];
+                    u[e][2 * h] = fmaf(f0, fmaf(k.x, sum[e][2 * h], k.y * qs0), k.z);
+                    u[e][2 * h + 1] = fmaf(f1, fmaf(k.x, sum[e][2 * h + 1], k.y * qs1), k.z);
+                    inv[e][h] = k.w;
+                    x0m = fmaxf(x0m, u[e][2 * h]);
+                    x1m = fmaxf(x1m, u[e][2 * h + 1]);
+                }
             if (__any_sync(0xffffffffu, x0m > mu0 + 7.0f || x1m > mu1 + 7.0f)) {   // rare after the first chunks
 #pragma unroll
-                for (int d = 4; d < 32; d *= 2) {
+                for (int d = NARROW ? 2 : 4; d < 32; d *= 2) {
                     x0m = fmaxf(x0m, __shfl_xor_sync(0xffffffffu, x0m, d));
                     x1m = fmaxf(x1m, __shfl_xor_sync(0xffffffffu, x1m, d));
                 }
@@ -426,21 +442,26 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
             }
             ++unflushed;
             const float z0 = mu0 == -INFINITY ? 0.0f : mu0 - 8.0f, z1 = mu1 == -INFINITY ? 0.0f : mu1 - 8.0f;
+            uint32_t pp[TILES][2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const uint8_t* const tile = stage + e * KV4_TILE_BYTES + KV4_V;
-                uint32_t pf[2];
+            for (int e = 0; e < TILES; ++e)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float mid = sm.mid[warp][16 * e + row0 + 8 * h];
+                    const float mid = sm.mid[warp][16 * (NARROW ? t >> 1 : e) + row0 + 8 * h];
                     const float p0 = kd_ex2(u[e][2 * h] - z0), p1 = kd_ex2(u[e][2 * h + 1] - z1);
                     const float w0 = p0 * inv[e][h], w1 = p1 * inv[e][h];
                     l0 += w0;
                     l1 += w1;
                     m0 = fmaf(w0, mid, m0);
                     m1 = fmaf(w1, mid, m1);
-                    pf[h] = kd_transpose(RowType<__half>::pack(p0, p1));
+                    pp[e][h] = RowType<__half>::pack(p0, p1);
                 }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint8_t* const tile = stage + e * KV4_TILE_BYTES + KV4_V;
+                uint32_t pf[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) pf[h] = kd_transpose(!NARROW ? pp[e % TILES][h] : e == 0 ? pp[0][h] : __shfl_xor_sync(0xffffffffu, pp[0][h], 2));
                 const int ra = 2 * t + (t & 1), rb = 2 * t + (~t & 1);   // tokens of indexes 2t and 2t + 1
                 const uint2 a0 = *reinterpret_cast<const uint2*>(tile + ra * 64 + 8 * g), b0 = *reinterpret_cast<const uint2*>(tile + rb * 64 + 8 * g);
                 const uint2 a1 = *reinterpret_cast<const uint2*>(tile + ra * 64 + 512 + 8 * g), b1 = *reinterpret_cast<const uint2*>(tile + rb * 64 + 512 + 8 * g);
@@ -461,14 +482,14 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(co
 
         // the states of the four warps, then of the CTAs that share the pair
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2) {
+        for (int d = NARROW ? 2 : 4; d < 32; d *= 2) {
             l0 += __shfl_xor_sync(0xffffffffu, l0, d);
             l1 += __shfl_xor_sync(0xffffffffu, l1, d);
             m0 += __shfl_xor_sync(0xffffffffu, m0, d);
             m1 += __shfl_xor_sync(0xffffffffu, m1, d);
         }
         if (!ok) l0 = l1 = NAN;
-        if (g == 0) {
+        if (g == 0 && (!NARROW || t < 2)) {
             float* const st = sm.stat[warp][2 * t];
             st[0] = mu0; st[1] = l0; st[2] = m0;
             st[3] = mu1; st[4] = l1; st[5] = m1;
@@ -654,11 +675,12 @@ extern "C" int qw3_attn_kv4_decode(const Qw3Kv4Pool* pool, const Qw3AttnKv4Args*
     int grid = w->sm_count * KD_CTAS;
     if (grid > KD_MAX_GRID) grid = KD_MAX_GRID;
     if (most < grid) grid = most < 1.0 ? 1 : (int)most;
-    const auto kernel = pool->dtype == QW3_F16 ? attn_kv4_decode_kernel<__half> : attn_kv4_decode_kernel<__nv_bfloat16>;
+    void (*const kernels[4])(KdParams) = {attn_kv4_decode_kernel<__half, false>, attn_kv4_decode_kernel<__half, true>,
+                                          attn_kv4_decode_kernel<__nv_bfloat16, false>, attn_kv4_decode_kernel<__nv_bfloat16, true>};
+    const auto kernel = kernels[(pool->dtype == QW3_F16 ? 0 : 2) + (p.group <= 4 ? 1 : 0)];
     static std::atomic<bool> attr_set[64];   // per device: the kernels' shared-memory limit is raised once
     if (w->device >= 64 || !attr_set[w->device].load(std::memory_order_acquire)) {
-        QW3_CUDA(cudaFuncSetAttribute(attn_kv4_decode_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(KdSmem)));
-        QW3_CUDA(cudaFuncSetAttribute(attn_kv4_decode_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(KdSmem)));
+        for (const auto k : kernels) QW3_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(KdSmem)));
         if (w->device < 64) attr_set[w->device].store(true, std::memory_order_release);
     }
     QW3_CUDA(kv4_launch(kernel, dim3(grid), dim3(KD_THREADS), sizeof(KdSmem), static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, p));
