@@ -36,8 +36,8 @@ static_assert(2 * (size_t)KD_MAX_GRID * KD_PART <= WS_PARTIALS && KD_MAX_GRID <=
 struct KdSmem {
     uint8_t ring[KD_WARPS][KD_STAGES][KD_STAGE_BYTES];
     float4 o[KD_WARPS][8][32];        // sums of a warp, in the order of its fragments
-    struct { const uint8_t* at[2]; } src[KD_WARPS][32];   // tiles of the chunks that are looked up, and of each the tokens in them: 16 bits a tile
-    int tokens[KD_WARPS][32];
+    struct { const uint8_t* at[2]; } src[KD_WARPS][32];   // of the chunks that are looked up: the tiles (the second null where it follows the
+    int2 tokens[KD_WARPS][32];                            // first), the tokens in them, 16 bits a tile, and the bytes of the first copy
     float4 token[KD_WARPS][KD_CHUNK];  // of the chunk's tokens: scale of K * 2^24, minimum of K, log2 of V's scale, 1 / V's scale
     float mid[KD_WARPS][KD_CHUNK];     // and V's minimum + 8 * scale
     float stat[KD_WARPS][8][3];
@@ -235,9 +235,10 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
                 if (src1 != nullptr) tokens |= min(n1, 16) << 16;
             }
         }
+        const bool one = tokens >> 16 != 0 && src1 - src0 == KV4_TILE_BYTES;   // of one page
         sm.src[warp][lane].at[0] = src0;
-        sm.src[warp][lane].at[1] = src1;
-        sm.tokens[warp][lane] = tokens;
+        sm.src[warp][lane].at[1] = one ? nullptr : src1;
+        sm.tokens[warp][lane] = make_int2(tokens, one ? 2 * KV4_TILE_BYTES : (tokens & 0xffff) != 0 ? KV4_TILE_BYTES : 0);
         __syncwarp();
         // the next thirty-two are found from the last of these (used only where there is one)
         ahead.ht = __shfl_sync(0xffffffffu, q.ht, 31);
@@ -251,17 +252,12 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
         if (turn == 0) look_up();
         if (elect_one()) {
             const uint32_t bar = smem_u32(&sm.bar[warp][s]), to = smem_u32(sm.ring[warp][s]);
-            const int n = sm.tokens[warp][turn];
-            const uint8_t *const a = sm.src[warp][turn].at[0], *const b = sm.src[warp][turn].at[1];
-            const bool n0 = (n & 0xffff) != 0, n1 = n >> 16 != 0;
-            sm.valid[warp][s] = n;
-            mbar_expect_tx(bar, (n0 ? KV4_TILE_BYTES : 0) + (n1 ? KV4_TILE_BYTES : 0));
-            if (n0 && n1 && b - a == KV4_TILE_BYTES) {   // of one page
-                bulk_load(to, a, 2 * KV4_TILE_BYTES, bar);
-            } else {
-                if (n0) bulk_load(to, a, KV4_TILE_BYTES, bar);
-                if (n1) bulk_load(to + KV4_TILE_BYTES, b, KV4_TILE_BYTES, bar);
-            }
+            const int2 n = sm.tokens[warp][turn];
+            const uint8_t* const b = sm.src[warp][turn].at[1];
+            sm.valid[warp][s] = n.x;
+            mbar_expect_tx(bar, n.y + (b != nullptr ? KV4_TILE_BYTES : 0));
+            if (n.y != 0) bulk_load(to, sm.src[warp][turn].at[0], n.y, bar);
+            if (b != nullptr) bulk_load(to + KV4_TILE_BYTES, b, KV4_TILE_BYTES, bar);
         }
         __syncwarp();
         ++issued;
@@ -359,6 +355,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
             flushed = true;
         };
         clear();
+        float top0 = -INFINITY, top1 = -INFINITY, z0 = 0.0f, z1 = 0.0f;   // mu + 7, beyond which it has to follow, and mu - 8
         float mu0 = -INFINITY, mu1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, m0 = 0.0f, m1 = 0.0f;
 
         for (; warp + KD_WARPS * used < part_end; ++used) {
@@ -372,9 +369,15 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
             {   // lane i: what belongs to token i of the chunk; behind the last one nothing is left but codes, which are finite, times zero
                 const uint8_t* const tile = stage + (lane >> 4) * KV4_TILE_BYTES + 4 * (lane & 15);
                 const float2 ks = R::unpack(*reinterpret_cast<const uint32_t*>(tile + KV4_KP)), vs = R::unpack(*reinterpret_cast<const uint32_t*>(tile + KV4_VP));
-                const bool in = (lane & 15) < (sm.valid[warp][s] >> (lane & 16) & 0xffff);
-                sm.token[warp][lane] = in ? make_float4(ks.x * 16777216.0f, ks.y, kd_lg2(vs.x), kd_rcp(vs.x)) : make_float4(0.0f, 0.0f, -INFINITY, 0.0f);
-                sm.mid[warp][lane] = in ? fmaf(8.0f, vs.x, vs.y) : 0.0f;
+                const int valid = sm.valid[warp][s];
+                float4 of = make_float4(ks.x * 16777216.0f, ks.y, kd_lg2(vs.x), kd_rcp(vs.x));
+                float mid = fmaf(8.0f, vs.x, vs.y);
+                if (valid != (16 | 16 << 16) && (lane & 15) >= (valid >> (lane & 16) & 0xffff)) {
+                    of = make_float4(0.0f, 0.0f, -INFINITY, 0.0f);
+                    mid = 0.0f;
+                }
+                sm.token[warp][lane] = of;
+                sm.mid[warp][lane] = mid;
             }
             __syncwarp();
             float sum[2][4];     // of a tile: tokens row0, row0 + 8 x heads 2t, 2t + 1
@@ -419,7 +422,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
                     x0m = fmaxf(x0m, u[e][2 * h]);
                     x1m = fmaxf(x1m, u[e][2 * h + 1]);
                 }
-            if (__any_sync(0xffffffffu, x0m > mu0 + 7.0f || x1m > mu1 + 7.0f)) {   // rare after the first chunks
+            if (__any_sync(0xffffffffu, x0m > top0 || x1m > top1)) {   // rare after the first chunks
 #pragma unroll
                 for (int d = NARROW ? 2 : 4; d < 32; d *= 2) {
                     x0m = fmaxf(x0m, __shfl_xor_sync(0xffffffffu, x0m, d));
@@ -429,6 +432,10 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
                 const float r0 = mu0 == -INFINITY ? 0.0f : kd_ex2(mu0 - n0), r1 = mu1 == -INFINITY ? 0.0f : kd_ex2(mu1 - n1);
                 mu0 = n0;
                 mu1 = n1;
+                top0 = mu0 + 7.0f;
+                top1 = mu1 + 7.0f;
+                z0 = mu0 == -INFINITY ? 0.0f : mu0 - 8.0f;
+                z1 = mu1 == -INFINITY ? 0.0f : mu1 - 8.0f;
                 l0 *= r0; m0 *= r0;
                 l1 *= r1; m1 *= r1;
                 if (flushed || unflushed > 0) {
@@ -441,7 +448,6 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
                 clear();
             }
             ++unflushed;
-            const float z0 = mu0 == -INFINITY ? 0.0f : mu0 - 8.0f, z1 = mu1 == -INFINITY ? 0.0f : mu1 - 8.0f;
             uint32_t pp[TILES][2];
 #pragma unroll
             for (int e = 0; e < TILES; ++e)
