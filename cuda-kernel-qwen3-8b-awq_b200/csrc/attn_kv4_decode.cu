@@ -7,8 +7,9 @@
 // exponent: u_j = score_j + log2(sv_j), P_j = 2^(u_j - max u + 8) enters the second product as fp16 (the largest is between 2^8 and 2^15, so
 // the 11 bits reach 22 powers of two below it, whatever the scales are), and the sums of p and p (mv + 8 sv) take P_j / sv_j in fp32.
 // The sum of P code is far larger than that of P (code - 8), and the tensor cores cut off what an accumulator cannot hold, which
-// shortens it: one more product sums P * 8 the same way, and the difference goes to fp32 sums in shared memory after eight chunks
-// at most (a list of 40 K tokens: error KD_ERR of the output's size, 2.0e-3 without either).
+// shortens it: one more product sums P * 8 the same way, and the difference goes to fp32 sums in shared memory after sixteen
+// chunks at most (lists of 20 to 41 K tokens: error 3.3e-4 of the outputs' size, after one chunk the same; without the flush 9e-4, without
+// either 2.0e-3).  What is left is the rounding of P, 2.5e-4, and that of the output, 2.1e-4.
 //
 // A warp works on 32 tokens at a time, two tiles of 16 that bulk copies bring into its own ring of two: S^T = K Q^T (16 tokens x 8 heads
 // of the group), then O^T += V^T P^T, with mma.sync m16n8k16.  At 136 bytes a token and KV head the kernel is bound by HBM; one m16n8k16 a
@@ -25,7 +26,7 @@ namespace qw3 {
 
 constexpr int KD_WARPS = 4, KD_THREADS = 32 * KD_WARPS, KD_STAGES = 2, KD_CTAS = 3;   // CTAs an SM
 constexpr int KD_CHUNK = 32, KD_STAGE_BYTES = 2 * KV4_TILE_BYTES;
-constexpr int KD_FLUSH = 8;            // chunks whose products are summed in an accumulator
+constexpr int KD_FLUSH = 16;           // chunks whose products are summed in an accumulator
 constexpr int KD_MIN_CHUNKS = 8;       // chunks a CTA takes at least
 constexpr int KD_WHOLE = 32;           // pairs of so many chunks are not cut: joining two parts costs some 4 us, eight chunks a warp 3
 constexpr int KD_PAIR = 6;             // what a pair costs a CTA beside its chunks (q, joining the warps' states), in chunks
