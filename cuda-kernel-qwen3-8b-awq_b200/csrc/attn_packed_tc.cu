@@ -14,11 +14,13 @@
 //   warps 4..7, 8..11   one row a thread of the upper / lower tile: S from tensor memory, online softmax, P back in its place
 // Tensor memory, per tile: O 128 columns, S 128, of which P takes the upper half as the exponentials consume it: the keys 64..127 first, so that
 // their product runs under the exponentials of the others.  While one tile is in its softmax the tensor cores work for the other.
-// 128 keys a tile: an MMA of 128 x 64 x 16 takes 48 cycles of shared-memory reads for 32 of products (64 keys a tile: 135 us for
-// 4001 rows, 129 with the softmax left out), one of 128 x 128 x 16 64 for 64.
+// 128 keys a tile: an MMA of 128 x 64 x 16 takes 48 cycles of shared-memory reads for 32 of products (with the softmax left out, before CTAs
+// were persistent, 4001 rows took 129 us with 64 keys a tile and 110 with 128), one of 128 x 128 x 16 64 for 64.
 // P is rounded to the rows' type, whose 8 or 11 bits the result has as well; its sum is taken before.  An fp16 P is kept between 2^8 and
 // 2^15 at the row's maximum, so that its normal numbers reach 22 powers of two below.  O is rescaled only when a row's maximum has grown by
 // more than 7 (bf16: 8) powers of two.
+// 4001 rows, 32 heads over 8 KV heads, bf16: 125 us, 1050 TFLOP/s, 0.63 of the measured rate (137 us in sustained use).  The tensor pipe is active
+// in 58 % of active cycles, the exponential unit in 40 %; a softmax warp waits 1140 of some 3660 cycles a tile for scores.
 // All waits are bounded.  After one that gives up the error word is set, rows that are not finished are written as NaN, and the CTA
 // leaves when its copies and MMAs in flight are done.
 #include <atomic>

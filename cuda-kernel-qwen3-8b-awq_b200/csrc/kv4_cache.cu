@@ -10,7 +10,8 @@ namespace qw3 {
 // ---- block tables and slots ------------------------------------------------------------------------------------------------------
 // One cluster.  Every CTA sums the lengths of all requests for itself (two prefix sums, of new tokens and of new pages, kept in shared
 // memory), the cluster meets once, so that outputs may be the inputs' own buffers, and then its threads fill the lists: a thread takes
-// four tokens in a row and finds their request by bisection.  Bound by latency: two dependent rounds of global loads.
+// four tokens in a row and finds their request by bisection.  Bound by latency, two dependent rounds of global loads: 10.3 us
+// for 7 requests, 14.4 for 250 with 34 K new tokens (launch included, caches cold).
 constexpr int PS_THREADS = 512;
 constexpr int PS_MAX_REQ = 16384;
 
@@ -287,7 +288,9 @@ rope_kv4_append_kernel(const Qw3Kv4Pool pool, const Qw3Kv4AppendArgs p, int* err
 }
 
 // ---- rows read back --------------------------------------------------------------------------------------------------------------
-// A half-warp takes four rows at a time: four bytes of codes in, sixteen out, a lane, of K and of V.  A slot below zero gives zeros.
+// A half-warp takes four rows at a time: four bytes of codes in, sixteen out, a lane, of K and of V.  A slot below zero gives zeros.  30011
+// tokens of 8 KV heads, 156 MB: 30 us, 5.2 TB/s, 0.81 of the measured copy rate (before several rows were loaded
+// at once: 43 us).
 constexpr int RD_THREADS = 256, RD_GROUPS = RD_THREADS / 16, RD_ROWS = 4;
 
 template <class T>
