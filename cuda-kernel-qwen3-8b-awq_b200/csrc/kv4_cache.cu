@@ -13,6 +13,7 @@ namespace qw3 {
 // four tokens in a row and finds their request by bisection.  Bound by latency, two dependent rounds of global loads: 10.3 us
 // for 7 requests, 14.4 for 250 with 34 K new tokens (launch included, caches cold).
 constexpr int PS_THREADS = 512;
+constexpr int PS_CLUSTER = 8;   // one CTA instead: the same up to 2500 new tokens of 8 requests (10.2 us), 16.4 instead of 10.2 for 8000, 41 instead of 14.3 for 34000
 constexpr int PS_MAX_REQ = 16384;
 
 __global__ void __launch_bounds__(PS_THREADS) page_slots_kernel(const Qw3PageArgs p, int* err) {
@@ -75,8 +76,7 @@ __global__ void __launch_bounds__(PS_THREADS) page_slots_kernel(const Qw3PageArg
     }
     if (tid == 0) { cu[n] = (int)total; off[n] = (int)total_pages; }
     // all CTAs have read the lengths and the number of free pages
-    if (gridDim.x > 1) cooperative_groups::this_cluster().sync();
-    else __syncthreads();
+    cooperative_groups::this_cluster().sync();
 
     const int first = blockIdx.x * PS_THREADS + tid, step = gridDim.x * PS_THREADS;
     const auto find = [n](const int* starts, int i) {   // the last request that starts at or before i
@@ -129,7 +129,8 @@ __global__ void __launch_bounds__(PS_THREADS) page_slots_kernel(const Qw3PageArg
 }
 
 // ---- rotation, quantisation, store -----------------------------------------------------------------------------------------------
-// A CTA takes the rows of one token, or, of few tokens, a slice of them, so that all SMs take part; bulk copies bring them, while slot,
+// A CTA takes the rows of one token, a slice of 96 at most (slices of 16 for few tokens: the same up to 33 tokens, 12.4 instead of
+// 10.2 us for 280 tokens of 32 / 32 heads); bulk copies bring them, while slot,
 // position and the cosines and sines, which the lanes keep for all heads, are looked up.  A warp takes two rows at a time, eight dims a
 // lane.  Products and sums of the rotation are rounded one by one (no contraction), so that a row's codes do not depend on the compiler.  K
 // is quantised from the fp32 rotated row, not from its rounding.  Bound by issue slots: 4001 tokens, 32 KV
@@ -379,8 +380,7 @@ int qw3_page_slots(const Qw3PageArgs* a, qw3_ws_t ws, void* stream) {
     if (rc != QW3_OK) return rc;
     const size_t smem = (size_t)(3 * a->n_req + 2) * 4;
     if (smem > 48 * 1024) QW3_CUDA(cudaFuncSetAttribute(page_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * PS_MAX_REQ + 2) * 4));
-    const int cluster = a->max_tokens > 4 * PS_THREADS ? 8 : 1;
-    QW3_CUDA(kv4_launch(page_slots_kernel, dim3(cluster), dim3(PS_THREADS), smem, static_cast<cudaStream_t>(stream), ws_pdl(ws), cluster, *a, ws_struct(ws)->err));
+    QW3_CUDA(kv4_launch(page_slots_kernel, dim3(PS_CLUSTER), dim3(PS_THREADS), smem, static_cast<cudaStream_t>(stream), ws_pdl(ws), PS_CLUSTER, *a, ws_struct(ws)->err));
     return QW3_OK;
 }
 
@@ -402,8 +402,7 @@ int qw3_rope_kv4_append(const Qw3Kv4Pool* pool, const Qw3Kv4AppendArgs* a, qw3_w
                 "%s: rows and tables must be 16-byte aligned", who);
     const auto kernel = pool->dtype == QW3_F16 ? (a->layout == QW3_ROPE_PAIRS ? rope_kv4_append_kernel<__half, true> : rope_kv4_append_kernel<__half, false>)
                                                : (a->layout == QW3_ROPE_PAIRS ? rope_kv4_append_kernel<__nv_bfloat16, true> : rope_kv4_append_kernel<__nv_bfloat16, false>);
-    // few tokens: slices of some sixteen rows side by side
-    const int rows = a->heads + 2 * pool->kv_heads, most = a->tokens < 2 * ws_struct(ws)->sm_count ? 16 : AP_MAX_ROWS, slices = (rows + most - 1) / most;
+    const int rows = a->heads + 2 * pool->kv_heads, slices = (rows + AP_MAX_ROWS - 1) / AP_MAX_ROWS;
     const size_t smem = 256 * ((size_t)(a->heads + slices - 1) / slices + 2 * ((size_t)(pool->kv_heads + slices - 1) / slices));
     QW3_CUDA(kv4_launch(kernel, dim3((unsigned)a->tokens, slices), dim3(AP_THREADS), smem, static_cast<cudaStream_t>(stream), ws_pdl(ws), 1, *pool, *a, ws_struct(ws)->err));
     return QW3_OK;
