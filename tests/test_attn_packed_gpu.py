@@ -277,3 +277,21 @@ def test_packed_many_sequences(ops, cuda):
     got = ops.attn_packed(q, k, v, _cu(lens, cuda), _cu(lens, cuda), ws)
     ws.check()
     _check(got, q, k, v, lens, lens)
+
+
+def test_packed_on_two_streams_at_once(ops, cuda):
+    lens = ([700, 3, 90], [900, 3, 90])
+    q, k, v = _rows(*lens, 8, 2, torch.bfloat16, cuda, seed=31)
+    cu = _cu(lens[0], cuda), _cu(lens[1], cuda)
+    want = ops.attn_packed(q, k, v, *cu, ops.Workspace())
+    torch.cuda.synchronize()
+    streams, ws, got = [torch.cuda.Stream() for _ in range(2)], [ops.Workspace(pdl=True) for _ in range(2)], []
+    for _ in range(8):
+        for s, w in zip(streams, ws):
+            with torch.cuda.stream(s):
+                got.append(ops.attn_packed(q, k, v, *cu, w))
+    torch.cuda.synchronize()
+    for w in ws:
+        w.check()
+    assert all(torch.equal(x, want) for x in got)
+    _check(want, q, k, v, *lens)

@@ -505,3 +505,61 @@ def test_decode_step_captured_in_a_graph(ops, cuda):
     ws.check()
     assert torch.equal(cache.pages.cpu(), pool.bytes)
     assert lens.tolist() == [len(h) for h in held] and n_free.item() == n_pages - sum(-(-len(h) // page) for h in held)
+
+
+# ---- the widest calls, and one workspace in turn ---------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n,page,ctx_max,new_max,pad", [(16384, 16, 20, 1, 9), (16384, 64, 3, 2, 0)])
+def test_page_slots_of_the_most_requests(ops, cuda, n, page, ctx_max, new_max, pad):
+    test_page_slots(ops, cuda, n, page, ctx_max, new_max, pad)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("pairs", [False, True])
+@pytest.mark.parametrize("tokens,heads,kv,page,rot,pad,extra", [(2, 97, 3, 16, 128, 0, 0), (5, 96, 48, 32, 64, 1, 0), (1, 94, 1, 16, 0, 0, 0), (3, 300, 4, 16, 128, 0, 32),
+                                                                (301, 95, 1, 16, 128, 2, 0)])
+def test_append_in_slices_of_rows(ops, cuda, dtype, pairs, tokens, heads, kv, page, rot, pad, extra):
+    """Tokens of 96 rows and more: slices of different sizes, some without rows of k or v."""
+    test_append_and_read(ops, cuda, dtype, pairs, tokens, heads, kv, page, rot, pad, extra)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_same_slot_read_many_times(ops, cuda, dtype):
+    pool = ref.Pool(3, 16, 2, dtype)
+    g = _gen(21)
+    pool.put_rows(list(range(48)), torch.randn(48, 2, 128, generator=g), torch.randn(48, 2, 128, generator=g))
+    cache, ws = ops.Kv4Cache(pool.bytes.to(cuda), 16, 2, dtype), ops.Workspace()
+    slots = [5, 5, 47, -1, 5, 0, 47, 0] * 9
+    once_k, once_v = ops.kv4_read(cache, _i32(list(range(48)), cuda), ws)
+    k, v = ops.kv4_read(cache, _i32(slots, cuda), ws)
+    ws.check()
+    for i, s in enumerate(slots):
+        assert torch.equal(k[i], once_k[s] if s >= 0 else torch.zeros_like(k[i])) and torch.equal(v[i], once_v[s] if s >= 0 else torch.zeros_like(v[i]))
+
+
+def test_two_graphs_share_a_workspace_in_turn(ops, cuda):
+    """Decode leaves its counters as it found them, so the graphs may alternate on a stream, packed attention of the same workspace between them."""
+    heads, kv, page, dtype = 8, 2, 32, torch.float16
+    ws, calls = ops.Workspace(pdl=True), []
+    for lens, seed in (([2100, 0, 33], 5), ([1, 40, 3000], 6)):
+        pool, table, rows, q = _case(lens, heads, kv, page, dtype, seed=seed)
+        d_cache, d_q, d_t, d_l = ops.Kv4Cache(pool.bytes.to(cuda), page, kv, dtype), q.to(cuda), _i32(table, cuda), _i32(lens, cuda)
+        want = ops.attn_kv4_decode(d_q, d_cache, d_t, d_l, ops.Workspace())
+        torch.cuda.synchronize()
+        ops.attn_kv4_decode(d_q, d_cache, d_t, d_l, ws)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.attn_kv4_decode(d_q, d_cache, d_t, d_l, ws)
+        calls.append((graph, out, want, d_cache, d_q, d_t, d_l))
+    g = torch.Generator(device=cuda).manual_seed(2)
+    x = [torch.randn(300, h, 128, device=cuda, generator=g).half() for h in (heads, kv, kv)]
+    cu = _i32([0, 100, 300], cuda)
+    packed = ops.attn_packed(*x, cu, cu, ops.Workspace())
+    for _ in range(6):
+        for graph, out, want, *_ in calls:
+            out.fill_(7.0)
+            graph.replay()
+            assert torch.equal(ops.attn_packed(*x, cu, cu, ws), packed)
+            assert torch.equal(out, want)
+    ws.check()
