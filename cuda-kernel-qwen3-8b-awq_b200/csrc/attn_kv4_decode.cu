@@ -14,7 +14,7 @@
 // A warp works on 32 tokens at a time, two tiles of 16 that bulk copies bring into its own ring of two: S^T = K Q^T (16 tokens x 8 heads
 // of the group), then O^T += V^T P^T, with mma.sync m16n8k16: one product a token and KV head is a third of what the warp-level path can
 // issue while HBM brings the 136 bytes, and its operands need no pass through tensor memory.
-// 48 requests of 20 to 41 K tokens, 32 heads over 8 KV heads, 1.66 GB: 303 us, 5.5 TB/s, 0.85 of the measured copy rate (341 in sustained
+// 48 requests of 20 to 41 K tokens, 32 heads over 8 KV heads, 1.66 GB: 303 us, 5.5 TB/s, 0.85 of the measured copy rate (342 in sustained
 // use).  No unit is saturated (16 requests of 16384 tokens: ALU pipe 51 % of active cycles, warp-level tensor pipe 28 %, issue slots 48 %).  When
 // the kernel took 332 us, copies without products took 272 and products without copies 276: neither alone explains the time.
 // The 32-token chunks of all (KV head, request) pairs form one list that is cut into equal parts, one a CTA, whatever the lengths are; the four
