@@ -8,15 +8,15 @@
 // the 11 bits reach 22 powers of two below it, whatever the scales are), and the sums of p and p (mv + 8 sv) take P_j / sv_j in fp32.
 // The sum of P code is far larger than that of P (code - 8), and the tensor cores cut off what an accumulator cannot hold, which
 // shortens it: one more product sums P * 8 the same way, and the difference goes to fp32 sums in shared memory after sixteen
-// chunks at most (lists of 20 to 41 K tokens: error 3.3e-4 of the outputs' size, after one chunk the same; without the flush 9e-4, without
-// either 2e-3).  What is left is the rounding of P, 2.5e-4, and that of the output, 2.1e-4.
+// chunks at most (lists of 20 to 41 K tokens: error 3.4e-4 of the outputs' size, after one chunk the same; without the flush 9e-4, without
+// either 2e-3; 2.6e-4 with the low terms of P that fp16 rows and groups of four heads at most have, 2.1e-4 being that of the output's own rounding).
 //
 // A warp works on 32 tokens at a time, two tiles of 16 that bulk copies bring into its own ring of two: S^T = K Q^T (16 tokens x 8 heads
 // of the group), then O^T += V^T P^T, with mma.sync m16n8k16: one product a token and KV head is a third of what the warp-level path can
 // issue while HBM brings the 136 bytes, and its operands need no pass through tensor memory.
-// 48 requests of 20 to 41 K tokens, 32 heads over 8 KV heads, 1.66 GB: 303 us, 5.5 TB/s, 0.85 of the measured copy rate (342 in sustained
-// use).  No unit is saturated (16 requests of 16384 tokens: ALU pipe 51 % of active cycles, warp-level tensor pipe 28 %, issue slots 48 %).  When
-// the kernel took 332 us, copies without products took 272 and products without copies 276: neither alone explains the time.
+// 48 requests of 20 to 41 K tokens, 32 heads over 8 KV heads, fp16, 1.66 GB: 311 us, 5.3 TB/s, 0.83 of the measured copy rate (348 in
+// sustained use).  16 requests of 16384 tokens: ALU pipe 51 % of active cycles, warp-level tensor pipe 28 %, issue slots 49 %: no unit is saturated.  When the kernel took
+// 332 us, copies without products took 272 and products without copies 276: neither alone explains the time.
 // The 32-token chunks of all (KV head, request) pairs form one list that is cut into equal parts, one a CTA, whatever the lengths are; the four
 // warps of a CTA take its chunks in turn and join their states in shared memory, and pairs that are cut by the border of a CTA are joined
 // from the workspace by the last CTA to arrive, in order of the parts: results do not depend on timing.
@@ -96,13 +96,15 @@ struct KdPlace {
 };
 
 // NARROW: groups of four heads at most, which leave half of a fragment's columns empty.  The lanes of the empty columns take the scores of the
-// second tile, so that each has half as many exponentials; what they put into the products' empty columns is read by nobody.
-// 48 requests of 20 to 41 K tokens, groups of four: 303 us, without it 315; short requests the same.
+// second tile, so that each has half as many exponentials; fp16 rows use the products' empty columns for
+// what the rounding of P to fp16 took off (bf16 rows round the result so much more that it does not show: 1.67e-3 with and without): 48 requests of
+// 20 to 41 K tokens 311 us and an error of 2.6e-4, without the low terms 303 and 3.4e-4, without NARROW 315; short requests the same.
 template <class T, bool NARROW>
 __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(KdParams p) {
     extern __shared__ __align__(128) uint8_t kd_smem[];
     KdSmem& sm = *reinterpret_cast<KdSmem*>(kd_smem);
     using R = RowType<T>;
+    constexpr bool LOW = NARROW && R::FLOOR > 1e-9f;   // fp16 rows
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int B = p.a.n_req, tiles_page = p.pool.page_size / 16;
     pdl_launch_dependents();
@@ -454,7 +456,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
                 clear();
             }
             ++unflushed;
-            uint32_t pp[TILES][2];
+            uint32_t pp[TILES][2], low[2], other[2];   // P; LOW: what its rounding took off; what the lane needs from the one opposite
 #pragma unroll
             for (int e = 0; e < TILES; ++e)
 #pragma unroll
@@ -467,13 +469,20 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
                     m0 = fmaf(w0, mid, m0);
                     m1 = fmaf(w1, mid, m1);
                     pp[e][h] = RowType<__half>::pack(p0, p1);
+                    if (LOW) {
+                        const float2 rounded = RowType<__half>::unpack(pp[e][h]);
+                        low[h] = RowType<__half>::pack(p0 - rounded.x, p1 - rounded.y);
+                    } else {
+                        low[h] = pp[e][h];
+                    }
+                    if (NARROW) other[h] = __shfl_xor_sync(0xffffffffu, t < 2 ? low[h] : pp[e][h], 2);
                 }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const uint8_t* const tile = stage + e * KV4_TILE_BYTES + KV4_V;
                 uint32_t pf[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) pf[h] = kd_transpose(!NARROW ? pp[e % TILES][h] : e == 0 ? pp[0][h] : __shfl_xor_sync(0xffffffffu, pp[0][h], 2));
+                for (int h = 0; h < 2; ++h) pf[h] = kd_transpose(!NARROW ? pp[e % TILES][h] : t < 2 ? (e == 0 ? pp[0][h] : other[h]) : (e == 0 ? other[h] : low[h]));
                 const int ra = 2 * t + (t & 1), rb = 2 * t + (~t & 1);   // tokens of indexes 2t and 2t + 1
                 const uint2 a0 = *reinterpret_cast<const uint2*>(tile + ra * 64 + 8 * g), b0 = *reinterpret_cast<const uint2*>(tile + rb * 64 + 8 * g);
                 const uint2 a1 = *reinterpret_cast<const uint2*>(tile + ra * 64 + 512 + 8 * g), b1 = *reinterpret_cast<const uint2*>(tile + rb * 64 + 512 + 8 * g);
@@ -509,7 +518,7 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
         flush(1.0f, 1.0f);
         __syncthreads();
         // thread (i, lane): dims 16 g + 4 i .. + 3 of heads 2t and 2t + 1
-        const int i = warp;
+        const int i = warp, ts = NARROW ? t & 1 : t;   // statistics of its heads
         float top[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, m[2] = {0.0f, 0.0f};
         float4 lo = make_float4(0, 0, 0, 0), hi = make_float4(0, 0, 0, 0);
         const auto add = [&](int h, float mu, float sl, float smv) {   // joins a state's sums of head 2t + h; returns its factor
@@ -528,13 +537,20 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
 #pragma unroll
         for (int w = 0; w < KD_WARPS; ++w)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) top[h] = fmaxf(top[h], sm.stat[w][2 * t + h][0]);
+            for (int h = 0; h < 2; ++h) top[h] = fmaxf(top[h], sm.stat[w][2 * ts + h][0]);
 #pragma unroll
         for (int w = 0; w < KD_WARPS; ++w) {
-            const float* const st = sm.stat[w][2 * t];
+            const float* const st = sm.stat[w][2 * ts];
             const float fa = add(0, st[0], st[1], st[2]), fb = add(1, st[3], st[4], st[5]);
             accumulate(lo, sm.o[w][2 * i][lane], fa, fb);
             accumulate(hi, sm.o[w][2 * i + 1][lane], fa, fb);
+        }
+        if (LOW) {   // the sums of P and of what its rounding took off
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                (&lo.x)[e] += __shfl_xor_sync(0xffffffffu, (&lo.x)[e], 2);
+                (&hi.x)[e] += __shfl_xor_sync(0xffffffffu, (&hi.x)[e], 2);
+            }
         }
         int first = 0, parts = 1;   // CTAs that have a part of the pair
         if (place.n > KD_WHOLE && (place.c > 0 || done + place.n > n_mine)) {

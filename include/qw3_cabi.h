@@ -267,7 +267,8 @@ typedef struct Qw3AttnKv4Args {
 } Qw3AttnKv4Args;
 
 /* Attention of one token a request over its cached tokens (attentionKernel, Inference.cu:182-266, intended math), read as codes: the rows
- * are never expanded.  Scores, probabilities' sums and outputs are fp32; probabilities times V scales enter the products as fp16. */
+ * are never expanded.  Scores, probabilities' sums and outputs are fp32; probabilities times V scales enter the products as
+ * fp16 (fp16 rows, groups of four heads at most: as two fp16 terms). */
 int qw3_attn_kv4_decode(const Qw3Kv4Pool* pool, const Qw3AttnKv4Args* args, qw3_ws_t ws, void* stream);
 
 typedef struct Qw3AttnPackedArgs {
