@@ -378,8 +378,10 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
                 const uint8_t* const tile = stage + (lane >> 4) * KV4_TILE_BYTES + 4 * (lane & 15);
                 const float2 ks = R::unpack(*reinterpret_cast<const uint32_t*>(tile + KV4_KP)), vs = R::unpack(*reinterpret_cast<const uint32_t*>(tile + KV4_VP));
                 const int valid = sm.valid[warp][s];
-                float4 of = make_float4(ks.x * 16777216.0f, ks.y, kd_lg2(vs.x), kd_rcp(vs.x));
-                float mid = fmaf(8.0f, vs.x, vs.y);
+                // V's scale below the floor, 0 in a row of zero bytes that append never wrote, is taken for the floor: a logarithm of 0 has no use
+                const float sv = vs.x >= 0.0f ? fmaxf(vs.x, R::FLOOR) : NAN;
+                float4 of = make_float4(ks.x * 16777216.0f, ks.y, kd_lg2(sv), kd_rcp(sv));
+                float mid = fmaf(8.0f, sv, vs.y);
                 if (valid != (16 | 16 << 16) && (lane & 15) >= (valid >> (lane & 16) & 0xffff)) {
                     of = make_float4(0.0f, 0.0f, -INFINITY, 0.0f);
                     mid = 0.0f;

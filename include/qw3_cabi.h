@@ -185,6 +185,7 @@ int qw3_attn_prefill_poll_once(const void* d_qkv, const void* d_k_cache, const v
  * in fp32, T() rounding to the rows' type; the floor is 2^-24 (fp16) or 2^-60 (bf16).  A row with Inf or NaN (bf16: or with a range
  * of more than 15 * 2^60) reads back as NaN.  16 tokens of a KV head lie together in 2176 bytes: 16 rows of 64 bytes of K codes (byte i:
  * dim 2i in the low nibble), the same of V, 16 pairs (scale, minimum) of K, 16 of V; a page is [kv_heads][page_size / 16] of these.
+ * A row of zero bytes, which was never stored, stands for zeros; qw3_attn_kv4_decode takes a V scale below the floor for the floor.
  *
  * A slot is page * page_size + offset.  What the device finds out of range (slots, pages, positions, lengths) is left out, never read
  * or written, and recorded: qw3_ws_check returns QW3_ERR_RANGE.  The workspace must belong to the current device. */
