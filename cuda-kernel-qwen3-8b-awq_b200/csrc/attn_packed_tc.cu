@@ -78,8 +78,9 @@ struct PackedBlock {
     int q0, k0, nq, nk, block, head0;
 };
 
-// One row by a warp, from global memory and in 32-bit arithmetic: rows whose tile holds Inf or NaN in V behind the row.  The tensor
-// cores multiply these by the zeros of the masked probabilities, and the sum is NaN; here nothing past the row's last key is read.
+// One row by a warp, from global memory and in 32-bit arithmetic: rows whose tile holds Inf or NaN in V behind the row, or whose sum of P V passes
+// fp32.  The tensor cores multiply what is behind the row by the zeros of the masked probabilities, and the sum is NaN; here nothing past the row's
+// last key is read.
 template <class T>
 __device__ __noinline__ void packed_row(const T* q, const T* k, long long k_stride, const T* v, long long v_stride, int n_keys, float c, T* dst, int lane) {
     using R = RowType<T>;
@@ -119,6 +120,49 @@ __device__ __noinline__ void packed_row(const T* q, const T* k, long long k_stri
     }
     for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
     *reinterpret_cast<uint2*>(dst + 4 * lane) = make_uint2(R::pack(o[0] / l, o[1] / l), R::pack(o[2] / l, o[3] / l));
+}
+
+// Which of a warp's rows (`rows`, one a lane: its last key `pos`, its stored result `dst`) have to be done again: those with a value that is not
+// finite in a dim where no V row that they see has Inf or NaN.  The others are what the definition gives, however many they are.  One pass
+// over V, up to the first such value in every dim that is asked for: 32 keys a step.
+template <class T>
+__device__ __noinline__ uint32_t packed_spoiled(uint32_t rows, int pos, const T* dst, const T* v, long long v_stride, int lane) {
+    using R = RowType<T>;
+    const auto bad = [](uint2 w) {   // of the lane's four dims, a bit each
+        const float2 a = R::unpack(w.x), b = R::unpack(w.y);
+        return (a.x - a.x != 0.0f ? 1u : 0u) | (a.y - a.y != 0.0f ? 2u : 0u) | (b.x - b.x != 0.0f ? 4u : 0u) | (b.y - b.y != 0.0f ? 8u : 0u);
+    };
+    const auto result = [&](int row) {
+        const T* const at = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), row));
+        return bad(*reinterpret_cast<const uint2*>(at + 4 * lane));
+    };
+    uint32_t asked = 0;
+    for (uint32_t m = rows; m != 0; m &= m - 1) asked |= result(__ffs(m) - 1);
+    const int n = __reduce_max_sync(0xffffffffu, rows >> lane & 1 ? pos + 1 : 0);
+    int first[4] = {0x7fffffff, 0x7fffffff, 0x7fffffff, 0x7fffffff};   // key of the first Inf or NaN in a dim
+    for (int k0 = 0; k0 < n && __any_sync(0xffffffffu, asked != 0); k0 += 32)
+        for (int j0 = 0; j0 < 32; j0 += 8) {
+            uint2 w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = k0 + j0 + j < n ? *reinterpret_cast<const uint2*>(v + (k0 + j0 + j) * v_stride + 4 * lane) : make_uint2(0, 0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t now = bad(w[j]) & asked;
+                asked &= ~now;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) first[e] = now >> e & 1 ? k0 + j0 + j : first[e];
+            }
+        }
+    uint32_t again = 0;
+    for (uint32_t m = rows; m != 0; m &= m - 1) {
+        const int row = __ffs(m) - 1, last = __shfl_sync(0xffffffffu, pos, row);
+        const uint32_t b = result(row);
+        bool spoiled = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) spoiled |= (b >> e & 1) != 0 && first[e] > last;
+        if (__any_sync(0xffffffffu, spoiled)) again |= 1u << row;
+    }
+    return again;
 }
 
 template <class T>
@@ -561,13 +605,17 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 }
             }
             __syncwarp();   // a row that is done again has been stored
-            for (uint32_t redo = ok ? __ballot_sync(0xffffffffu, mine && pos >= 0 && finite != 0.0f) : 0u; redo != 0; redo &= redo - 1) {
-                const int rr = 32 * q + __ffs(redo) - 1, tok = tile_tokens * t + rr / pack, head = b.head0 + rr % pack;
-                const int kv_head = head / (p.a.heads / p.a.kv_heads);
-                packed_row<T>(static_cast<const T*>(p.a.d_q) + (b.q0 + sh.t0 + tok) * p.a.q_stride + head * 128,
-                              static_cast<const T*>(p.a.d_k) + b.k0 * p.a.k_stride + kv_head * 128, p.a.k_stride,
-                              static_cast<const T*>(p.a.d_v) + b.k0 * p.a.v_stride + kv_head * 128, p.a.v_stride, sh.past + sh.t0 + tok + 1, c,
-                              out + ((size_t)tok * p.a.heads + rr % pack) * 128, lane);
+            // a sum that is not finite is that of scores the row sees, and its result is NaN whatever is done
+            uint32_t redo = ok ? __ballot_sync(0xffffffffu, mine && pos >= 0 && finite != 0.0f && l - l == 0.0f) : 0u;
+            if (redo != 0) {
+                const int kv_head = b.head0 / (p.a.heads / p.a.kv_heads);
+                const T* const k_rows = static_cast<const T*>(p.a.d_k) + b.k0 * p.a.k_stride + kv_head * 128;
+                const T* const v_rows = static_cast<const T*>(p.a.d_v) + b.k0 * p.a.v_stride + kv_head * 128;
+                for (redo = packed_spoiled<T>(redo, pos, dst, v_rows, p.a.v_stride, lane); redo != 0; redo &= redo - 1) {
+                    const int rr = 32 * q + __ffs(redo) - 1, tok = tile_tokens * t + rr / pack, head = b.head0 + rr % pack;
+                    packed_row<T>(static_cast<const T*>(p.a.d_q) + (b.q0 + sh.t0 + tok) * p.a.q_stride + head * 128, k_rows, p.a.k_stride, v_rows, p.a.v_stride,
+                                  sh.past + sh.t0 + tok + 1, c, out + ((size_t)tok * p.a.heads + rr % pack) * 128, lane);
+                }
             }
         }
     }
