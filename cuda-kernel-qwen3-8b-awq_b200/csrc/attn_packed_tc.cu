@@ -108,14 +108,19 @@ __device__ __noinline__ void packed_row(const T* q, const T* k, long long k_stri
         l = l * f + pr;   // this lane's keys
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] *= f;
-        for (int j = 0; j < 32 && k0 + j < n_keys; ++j) {
-            const float pj = __shfl_sync(0xffffffffu, pr, j);
-            const uint2 w = *reinterpret_cast<const uint2*>(v + (k0 + j) * v_stride + 4 * lane);
-            const float2 a = R::unpack(w.x), b = R::unpack(w.y);
-            o[0] = fmaf(pj, a.x, o[0]);
-            o[1] = fmaf(pj, a.y, o[1]);
-            o[2] = fmaf(pj, b.x, o[2]);
-            o[3] = fmaf(pj, b.y, o[3]);
+        for (int j0 = 0; j0 < 32; j0 += 8) {   // eight loads on their way at once
+            uint2 w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[j] = k0 + j0 + j < n_keys ? *reinterpret_cast<const uint2*>(v + (k0 + j0 + j) * v_stride + 4 * lane) : make_uint2(0, 0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float pj = __shfl_sync(0xffffffffu, pr, j0 + j);
+                const float2 a = R::unpack(w[j].x), b = R::unpack(w[j].y);
+                o[0] = fmaf(pj, a.x, o[0]);
+                o[1] = fmaf(pj, a.y, o[1]);
+                o[2] = fmaf(pj, b.x, o[2]);
+                o[3] = fmaf(pj, b.y, o[3]);
+            }
         }
     }
     for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
