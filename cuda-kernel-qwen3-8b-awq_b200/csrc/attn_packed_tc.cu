@@ -21,8 +21,9 @@
 // more than 7 (bf16: 8) powers of two.
 // 4001 rows, 32 heads over 8 KV heads, bf16: 125 us, 1050 TFLOP/s, 0.63 of the measured rate (136 us in sustained use).  The tensor pipe is active
 // in 58 % of active cycles, the exponential unit in 40 %; a softmax warp waits 1140 of some 3660 cycles a tile for scores.
-// All waits are bounded.  After one that gives up the error word is set, rows that are not finished are written as NaN, and the CTA
-// leaves when its copies and MMAs in flight are done.
+// All waits are bounded, by a second and what 32 rows done again may take: over 250000 keys 1.1 s, and the block behind them waits for that.
+// After a wait that gives up the error word is set, the rows that the CTA has begun are written as NaN, blocks that no other CTA takes stay
+// as they were, and the CTA leaves when its copies and MMAs in flight are done.
 #include <atomic>
 
 #include "kv4.cuh"
@@ -34,6 +35,7 @@ constexpr int PK_ROWS = 128, PK_KEYS = 128, PK_STAGES = 5;
 constexpr int PK_THREADS = 384;
 constexpr int PK_Q_BYTES = PK_ROWS * 256;   // one tile of q rows: two halves of 64 dims
 constexpr int PK_KV_BYTES = PK_KEYS * 256;  // one tile of K or V
+constexpr long long PK_REDO_TICKS = 32 * 1024;   // a key: four times what a warp was away for that did 32 rows again over 250000 keys
 constexpr size_t PK_SMEM = 2 * PK_Q_BYTES + (size_t)PK_STAGES * PK_KV_BYTES + 512;
 
 __device__ __forceinline__ float pk_ex2(float x) {
@@ -67,6 +69,7 @@ constexpr int PK_FMA = 5;   // of sixteen pairs of exponentials, those on the FM
 struct PackedParams {
     Qw3AttnPackedArgs a;
     float c;        // scale * log2(e)
+    long long limit;   // clock ticks after which a wait gives up
     int pack;       // heads that share a tile
     int* ticket;    // the next block to be taken, and the CTAs that are done; zero between launches
     int* done;
@@ -77,6 +80,16 @@ struct PackedParams {
 struct PackedBlock {
     int q0, k0, nq, nk, block, head0;
 };
+
+// As mbar_wait, with a limit of the call's own.
+__device__ __forceinline__ bool packed_wait(uint32_t bar, uint32_t parity, long long limit) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity)) {
+        if (clock64() - t0 > limit) return false;
+    }
+    return true;
+}
 
 // One row by a warp, from global memory and in 32-bit arithmetic: rows whose tile holds Inf or NaN in V behind the row, or whose sum of P V passes
 // fp32.  The tensor cores multiply what is behind the row by the zeros of the masked probabilities, and the sum is NaN; here nothing past the row's
@@ -188,6 +201,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                    drain = place_empty + 16, v_last = drain + 8, v_clean = v_last + 8;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * PK_STAGES + 19);
     volatile int* s_dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const auto wait = [&](uint32_t bar, uint32_t parity) { return packed_wait(bar, parity, p.limit); };
 
     const auto give_up = [&](int code) {
         atomicCAS(p.err, 0, code);
@@ -293,7 +307,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 }
             }
             const uint32_t at = 8 * (k & 1);
-            if (k > 1 && !__all_sync(0xffffffffu, mbar_wait(place_empty + at, (uint32_t)((k >> 1) - 1) & 1u))) {
+            if (k > 1 && !__all_sync(0xffffffffu, wait(place_empty + at, (uint32_t)((k >> 1) - 1) & 1u))) {
                 if (lane == 0) give_up(0x30045);
                 break;
             }
@@ -305,7 +319,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             const Shape sh = shape_of(b);
             if (sh.n_tiles > 0 && elect_one()) {
                 const int kv_head = b.head0 / (p.a.heads / p.a.kv_heads), end = i + 2 * sh.n_tiles;
-                bool ok = used == 0 || mbar_wait(q_empty, (uint32_t)(used - 1) & 1u);
+                bool ok = used == 0 || wait(q_empty, (uint32_t)(used - 1) & 1u);
                 const bool q_asked = ok;
                 if (ok) {
                     mbar_expect_tx(q_full, 2 * PK_Q_BYTES);
@@ -316,7 +330,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 int n = i;
                 for (int j = 0; ok && n < end; ++n) {
                     const int s = n % PK_STAGES, v = (n - i) & 1;
-                    if (n >= PK_STAGES) ok = mbar_wait(empty + 8 * s, (uint32_t)(n / PK_STAGES - 1) & 1u);
+                    if (n >= PK_STAGES) ok = wait(empty + 8 * s, (uint32_t)(n / PK_STAGES - 1) & 1u);
                     if (*s_dead != 0) ok = false;
                     if (!ok) break;
                     mbar_expect_tx(full + 8 * s, PK_KV_BYTES);
@@ -338,8 +352,8 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         }
         // drain: the last release arrivals land before the CTA may leave
         if (*s_dead == 0 && used > 0) {
-            bool ok = mbar_wait(q_empty, (uint32_t)(used - 1) & 1u);
-            for (int m = max(i - PK_STAGES, 0); m < i && ok; ++m) ok = mbar_wait(empty + 8 * (m % PK_STAGES), (uint32_t)(m / PK_STAGES) & 1u);
+            bool ok = wait(q_empty, (uint32_t)(used - 1) & 1u);
+            for (int m = max(i - PK_STAGES, 0); m < i && ok; ++m) ok = wait(empty + 8 * (m % PK_STAGES), (uint32_t)(m / PK_STAGES) & 1u);
             if (!ok && lane == 0) give_up(0x30046);
         }
         if (lane == 0 && atomicAdd(p.done, 1) == (int)gridDim.x - 1) {   // all CTAs have taken their last ticket
@@ -375,7 +389,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             bool ok = true;
             int i = 0, used = 0, n_a = 0, n_b = 0, n_v = 0;   // tiles of the ring, blocks with keys, halves of P, cleaned tiles so far
             for (int k = 0;; ++k) {
-                if (!mbar_wait(place_full + 8 * (k & 1), (uint32_t)(k >> 1) & 1u)) {
+                if (!wait(place_full + 8 * (k & 1), (uint32_t)(k >> 1) & 1u)) {
                     ok = false;
                     break;
                 }
@@ -384,9 +398,9 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 if (b.block < 0) break;
                 const Shape sh = shape_of(b);
                 if (sh.n_tiles == 0 || !ok) continue;
-                const auto tile_wait = [&](int at) { return mbar_wait(full + 8 * (at % PK_STAGES), (uint32_t)(at / PK_STAGES) & 1u); };
+                const auto tile_wait = [&](int at) { return wait(full + 8 * (at % PK_STAGES), (uint32_t)(at / PK_STAGES) & 1u); };
                 const auto keys_of = [&](int j) { return (uint32_t)(j == sh.n_tiles - 1 && sh.short_last ? PK_KEYS / 2 : PK_KEYS); };
-                ok = *s_dead == 0 && mbar_wait(q_full, (uint32_t)used & 1u) && tile_wait(i);
+                ok = *s_dead == 0 && wait(q_full, (uint32_t)used & 1u) && tile_wait(i);
                 if (ok)
                     for (int t = 0; t < 2; ++t) scores(t, i, keys_of(0), sh.n_tiles == 1);
                 for (int j = 0; j < sh.n_tiles && ok; ++j) {
@@ -394,16 +408,16 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                     ok = *s_dead == 0 && tile_wait(i + 2 * j + 1);
                     if (ok && clean) mbar_arrive(v_last);
                     for (int t = 0; t < 2 && ok; ++t) {
-                        if (j == 0 && used > 0) ok = mbar_wait(o_empty + 8 * t, (uint32_t)(used - 1) & 1u);   // the block before has left
+                        if (j == 0 && used > 0) ok = wait(o_empty + 8 * t, (uint32_t)(used - 1) & 1u);   // the block before has left
                         if (ok && both) {
-                            ok = mbar_wait(p_full + 16 * t + 8, (uint32_t)n_b & 1u);
-                            if (ok && clean && t == 0) ok = mbar_wait(v_clean, (uint32_t)n_v & 1u);
+                            ok = wait(p_full + 16 * t + 8, (uint32_t)n_b & 1u);
+                            if (ok && clean && t == 0) ok = wait(v_clean, (uint32_t)n_v & 1u);
                             if (!ok) break;
                             tc_fence_after();
                             products(t, i + 2 * j + 1, 1, j == 0);
                         }
-                        if (ok) ok = mbar_wait(p_full + 16 * t, (uint32_t)n_a & 1u);
-                        if (ok && clean && t == 0 && !both) ok = mbar_wait(v_clean, (uint32_t)n_v & 1u);
+                        if (ok) ok = wait(p_full + 16 * t, (uint32_t)n_a & 1u);
+                        if (ok && clean && t == 0 && !both) ok = wait(v_clean, (uint32_t)n_v & 1u);
                         if (!ok) break;
                         tc_fence_after();
                         products(t, i + 2 * j + 1, 0, j == 0 && !both);
@@ -434,7 +448,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     } else if (warp == 2) {
         int i = 0, n_v = 0;
         for (int k = 0;; ++k) {
-            if (!__all_sync(0xffffffffu, mbar_wait(place_full + 8 * (k & 1), (uint32_t)(k >> 1) & 1u))) {
+            if (!__all_sync(0xffffffffu, wait(place_full + 8 * (k & 1), (uint32_t)(k >> 1) & 1u))) {
                 if (lane == 0) give_up(0x30044);
                 break;
             }
@@ -445,7 +459,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             const Shape sh = shape_of(b);
             i += 2 * sh.n_tiles;
             if (!sh.ragged || *s_dead != 0) continue;
-            const bool ok = __all_sync(0xffffffffu, mbar_wait(v_last, (uint32_t)n_v & 1u));   // the issuer has seen the tile land
+            const bool ok = __all_sync(0xffffffffu, wait(v_last, (uint32_t)n_v & 1u));   // the issuer has seen the tile land
             ++n_v;
             if (ok) {
                 uint8_t* const tile = kv_s + (i - 1) % PK_STAGES * PK_KV_BYTES;
@@ -471,7 +485,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         bool ok = true;
         int used = 0, n_a = 0;   // blocks with keys, key tiles so far
         for (int k = 0;; ++k) {
-            if (!__all_sync(0xffffffffu, mbar_wait(place_full + 8 * (k & 1), (uint32_t)(k >> 1) & 1u))) {
+            if (!__all_sync(0xffffffffu, wait(place_full + 8 * (k & 1), (uint32_t)(k >> 1) & 1u))) {
                 if (lane == 0) give_up(0x30043);
                 break;
             }
@@ -535,7 +549,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
                 const bool both = j < sh.n_tiles - 1 || !sh.short_last;
                 const int k0 = j * PK_KEYS;
                 // the scores, and with them the products of the tile before, which were issued earlier
-                ok = __all_sync(0xffffffffu, *s_dead == 0 && mbar_wait(s_full + 8 * t, (uint32_t)(n_a + j) & 1u));
+                ok = __all_sync(0xffffffffu, *s_dead == 0 && wait(s_full + 8 * t, (uint32_t)(n_a + j) & 1u));
                 if (!ok) break;
                 tc_fence_after();
                 load(0, k0);
@@ -574,7 +588,7 @@ attn_packed_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             }
             n_a += sh.n_tiles;
             if (sh.n_tiles > 0) {
-                ok = __all_sync(0xffffffffu, ok && mbar_wait(o_full + 8 * t, (uint32_t)used & 1u));
+                ok = __all_sync(0xffffffffu, ok && wait(o_full + 8 * t, (uint32_t)used & 1u));
                 ++used;
                 if (!ok && lane == 0) give_up(0x30043);
             }
@@ -640,6 +654,7 @@ static int packed_launch(const Qw3AttnPackedArgs& a, const Workspace* ws, bool p
     const int group = a.heads / a.kv_heads;
     p.pack = group & -group;
     if (p.pack > 16) p.pack = 16;
+    p.limit = (1ll << 31) + PK_REDO_TICKS * a.k_rows;
     p.ticket = ws->counters;
     p.done = ws->counters + 1;
     p.err = ws->err;

@@ -100,3 +100,27 @@ def test_sums_that_pass_fp32_are_done_again(ops, cuda):
     got = ops.attn_packed(q, k, v, _cu([n], cuda), _cu([n], cuda), ws)
     ws.check()
     _check_rows(got, q, k, v, 0, torch.arange(n, device=cuda))
+
+
+def test_rows_done_again_for_seconds_are_waited_for(ops, cuda):
+    """NaN in the last key of a sequence of 600000: its rows before are done again, 32 a warp, which takes longer than a wait for one tile may, while
+    the CTA has the next block already.  Nothing gives up, and that block is whole."""
+    n, long, rows, many = 25600, 600000, 200, 96
+    g = torch.Generator(device=cuda).manual_seed(4)
+    total = many * n + long
+    q = torch.zeros(many * n + rows, 1, 128, device=cuda, dtype=torch.bfloat16)
+    k = torch.zeros(total, 1, 128, device=cuda, dtype=torch.bfloat16)
+    v = torch.randn(total, 1, 128, device=cuda, generator=g).bfloat16() + 0.5
+    v[-1, 0, 3] = float("nan")
+    ws = ops.Workspace()
+    got = ops.attn_packed(q, k, v, _cu([n] * many + [rows], cuda), _cu([n] * many + [long], cuda), ws)
+    ws.check()
+    bad = got.isnan().nonzero().tolist()
+    assert bad == [[many * n + rows - 1, 0, 3]]
+    # scores are 0: every row is the mean of the V rows that it sees
+    for a, c, nq, nk in [(b * n, b * n, n, n) for b in (0, 20, many - 1)] + [(many * n, many * n, rows, long)]:
+        vv = v[c:c + nk, 0].double().nan_to_num(0.0)
+        count = torch.arange(1, nk + 1, device=cuda, dtype=torch.float64)[:, None]
+        want, size = (torch.cumsum(x, 0).div_(count)[nk - nq:] for x in (vv, vv.abs()))
+        err = (got[a:a + nq, 0].double() - want).abs()
+        assert ((err <= HALF[torch.bfloat16] * (want.abs() + 2 * size) + 2.0 ** -19 * size) | got[a:a + nq, 0].isnan()).all()
