@@ -9,7 +9,8 @@ namespace qw3 {
 
 // ---- block tables and slots ------------------------------------------------------------------------------------------------------
 // One cluster.  Every CTA sums the lengths of all requests for itself (two prefix sums, of new tokens and of new pages, kept in shared
-// memory), the cluster meets once, so that outputs may be the inputs' own buffers, and then its threads fill the lists: a thread takes
+// memory) and checks its share of the pages that will get tokens, the cluster meets, so that outputs may be the inputs' own buffers and a call that
+// cannot be served changes nothing, and then its threads fill the lists: a thread takes
 // four tokens in a row and finds their request by bisection.  Bound by latency, two dependent rounds of global loads: 10.3 us
 // for 7 requests, 14.4 for 250 with 34 K new tokens (launch included, caches cold).
 constexpr int PS_THREADS = 512;
@@ -19,15 +20,25 @@ constexpr int PS_MAX_REQ = 16384;
 __global__ void __launch_bounds__(PS_THREADS) page_slots_kernel(const Qw3PageArgs p, int* err) {
     extern __shared__ int ps_smem[];
     __shared__ long long warp_sum[2][PS_THREADS / 32];
+    __shared__ int ps_bad;
     const int n = p.n_req, P = p.page_size;
     int* const cu = ps_smem;            // [n + 1] tokens before a request
     int* const off = cu + n + 1;        // [n + 1] pages before a request
     int* const ctx = off + n + 1;       // [n]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int first = blockIdx.x * PS_THREADS + tid, step = gridDim.x * PS_THREADS;
+    const auto cluster = cooperative_groups::this_cluster();
+    if (tid == 0) ps_bad = 0;
     pdl_launch_dependents();
+    cluster.barrier_arrive();
     pdl_wait();
 
     const int n_free = *p.d_n_free;
+    // the pages that will get tokens are looked at in shares of the CTAs: those to be taken, the first of a thread while the lengths come, and the last
+    // ones of requests that go on in them
+    const int most_pages = 0x7fffffff / P;
+    const int ahead = n_free <= p.free_capacity && first < n_free ? p.d_free[n_free - 1 - first] : 0;
+    bool bad_page = false;
     const int each = (n + PS_THREADS - 1) / PS_THREADS, b0 = min(tid * each, n), b1 = min(b0 + each, n);
     long long tokens = 0, pages = 0;
     int bad = 0;
@@ -41,6 +52,10 @@ __global__ void __launch_bounds__(PS_THREADS) page_slots_kernel(const Qw3PageArg
             if (need > p.max_blocks) bad = max(bad, 2);
             pages += need - ((long long)c + P - 1) / P;
             tokens += x;
+            if (b % PS_CLUSTER == (int)blockIdx.x && x > 0 && c % P != 0 && need <= p.max_blocks) {
+                const int page = p.d_block_table[b * p.table_stride + c / P];
+                bad_page |= page < 0 || page >= most_pages;
+            }
         }
     }
     long long t = tokens, g = pages;
@@ -75,10 +90,19 @@ __global__ void __launch_bounds__(PS_THREADS) page_slots_kernel(const Qw3PageArg
         }
     }
     if (tid == 0) { cu[n] = (int)total; off[n] = (int)total_pages; }
-    // all CTAs have read the lengths and the number of free pages
-    cooperative_groups::this_cluster().sync();
+    cluster.barrier_wait();   // the others' words are set up
+    if (code == 0) {
+        for (int i = first; i < (int)total_pages; i += step) {
+            const int page = i == first ? ahead : p.d_free[n_free - 1 - i];
+            bad_page |= page < 0 || page >= most_pages;
+        }
+        if (bad_page)
+            for (int r = 0; r < PS_CLUSTER; ++r) *cluster.map_shared_rank(&ps_bad, r) = 1;
+    }
+    // all CTAs have read the lengths, the number of free pages and their share of the pages
+    cluster.sync();
+    if (code == 0 && *static_cast<volatile int*>(&ps_bad) != 0) code = KV4_ERR_FREE_ID;
 
-    const int first = blockIdx.x * PS_THREADS + tid, step = gridDim.x * PS_THREADS;
     const auto find = [n](const int* starts, int i) {   // the last request that starts at or before i
         int lo = 0, hi = n;
         while (hi - lo > 1) {
@@ -119,8 +143,7 @@ __global__ void __launch_bounds__(PS_THREADS) page_slots_kernel(const Qw3PageArg
                 pos = c + i - cu[b];
                 const int block = pos / P, fresh = block - (c + P - 1) / P;
                 const int page = fresh >= 0 ? p.d_free[n_free - 1 - (off[b] + fresh)] : p.d_block_table[b * p.table_stride + block];
-                if (page < 0 || page >= 0x7fffffff / P) kv4_error(err, KV4_ERR_FREE_ID);
-                else slot = page * P + pos % P;
+                slot = page * P + pos % P;
             }
             p.d_pos[i] = pos;
             p.d_slot[i] = slot;

@@ -226,8 +226,10 @@ typedef struct Qw3PageArgs {
 } Qw3PageArgs;
 
 /* Pages for the requests' new tokens, from the top of the stack in the order of requests and blocks, and the position and slot of every new
- * token.  A call that cannot be served (a negative length, a table too narrow, too few pages, more than max_tokens tokens) changes neither
- * table nor stack, returns no slots (all -1, cu 0, kv_len = ctx) and is reported by qw3_ws_check. */
+ * token.  A call that cannot be served (a negative length, a table too narrow, too few pages, more than max_tokens tokens, a page for a new token,
+ * from the stack or in the table, that is below 0 or whose slots would pass 31 bits) changes neither table nor stack, returns no
+ * slots (all -1, cu 0, kv_len = ctx) and is reported by qw3_ws_check.  The size of the pool is not known here: a page behind its end is
+ * handed out, and left out and reported by the operators that are given the pool. */
 int qw3_page_slots(const Qw3PageArgs* args, qw3_ws_t ws, void* stream);
 
 typedef struct Qw3Kv4AppendArgs {
