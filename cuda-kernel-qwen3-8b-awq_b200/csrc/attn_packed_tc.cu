@@ -684,6 +684,13 @@ static int packed_launch(const Qw3AttnPackedArgs& a, const Workspace* ws, bool p
     return QW3_OK;
 }
 
+// Whether `out` shares bytes with one of `rows` rows of `width` bytes, `stride` bytes apart.
+static bool rows_overlap(const void* out, int64_t out_bytes, const void* base, int64_t rows, int64_t width, int64_t stride) {
+    const int64_t lo = reinterpret_cast<intptr_t>(out) - reinterpret_cast<intptr_t>(base), hi = lo + out_bytes;   // beside the first row
+    const int64_t row = lo < width ? 0 : (lo - width) / stride + 1;   // the first that ends behind lo
+    return row < rows && row * stride < hi;
+}
+
 }  // namespace qw3
 
 using namespace qw3;
@@ -704,6 +711,12 @@ extern "C" int qw3_attn_packed(const Qw3AttnPackedArgs* a, qw3_ws_t ws, void* st
     QW3_REQUIRE(((reinterpret_cast<uintptr_t>(a->d_q) | reinterpret_cast<uintptr_t>(a->d_out) | reinterpret_cast<uintptr_t>(a->d_k) | reinterpret_cast<uintptr_t>(a->d_v)) & 15) == 0,
                 "%s: rows must be 16-byte aligned", who);
     QW3_REQUIRE((reinterpret_cast<uintptr_t>(a->d_out) & 31) == 0, "%s: out must be 32-byte aligned", who);
+    // blocks run in any order, and rows that are done again read q, k and v after rows have been stored
+    const int64_t out_bytes = a->q_rows * a->heads * 256;
+    QW3_REQUIRE(!rows_overlap(a->d_out, out_bytes, a->d_q, a->q_rows, a->heads * 256ll, a->q_stride * 2) &&
+                    !rows_overlap(a->d_out, out_bytes, a->d_k, a->k_rows, a->kv_heads * 256ll, a->k_stride * 2) &&
+                    !rows_overlap(a->d_out, out_bytes, a->d_v, a->k_rows, a->kv_heads * 256ll, a->v_stride * 2),
+                "%s: out must not overlap q, k or v", who);
     const int rc = ws_on_device(who, ws);
     if (rc != QW3_OK) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -288,7 +288,8 @@ def attn_kv4_decode(q, cache, block_table, kv_len, ws, scale=None):
 def attn_packed(q, k, v, cu_q, cu_k, ws, scale=None, out=None):
     """Causal attention of packed sequences: q [q_rows][heads][128], k and v [k_rows][kv_heads][128] (rows may be further apart), sequence b in
     rows cu_q[b] .. cu_q[b + 1] of q and cu_k[b] .. cu_k[b + 1] of k and v.  Its queries are its last rows: row i of nq sees keys
-    0 .. nk - nq + i, a row that sees none is zeros.  Rows behind the last sequence are left as they were (undefined in a new `out`)."""
+    0 .. nk - nq + i, a row that sees none is zeros.  Rows behind the last sequence are left as they were (undefined in a new `out`).
+    `out` must not share memory with q, k or v."""
     dev, dtype = q.device, q.dtype
     _want(dtype in _DTYPES, "q: torch.float16 or torch.bfloat16 expected")
     _want(scale is None or scale > 0, "scale: above 0 expected")

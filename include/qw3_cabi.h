@@ -188,7 +188,8 @@ int qw3_attn_prefill_poll_once(const void* d_qkv, const void* d_k_cache, const v
  * A row of zero bytes, which was never stored, stands for zeros; qw3_attn_kv4_decode takes a V scale below the floor for the floor.
  *
  * A slot is page * page_size + offset.  What the device finds out of range (slots, pages, positions, lengths) is left out, never read
- * or written, and recorded: qw3_ws_check returns QW3_ERR_RANGE.  The workspace must belong to the current device. */
+ * or written, and recorded: qw3_ws_check returns QW3_ERR_RANGE.  The workspace must belong to the current device.  An output overlaps no input but where it
+ * is said. */
 enum Qw3Dtype { QW3_F16 = 0, QW3_BF16 = 1 };
 enum Qw3RopeLayout {
     QW3_ROPE_HALVES = 0,  /* dim i turns with dim i + rot_dim / 2 */
@@ -291,7 +292,7 @@ typedef struct Qw3AttnPackedArgs {
     int32_t  head_dim;        /* 128 */
     int32_t  dtype;           /* enum Qw3Dtype */
     float    scale;           /* of the scores, above 0; 0: 1 / sqrt(128) */
-    void*    d_out;           /* [q_rows][heads][128], 32-byte aligned */
+    void*    d_out;           /* [q_rows][heads][128], 32-byte aligned; not q, k or v, nor parts of them */
 } Qw3AttnPackedArgs;
 
 /* Causal attention of packed sequences (attentionKernel, Inference.cu:182-266, intended math; the reference has one sequence and as

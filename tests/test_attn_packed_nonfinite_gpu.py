@@ -124,3 +124,16 @@ def test_rows_done_again_for_seconds_are_waited_for(ops, cuda):
         want, size = (torch.cumsum(x, 0).div_(count)[nk - nq:] for x in (vv, vv.abs()))
         err = (got[a:a + nq, 0].double() - want).abs()
         assert ((err <= HALF[torch.bfloat16] * (want.abs() + 2 * size) + 2.0 ** -19 * size) | got[a:a + nq, 0].isnan()).all()
+
+
+def test_out_in_the_place_of_an_input_is_refused(ops, cuda):
+    """Rows that are done again read q after their result is stored, so it cannot go there."""
+    g = torch.Generator(device=cuda).manual_seed(6)
+    q, k, v = (torch.randn(40, x, 128, device=cuda, generator=g).half() for x in (4, 4, 4))
+    ws, cu = ops.Workspace(), _cu([40], cuda)
+    for out in (q, k, v, q.view(-1, 512)):
+        with pytest.raises(ops.cabi.Qw3Error) as e:
+            ops.attn_packed(q, k, v, cu, cu, ws, out=out)
+        assert e.value.status == ops.cabi.QW3_ERR_ARG
+    ops.attn_packed(q, k, v, cu, cu, ws, out=torch.empty_like(q))
+    ws.check()

@@ -1,0 +1,36 @@
+"""Refusals of the batch server's operators that need no GPU, beside those of test_kv4_cpu.py."""
+import ctypes as C
+
+import pytest
+import torch
+
+PTR = 1 << 20   # an address that is never read: every call below is refused before
+
+
+def _packed(cabi, **kw):
+    a = cabi.AttnPackedArgs(PTR, 512, 2 * PTR, 256, 3 * PTR, 256, 10, 12, PTR, PTR, 1, 4, 2, 128, 0, 0.0, 4 * PTR)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+# q: 10 rows of 1024 bytes; k, v: 12 rows of 512 bytes; out: 10240 bytes
+@pytest.mark.parametrize("kw", [dict(d_out=PTR), dict(d_out=PTR + 10 * 1024 - 32), dict(d_out=PTR - 10240 + 32), dict(d_out=2 * PTR), dict(d_out=2 * PTR + 12 * 512 - 32),
+                                dict(d_out=3 * PTR - 10240 + 32), dict(d_out=3 * PTR + 32),
+                                dict(d_out=PTR + 1024, q_stride=768), dict(d_out=PTR + 9 * 16384 + 992, q_stride=8192), dict(d_out=PTR + 16384 - 10240 + 32, q_stride=8192),
+                                dict(d_out=2 * PTR + 8192 + 480, k_stride=4096, k_rows=2), dict(d_k=4 * PTR, d_v=4 * PTR + 512, k_stride=512, v_stride=512)])
+def test_out_that_overlaps_an_input_is_refused(pkg, kw):
+    cabi = pkg.cabi
+    assert cabi.lib().qw3_attn_packed(C.byref(_packed(cabi, **kw)), PTR, None) == cabi.QW3_ERR_ARG
+    assert b"overlap" in cabi.lib().qw3_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(d_out=PTR + 10 * 1024), dict(d_out=PTR - 10240), dict(d_out=2 * PTR + 12 * 512), dict(d_out=3 * PTR - 10240),
+                                dict(d_out=PTR + 1024, q_stride=8192), dict(d_out=PTR + 16384 - 10240, q_stride=8192), dict(d_out=PTR + 8192 * 20, q_stride=8192),
+                                dict(d_out=2 * PTR + 512, k_stride=8192)])
+def test_out_beside_and_between_the_rows_is_not(pkg, kw):
+    """These pass the checks of arguments; without a GPU the call ends there."""
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are none")
+    cabi = pkg.cabi
+    assert cabi.lib().qw3_attn_packed(C.byref(_packed(cabi, **kw)), PTR, None) == cabi.QW3_ERR_CUDA
