@@ -173,7 +173,9 @@ def _table(t, rows, device):
     return t.stride(0) if rows > 1 else shape[1]
 
 
-_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# The private functions take less of a call's time than the public ones; a build of torch without CUDA has none of them.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _on(device, name, *args):

@@ -34,3 +34,23 @@ def test_out_beside_and_between_the_rows_is_not(pkg, kw):
         pytest.skip("the addresses are none")
     cabi = pkg.cabi
     assert cabi.lib().qw3_attn_packed(C.byref(_packed(cabi, **kw)), PTR, None) == cabi.QW3_ERR_CUDA
+
+
+def test_the_operators_import_without_torchs_private_functions(pkg, monkeypatch):
+    """As in a build of torch without CUDA: the module loads, and its calls refuse tensors of the CPU."""
+    import importlib.util
+    import sys
+
+    cabi = pkg.cabi
+    for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+        if hasattr(torch._C, name):
+            monkeypatch.delattr(torch._C, name)
+    path = importlib.util.find_spec("qw3awq_b200.ops").origin
+    spec = importlib.util.spec_from_file_location("qw3awq_b200._ops_again", path)
+    ops = importlib.util.module_from_spec(spec)
+    monkeypatch.setitem(sys.modules, spec.name, ops)
+    spec.loader.exec_module(ops)
+    cache = ops.Kv4Cache(torch.zeros(2, 2 * 16 * 136, dtype=torch.uint8), 16, 2, torch.float16)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.kv4_read(cache, torch.zeros(3, dtype=torch.int32), type("Ws", (), {"h": C.c_void_p(PTR)}))
+    assert ops.cabi is cabi
