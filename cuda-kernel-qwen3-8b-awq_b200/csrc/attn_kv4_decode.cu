@@ -693,7 +693,7 @@ extern "C" int qw3_attn_kv4_decode(const Qw3Kv4Pool* pool, const Qw3AttnKv4Args*
     QW3_REQUIRE(a->q_stride >= (int64_t)a->heads * 128 && a->q_stride % 8 == 0 && a->q_stride < ((int64_t)1 << 31), "%s: q_stride must be a multiple of 8 and hold the heads", who);
     QW3_REQUIRE(a->max_blocks > 0 && a->table_stride >= a->max_blocks, "%s: block table out of range", who);
     QW3_REQUIRE(((reinterpret_cast<uintptr_t>(a->d_q) | reinterpret_cast<uintptr_t>(a->d_out)) & 15) == 0, "%s: q and out must be 16-byte aligned", who);
-    QW3_REQUIRE(a->scale == a->scale && a->scale - a->scale == 0.0f, "%s: scale must be finite", who);
+    QW3_REQUIRE(fabsf(a->scale) <= KV4_MAX_SCALE, "%s: scale must be finite, 2e38 at most", who);
     const Workspace* w = ws_struct(ws);
     KdParams p;
     p.pool = *pool;

@@ -702,7 +702,7 @@ extern "C" int qw3_attn_packed(const Qw3AttnPackedArgs* a, qw3_ws_t ws, void* st
     QW3_REQUIRE(a->dtype == QW3_F16 || a->dtype == QW3_BF16, "%s: dtype must be QW3_F16 or QW3_BF16", who);
     QW3_REQUIRE(a->kv_heads > 0 && a->heads > 0 && a->heads <= 4096 && a->heads % a->kv_heads == 0, "%s: heads must be a multiple of kv_heads", who);
     QW3_REQUIRE(a->q_rows >= 0 && a->q_rows <= 0x7fffffff - 1024 && a->k_rows >= 0 && a->k_rows <= 0x7fffffff - 1024 && a->n_seq >= 0, "%s: rows or n_seq out of range", who);
-    QW3_REQUIRE(a->scale >= 0.0f && a->scale - a->scale == 0.0f, "%s: scale must be finite and not below 0", who);
+    QW3_REQUIRE(a->scale >= 0.0f && a->scale <= KV4_MAX_SCALE, "%s: scale must be finite, 2e38 at most, and not below 0", who);
     if (a->q_rows == 0 || a->n_seq == 0) return QW3_OK;
     QW3_REQUIRE(a->d_q && a->d_out && a->d_cu_q && a->d_cu_k && (a->k_rows == 0 || (a->d_k && a->d_v)), "%s: null pointer", who);
     const auto stride_ok = [](int64_t s, int heads) { return s >= (int64_t)heads * 128 && s % 8 == 0 && s < ((int64_t)1 << 31); };

@@ -16,6 +16,8 @@ constexpr int KV4_TILE_TOKENS = 16;
 constexpr int KV4_TILE_BYTES = 2176;
 constexpr int KV4_V = 1024, KV4_KP = 2048, KV4_VP = 2112;   // offsets of the V codes and of the pairs of K and V in a tile
 
+constexpr float KV4_MAX_SCALE = 2e38f;   // of scores: times log2(e) it stays in fp32
+
 // Codes of the workspace's error word: an index or a length outside the buffers of the call (QW3_ERR_RANGE).
 enum { KV4_ERR_LENGTH = 0xE0001, KV4_ERR_TABLE = 0xE0002, KV4_ERR_PAGES = 0xE0003, KV4_ERR_TOKENS = 0xE0004, KV4_ERR_FREE_ID = 0xE0005,
        KV4_ERR_APPEND_SLOT = 0xE0011, KV4_ERR_APPEND_POS = 0xE0012, KV4_ERR_READ_SLOT = 0xE0021, KV4_ERR_DECODE_PAGE = 0xE0031,

@@ -192,6 +192,14 @@ def _on(device, name, *args):
         cabi.check(status, name)
 
 
+def _scale(scale):
+    """As the C ABI takes it: fp32, 0 for 1 / sqrt(128).  A number that fp32 rounds to 0 must not become that."""
+    if scale is None:
+        return 0.0
+    _want(C.c_float(scale).value != 0, "scale: 0 in fp32 is not a scale")
+    return scale
+
+
 class Kv4Cache:
     """A pool of pages of 4-bit K and V rows of one layer.  pages: uint8 [n_pages][page_bytes] (rows may be further apart, as where the
     pages of several layers are interleaved), page_bytes = kv_heads * page_size * 136."""
@@ -276,13 +284,13 @@ def attn_kv4_decode(q, cache, block_table, kv_len, ws, scale=None):
     zeros where there are none.  scale: of the scores, 1 / sqrt(128) by default."""
     dev, dtype = q.device, cache.dtype
     _want(cache.device == dev, "q and the cache's pages: one device expected")
-    _want(scale is None or scale != 0, "scale: 0 is not a scale")
+    scale = _scale(scale)
     heads, stride = _rows128(q, None, "q", dev, dtype)
     n = q.shape[0]
     d_len = _ints(kv_len, n, "kv_len", dev)
     table_stride = _table(block_table, n, dev)
     out = torch.empty_like(q) if q.dim() == 3 and q.is_contiguous() else q.new_empty((n, heads, 128))
-    a = cabi.AttnKv4Args(q.data_ptr(), stride, n, heads, block_table.data_ptr(), table_stride, block_table.shape[1], scale or 0.0, d_len, out.data_ptr())
+    a = cabi.AttnKv4Args(q.data_ptr(), stride, n, heads, block_table.data_ptr(), table_stride, block_table.shape[1], scale, d_len, out.data_ptr())
     _on(dev, "qw3_attn_kv4_decode", cache.ref, C.byref(a), ws.h)
     return out
 
@@ -295,6 +303,7 @@ def attn_packed(q, k, v, cu_q, cu_k, ws, scale=None, out=None):
     dev, dtype = q.device, q.dtype
     _want(dtype in _DTYPES, "q: torch.float16 or torch.bfloat16 expected")
     _want(scale is None or scale > 0, "scale: above 0 expected")
+    scale = _scale(scale)
     heads, q_stride = _rows128(q, None, "q", dev, dtype)
     kv, k_stride = _rows128(k, None, "k", dev, dtype)
     _, v_stride = _rows128(v, kv, "v", dev, dtype)
@@ -308,6 +317,6 @@ def attn_packed(q, k, v, cu_q, cu_k, ws, scale=None, out=None):
         _want(out.device == dev and out.dtype == dtype and out.is_contiguous() and out.numel() == q.shape[0] * heads * 128,
               "out: contiguous [q_rows][heads][128] expected")
     a = cabi.AttnPackedArgs(q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, q.shape[0], k.shape[0], d_cu_q, d_cu_k, n,
-                            heads, kv, 128, _DTYPES[dtype], scale or 0.0, out.data_ptr())
+                            heads, kv, 128, _DTYPES[dtype], scale, out.data_ptr())
     _on(dev, "qw3_attn_packed", C.byref(a), ws.h)
     return out

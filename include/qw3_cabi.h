@@ -265,7 +265,7 @@ typedef struct Qw3AttnKv4Args {
     const int32_t* d_block_table;  /* [n_req][table_stride] */
     int64_t  table_stride;
     int32_t  max_blocks;           /* entries of a row that may be read */
-    float    scale;                /* of the scores; 0: 1 / sqrt(128) */
+    float    scale;                /* of the scores, 2e38 in size at most; 0: 1 / sqrt(128) */
     const int32_t* d_kv_len;       /* [n_req] tokens to attend to; 0 gives a row of zeros */
     void*    d_out;                /* [n_req][heads][128] */
 } Qw3AttnKv4Args;
@@ -291,7 +291,7 @@ typedef struct Qw3AttnPackedArgs {
     int32_t  kv_heads;
     int32_t  head_dim;        /* 128 */
     int32_t  dtype;           /* enum Qw3Dtype */
-    float    scale;           /* of the scores, above 0; 0: 1 / sqrt(128) */
+    float    scale;           /* of the scores, above 0, 2e38 at most; 0: 1 / sqrt(128) */
     void*    d_out;           /* [q_rows][heads][128], 32-byte aligned; not q, k or v, nor parts of them */
 } Qw3AttnPackedArgs;
 

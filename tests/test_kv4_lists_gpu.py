@@ -70,3 +70,11 @@ def test_a_scale_of_zero_leaves_the_minimum(ops, cuda, dtype):
         tiles[0][2112 + 4 * 5:2112 + 4 * 6] = torch.tensor(pair, dtype=dtype, device=cuda).view(torch.uint8)
         assert ops.attn_kv4_decode(q, cache, table, _i32([64], cuda), ws).isnan().all()
     ws.check()
+
+
+@pytest.mark.parametrize("scale", [3e38, -3e38, float("inf"), float("nan")])
+def test_a_scale_that_passes_fp32_in_the_kernel_is_refused(ops, cuda, scale):
+    cache, ws = ops.Kv4Cache.alloc(2, 16, 1, torch.float16, cuda), ops.Workspace()
+    with pytest.raises(ops.cabi.Qw3Error) as e:
+        ops.attn_kv4_decode(torch.zeros(1, 2, 128, dtype=torch.float16, device=cuda), cache, _i32([[0]], cuda), _i32([1], cuda), ws, scale=scale)
+    assert e.value.status == ops.cabi.QW3_ERR_ARG

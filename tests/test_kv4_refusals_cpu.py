@@ -54,3 +54,30 @@ def test_the_operators_import_without_torchs_private_functions(pkg, monkeypatch)
     with pytest.raises(ValueError, match="CUDA"):
         ops.kv4_read(cache, torch.zeros(3, dtype=torch.int32), type("Ws", (), {"h": C.c_void_p(PTR)}))
     assert ops.cabi is cabi
+
+
+@pytest.fixture
+def ops(pkg):
+    import importlib
+    return importlib.import_module("qw3awq_b200.ops")
+
+
+@pytest.mark.parametrize("scale", [1e-46, -1e-50, 5e-324, 0.0, -0.0])
+def test_a_scale_that_is_zero_in_fp32_does_not_become_the_usual_one(ops, scale):
+    cache = ops.Kv4Cache(torch.zeros(2, 2 * 16 * 136, dtype=torch.uint8), 16, 2, torch.float16)
+    q, ints = torch.zeros(3, 4, 128, dtype=torch.float16), torch.zeros(3, dtype=torch.int32)
+    ws = type("Ws", (), {"h": C.c_void_p(PTR)})
+    with pytest.raises(ValueError, match="scale"):
+        ops.attn_kv4_decode(q, cache, ints[:, None], ints, ws, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        ops.attn_packed(q, q, q, ints, ints, ws, scale=scale)
+    # the smallest number of fp32 passes, and the next check is that of the device
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.attn_packed(q, q, q, ints, ints, ws, scale=1.4e-45)
+
+
+@pytest.mark.parametrize("scale", [3e38, float("inf"), float("nan")])
+def test_a_scale_that_passes_fp32_in_the_kernel_is_refused(pkg, scale):
+    cabi = pkg.cabi
+    assert cabi.lib().qw3_attn_packed(C.byref(_packed(cabi, scale=scale)), PTR, None) == cabi.QW3_ERR_ARG
+    assert b"scale" in cabi.lib().qw3_last_error()
