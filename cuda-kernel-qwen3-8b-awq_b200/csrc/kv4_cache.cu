@@ -416,6 +416,7 @@ int qw3_rope_kv4_append(const Qw3Kv4Pool* pool, const Qw3Kv4AppendArgs* a, qw3_w
     QW3_REQUIRE(a->heads > 0 && a->heads <= 4096, "%s: heads out of range", who);
     QW3_REQUIRE(a->rot_dim >= 0 && a->rot_dim <= 128 && a->rot_dim % 16 == 0, "%s: rot_dim must be a multiple of 16, 0 to 128", who);
     QW3_REQUIRE(a->layout == QW3_ROPE_HALVES || a->layout == QW3_ROPE_PAIRS, "%s: unknown layout", who);
+    QW3_REQUIRE(a->reserved == 0, "%s: reserved must be 0", who);
     if (a->tokens == 0) return QW3_OK;
     QW3_REQUIRE(a->d_qkv && a->d_q_out && a->d_slot, "%s: null pointer", who);
     QW3_REQUIRE(a->rot_dim == 0 || (a->d_pos && a->d_cos && a->d_sin && a->max_pos > 0), "%s: positions and tables are needed to rotate", who);

@@ -1,4 +1,6 @@
 """Decode attention over the paged 4-bit cache: rows that were never stored, long lists, lists cut between CTAs, the low terms of P."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -78,3 +80,13 @@ def test_a_scale_that_passes_fp32_in_the_kernel_is_refused(ops, cuda, scale):
     with pytest.raises(ops.cabi.Qw3Error) as e:
         ops.attn_kv4_decode(torch.zeros(1, 2, 128, dtype=torch.float16, device=cuda), cache, _i32([[0]], cuda), _i32([1], cuda), ws, scale=scale)
     assert e.value.status == ops.cabi.QW3_ERR_ARG
+
+
+def test_append_refuses_a_reserved_field_that_is_not_zero(ops, cuda):
+    cabi = ops.cabi
+    cache, ws = ops.Kv4Cache.alloc(2, 16, 2, torch.float16, cuda), ops.Workspace()
+    qkv, slots, q = torch.zeros(1, 8 * 128, dtype=torch.float16, device=cuda), _i32([3], cuda), torch.empty(1, 4, 128, dtype=torch.float16, device=cuda)
+    for reserved, status in ((1, cabi.QW3_ERR_ARG), (-1, cabi.QW3_ERR_ARG), (0, cabi.QW3_OK)):
+        a = cabi.Kv4AppendArgs(qkv.data_ptr(), 8 * 128, 1, 4, cabi.ROPE_HALVES, 0, reserved, slots.data_ptr(), None, None, None, 0, q.data_ptr(), None)
+        assert cabi.lib().qw3_rope_kv4_append(cache.ref, C.byref(a), ws.h, ops._stream()) == status
+    ws.check()
