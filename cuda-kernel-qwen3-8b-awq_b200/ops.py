@@ -19,13 +19,18 @@ def _ptr(t):
 
 
 class Workspace:
+    """Of the device that is current when it is made."""
+
     def __init__(self, pdl=False):
         self.h = C.c_void_p()
+        self.device = torch.cuda.current_device()
         cabi.check(cabi.lib().qw3_ws_create(C.byref(self.h)), "qw3_ws_create")
         cabi.check(cabi.lib().qw3_ws_set_pdl(self.h, int(pdl)), "qw3_ws_set_pdl")
 
     def check(self):
-        cabi.check(cabi.lib().qw3_ws_check(self.h, _stream()), "qw3_ws_check")
+        """Waits for the current stream of the workspace's device, whichever is current, and raises what its operators reported."""
+        with torch.cuda.device(self.device):
+            cabi.check(cabi.lib().qw3_ws_check(self.h, _stream()), "qw3_ws_check")
 
     def close(self):
         if self.h.value:

@@ -81,3 +81,36 @@ def test_a_scale_that_passes_fp32_in_the_kernel_is_refused(pkg, scale):
     cabi = pkg.cabi
     assert cabi.lib().qw3_attn_packed(C.byref(_packed(cabi, scale=scale)), PTR, None) == cabi.QW3_ERR_ARG
     assert b"scale" in cabi.lib().qw3_last_error()
+
+
+def test_a_workspace_is_checked_on_its_own_device(ops, monkeypatch):
+    """The operators go to the device of their tensors; so does the check, from a program whose current device is another one."""
+    import contextlib
+
+    current, calls = [1], []
+
+    @contextlib.contextmanager
+    def device(index):
+        before, current[0] = current[0], index
+        yield
+        current[0] = before
+
+    class Lib:
+        def qw3_ws_create(self, h):
+            return 0
+
+        def qw3_ws_set_pdl(self, h, pdl):
+            return 0
+
+        def qw3_ws_check(self, h, stream):
+            calls.append((current[0], stream.value))
+            return 0
+
+    monkeypatch.setattr(ops.cabi, "lib", Lib)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: type("Stream", (), {"cuda_stream": 100 + current[0]}))
+    ws = ops.Workspace()
+    current[0] = 0
+    ws.check()
+    assert calls == [(1, 101)] and current == [0]
