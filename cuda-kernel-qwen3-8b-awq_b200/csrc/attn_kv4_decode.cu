@@ -301,21 +301,19 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
         uint32_t qf[4][4];   // word j of a row: low nibbles k 0..7, 8..15, high nibbles the same
         float f0, f1, qs0, qs1;
         {
-            float sum = 0.0f, big = 0.0f;
+            constexpr bool HALF = R::FLOOR > 1e-9f;
+            float sum = 0.0f, big = 0.0f, f = p.c;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float2 f = R::unpack(u[e]);
-                    sum += f.x + f.y;
-                    big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    const float2 v = R::unpack(u[e]);
+                    if (HALF) sum += v.x + v.y;
+                    else big = fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y)));
                 }
             }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            float f = p.c;
-            if (sizeof(T) == 2 && R::FLOOR < 1e-9f) {   // bf16: the largest value of the head goes to [2^14, 2^15)
+            if (!HALF) {   // bf16: the largest value of the head goes to [2^14, 2^15); the sum is taken there, before it passes fp32
                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
                 const int ex = (int)(__float_as_uint(big) >> 23);   // biased; 255 for Inf
@@ -323,17 +321,20 @@ __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(Kd
                 shift = min(shift, 100);
                 const float up = __uint_as_float((uint32_t)(127 + shift) << 23);
                 f *= __uint_as_float((uint32_t)(127 - shift) << 23);
-                sum *= up;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     uint32_t* u = &w[j].x;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float2 v = R::unpack(u[e]);
-                        u[e] = RowType<__half>::pack(v.x * up, v.y * up);
+                        const float a = v.x * up, b = v.y * up;
+                        sum += a + b;
+                        u[e] = RowType<__half>::pack(a, b);
                     }
                 }
             }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 qf[j][0] = __byte_perm(w[j].x, w[j].z, 0x5410);

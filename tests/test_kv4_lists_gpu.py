@@ -90,3 +90,20 @@ def test_append_refuses_a_reserved_field_that_is_not_zero(ops, cuda):
         a = cabi.Kv4AppendArgs(qkv.data_ptr(), 8 * 128, 1, 4, cabi.ROPE_HALVES, 0, reserved, slots.data_ptr(), None, None, None, 0, q.data_ptr(), None)
         assert cabi.lib().qw3_rope_kv4_append(cache.ref, C.byref(a), ws.h, ops._stream()) == status
     ws.check()
+
+
+@pytest.mark.parametrize("heads,kv", [(4, 2), (6, 1)])
+def test_bf16_q_whose_sum_passes_fp32(ops, cuda, heads, kv):
+    """128 values of 2^126 and more of one sign: their sum, which the minimum of a K row is multiplied with, is not a number of fp32; the scores are."""
+    dtype, n, page = torch.bfloat16, 90, 16
+    g = torch.Generator(device=cuda).manual_seed(7)
+    cache, ws = ops.Kv4Cache.alloc(6, page, kv, dtype, cuda), ops.Workspace()
+    slots = torch.arange(n, device=cuda).int()
+    ops.rope_kv4_append(torch.randn(n, (heads + 2 * kv) * 128, device=cuda, generator=g).to(dtype), cache, slots, None, None, None, heads, ws)
+    q = ((1 + torch.rand(1, heads, 128, device=cuda, generator=g)) * 2.0 ** 126).to(dtype)
+    q[:, 1] = -q[:, 1]
+    assert q.float().sum(-1).isinf().all()
+    table = torch.arange(6, device=cuda).int()[None]
+    got = ops.attn_kv4_decode(q, cache, table, _i32([n], cuda), ws, scale=2.0 ** -126)
+    ws.check()
+    ref.check_decode(got, q, cache, table, [n], 2.0 ** -126)
