@@ -183,7 +183,7 @@ int qw3_attn_prefill_poll_once(const void* d_qkv, const void* d_k_cache, const v
  * for code * scale + minimum:
  *   minimum = T(min), scale = max(T((max - minimum) / 15), floor), code = clamp(rint((x - minimum) / scale), 0, 15)
  * in fp32, T() rounding to the rows' type; the floor is 2^-24 (fp16) or 2^-60 (bf16).  A row with Inf or NaN (bf16: or with a range
- * of more than 15 * 2^60) reads back as NaN.  16 tokens of a KV head lie together in 2176 bytes: 16 rows of 64 bytes of K codes (byte i:
+ * of more than 15 * 2^60; fp16: or with a minimum that fp16 does not have, as a rotation may give) reads back as NaN.  16 tokens of a KV head lie together in 2176 bytes: 16 rows of 64 bytes of K codes (byte i:
  * dim 2i in the low nibble), the same of V, 16 pairs (scale, minimum) of K, 16 of V; a page is [kv_heads][page_size / 16] of these.
  * A row of zero bytes, which was never stored, stands for zeros; qw3_attn_kv4_decode takes a V scale below the floor for the floor.
  *

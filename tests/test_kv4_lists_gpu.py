@@ -107,3 +107,102 @@ def test_bf16_q_whose_sum_passes_fp32(ops, cuda, heads, kv):
     got = ops.attn_kv4_decode(q, cache, table, _i32([n], cuda), ws, scale=2.0 ** -126)
     ws.check()
     ref.check_decode(got, q, cache, table, [n], 2.0 ** -126)
+
+
+# ---- long lists ------------------------------------------------------------------------------------------------------------------
+
+def _pool(ops, cuda, dtype, kv, page, n_pages, seed):
+    """A pool of stored rows; the V rows of a page share an offset of the page's own, so that no part of a list is like another."""
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    cache, ws = ops.Kv4Cache.alloc(n_pages, page, kv, dtype, cuda), ops.Workspace()
+    n = n_pages * page
+    qkv = torch.randn(n, 1 + 2 * kv, 128, device=cuda, generator=g)
+    qkv[:, 1 + kv:] += torch.randn(n_pages, 1, kv, 128, device=cuda, generator=g).expand(-1, page, -1, -1).reshape(n, kv, 128)
+    order = torch.randperm(n, device=cuda, generator=g)
+    ops.rope_kv4_append(qkv.to(dtype)[order].flatten(1), cache, order.int(), None, None, None, 1, ws)
+    ws.check()
+    return cache, ws, g
+
+
+def _check_and_see_parts(got, q, cache, table, lens, scale=128 ** -0.5):
+    """check_decode, and that it would see a part of 8 chunks missing: without these 256 tokens the 64-bit result itself is outside of the bound."""
+    ref.check_decode(got, q, cache, table, lens, scale)
+    b = max(range(len(lens)), key=lambda i: lens[i])
+    n, dtype = lens[b], cache.dtype
+    slots = ref.slots_of(table[b], n, cache.page_size)
+    want, bound = ref.decode(q[b], *ref.rows(cache, slots), scale, 2.0 ** -11)
+    for at in (0, n // 2 // 32 * 32, n - 256):
+        less, _ = ref.decode(q[b], *ref.rows(cache, torch.cat([slots[:at], slots[at + 256:]])), scale, 2.0 ** -11)
+        seen = ((less - want).abs() > 2 * (ref.HALF[dtype] * want.abs() + bound + 2.0 ** -25)).any(-1)
+        assert seen.all(), (at, seen)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv", [(5, 1), (8, 1), (12, 1), (17, 1), (14, 2), (3, 1)])
+def test_lists_cut_between_ctas(ops, cuda, dtype, heads, kv):
+    """Pairs of more than 32 chunks share CTAs with others and are joined: groups above four heads and above eight (two and three tiles of heads), rows of
+    both types."""
+    page, lens = 64, [5000, 40, 1100, 0, 2000, 33 * 32 + 1, 1]
+    cache, ws, g = _pool(ops, cuda, dtype, kv, page, 61, seed=heads)
+    table = torch.randint(0, 61, (len(lens), 80), device=cuda, generator=g).int()
+    q = torch.randn(len(lens), heads, 128, device=cuda, generator=g).to(dtype)
+    args = (q, cache, table, _i32(lens, cuda), ws)
+    got = ops.attn_kv4_decode(*args)
+    ws.check()
+    _check_and_see_parts(got, q, cache, table, lens)
+    assert torch.equal(ops.attn_kv4_decode(*args), got)
+    ws.check()
+
+
+@pytest.mark.parametrize("heads,kv,dtype", [(16, 4, torch.float16), (16, 4, torch.bfloat16), (32, 4, torch.float16), (48, 4, torch.bfloat16)])
+def test_lists_of_more_chunks_than_a_warp_looks_up_at_once(ops, cuda, heads, kv, dtype):
+    """60000 chunks and more, 135 a CTA and 33 a warp at least: the second look-up, sums that leave the accumulators, most pairs in several CTAs."""
+    page, n_pages, lens = 64, 97, [40000 + 17 * b for b in range(12)]
+    sms = torch.cuda.get_device_properties(cuda).multi_processor_count
+    assert sum(-(-n // 32) for n in lens) * kv > 128 * 3 * sms
+    cache, ws, g = _pool(ops, cuda, dtype, kv, page, n_pages, seed=heads + kv)
+    table = torch.randint(0, n_pages, (len(lens), 40960 // page), device=cuda, generator=g).int()
+    q = torch.randn(len(lens), heads, 128, device=cuda, generator=g).to(dtype)
+    args = (q, cache, table, _i32(lens, cuda), ws)
+    got = ops.attn_kv4_decode(*args)
+    ws.check()
+    _check_and_see_parts(got, q, cache, table, lens)
+    assert torch.equal(ops.attn_kv4_decode(*args), got)
+    ws.check()
+
+
+@pytest.mark.parametrize("heads,kv", [(1, 1), (4, 2), (3, 1), (8, 2)])
+def test_what_the_rounding_of_p_takes_off_is_added(ops, cuda, heads, kv):
+    """fp16 rows, groups of four heads at most: P is two fp16 numbers.  Scores of some thousandths, so that their own errors do not hide it, and results
+    that are small beside the values they come from.  With P as one fp16 number the errors are 4 to 10 times the bound."""
+    dtype, page, lens, scale = torch.float16, 16, [3, 31, 100, 117], 0.002
+    cache, ws, g = _pool(ops, cuda, dtype, kv, page, 40, seed=20 + heads)
+    table = torch.randperm(40, device=cuda, generator=g)[:32].int().view(4, 8)
+    q = torch.randn(4, heads, 128, device=cuda, generator=g).to(dtype)
+    got = ops.attn_kv4_decode(q, cache, table, _i32(lens, cuda), ws, scale=scale)
+    ws.check()
+    ref.check_decode(got, q, cache, table, lens, scale, p_round=2.0 ** -22)
+
+
+# ---- append ----------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("pairs", [False, True])
+def test_a_rotated_minimum_that_passes_fp16_reads_back_as_nan(ops, cuda, pairs):
+    """Finite fp16 rows that a rotation takes below fp16: the stored minimum would be -Inf.  Above, the row's other values are held, and the largest code
+    stands for what fp16 makes of it."""
+    kv, heads, page = 1, 1, 16
+    cache, ws = ops.Kv4Cache.alloc(1, page, kv, torch.float16, cuda), ops.Workspace()
+    angle = torch.full((4, 64), torch.pi / 4, dtype=torch.float64, device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(9)
+    qkv = torch.randn(3, 3 * 128, device=cuda, generator=g).half()
+    i, j = (10, 11) if pairs else (10, 74)
+    for token, sign in ((0, -1), (1, 1)):
+        qkv[token, 128 + i], qkv[token, 128 + j] = sign * 60000.0, sign * 60000.0
+    _, k = ops.rope_kv4_append(qkv, cache, _i32([2, 3, 4], cuda), _i32([0, 1, 2], cuda), angle.cos().float(), angle.sin().float(), heads, ws, pairs=pairs)
+    kr, vr = ops.kv4_read(cache, _i32([2, 3, 4], cuda), ws)
+    ws.check()
+    assert k[0, 0, j] == -float("inf") and k[1, 0, j] == float("inf") and k[2].isfinite().all()
+    assert kr[0].isnan().all() and vr.isfinite().all() and kr[2].isfinite().all()
+    # 84853 / 15: a step of 5660, and the sum of the largest code passes fp16
+    keep = torch.arange(128, device=cuda) != j
+    assert kr[1, 0, j] == float("inf") and ((kr[1, 0, keep].float() - k[1, 0, keep].float()).abs() <= 5660 / 2 + 4).all()
