@@ -686,6 +686,7 @@ static int packed_launch(const Qw3AttnPackedArgs& a, const Workspace* ws, bool p
 
 // Whether `out` shares bytes with one of `rows` rows of `width` bytes, `stride` bytes apart.
 static bool rows_overlap(const void* out, int64_t out_bytes, const void* base, int64_t rows, int64_t width, int64_t stride) {
+    if (rows <= 0) return false;   // nor is there a stride
     const int64_t lo = reinterpret_cast<intptr_t>(out) - reinterpret_cast<intptr_t>(base), hi = lo + out_bytes;   // beside the first row
     const int64_t row = lo < width ? 0 : (lo - width) / stride + 1;   // the first that ends behind lo
     return row < rows && row * stride < hi;

@@ -27,7 +27,7 @@ def test_out_that_overlaps_an_input_is_refused(pkg, kw):
 
 @pytest.mark.parametrize("kw", [dict(), dict(d_out=PTR + 10 * 1024), dict(d_out=PTR - 10240), dict(d_out=2 * PTR + 12 * 512), dict(d_out=3 * PTR - 10240),
                                 dict(d_out=PTR + 1024, q_stride=8192), dict(d_out=PTR + 16384 - 10240, q_stride=8192), dict(d_out=PTR + 8192 * 20, q_stride=8192),
-                                dict(d_out=2 * PTR + 512, k_stride=8192)])
+                                dict(d_out=2 * PTR + 512, k_stride=8192), dict(k_rows=0, d_k=None, d_v=None, k_stride=0, v_stride=0)])
 def test_out_beside_and_between_the_rows_is_not(pkg, kw):
     """These pass the checks of arguments; without a GPU the call ends there."""
     if torch.cuda.is_available():
