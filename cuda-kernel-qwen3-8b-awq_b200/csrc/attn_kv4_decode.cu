@@ -6,15 +6,16 @@
 // further up), so a mask is all the unpacking there is, products are exact, and scales are applied to fp32 sums.  V's scale is folded into the
 // exponent: u_j = score_j + log2(sv_j), P_j = 2^(u_j - max u + 8) enters the second product as fp16 (the largest is between 2^8 and 2^15, so
 // the 11 bits reach 22 powers of two below it, whatever the scales are), and the sums of p and p (mv + 8 sv) take P_j / sv_j in fp32.
-// The sum of P code is far larger than that of P (code - 8), and the tensor cores cut off what an accumulator cannot hold, which
-// shortens it: one more product sums P * 8 the same way, and the difference goes to fp32 sums in shared memory after sixteen
-// chunks at most (lists of 20 to 41 K tokens: error 3.4e-4 of the outputs' size, after one chunk the same; without the flush 9e-4, without
+// The tensor cores cut sums off 2^-23 below their largest term as it is encoded, which for a code in the low bits is 2^-14 times P, and the sum
+// of P code is far larger than that of P (code - 8), so that it comes out short: one more product sums P * 8 the same way, and the
+// difference goes to fp32 sums in shared memory after sixteen chunks at most (lists of 20 to 41 K tokens: error 3.4e-4 of the outputs' size, after one chunk the same; without the flush 9e-4, without
 // either 2e-3; 2.6e-4 with the low terms of P that fp16 rows and groups of four heads at most have, 2.1e-4 being that of the output's own rounding).
 //
 // A warp works on 32 tokens at a time, two tiles of 16 that bulk copies bring into its own ring of two: S^T = K Q^T (16 tokens x 8 heads
 // of the group), then O^T += V^T P^T, with mma.sync m16n8k16: one product a token and KV head is a third of what the warp-level path can
 // issue while HBM brings the 136 bytes, and its operands need no pass through tensor memory.
-// 48 requests of 20 to 41 K tokens, 32 heads over 8 KV heads, fp16, 1.66 GB: 311 us, 5.3 TB/s, 0.83 of the measured copy rate (348 in
+// A group of more than eight heads takes a pass over the cache for every eight.
+// 48 requests of 20 to 41 K tokens, 32 heads over 8 KV heads, fp16, 1.66 GB: 312 us, 5.3 TB/s, 0.82 of the measured copy rate (349 in
 // sustained use).  16 requests of 16384 tokens: ALU pipe 51 % of active cycles, warp-level tensor pipe 28 %, issue slots 49 %: no unit is saturated.  When the kernel took
 // 332 us, copies without products took 272 and products without copies 276: neither alone explains the time.
 // The 32-token chunks of all (KV head, request) pairs form one list that is cut into equal parts, one a CTA, whatever the lengths are; the four
@@ -106,7 +107,7 @@ struct KdPlace {
 // NARROW: groups of four heads at most, which leave half of a fragment's columns empty.  The lanes of the empty columns take the scores of the
 // second tile, so that each has half as many exponentials; fp16 rows use the products' empty columns for
 // what the rounding of P to fp16 took off (bf16 rows round the result so much more that it does not show: 1.67e-3 with and without): 48 requests of
-// 20 to 41 K tokens 311 us and an error of 2.6e-4, without the low terms 303 and 3.4e-4, without NARROW 315; short requests the same.
+// 20 to 41 K tokens 312 us and an error of 2.6e-4, without the low terms 303 and 3.4e-4, without NARROW 315; short requests the same.
 template <class T, bool NARROW>
 __global__ void __launch_bounds__(KD_THREADS, KD_CTAS) attn_kv4_decode_kernel(KdParams p) {
     extern __shared__ __align__(128) uint8_t kd_smem[];

@@ -19,8 +19,8 @@
 // P is rounded to the rows' type, whose 8 or 11 bits the result has as well; its sum is taken before.  An fp16 P is kept between 2^8 and
 // 2^15 at the row's maximum, so that its normal numbers reach 22 powers of two below.  O is rescaled only when a row's maximum has grown by
 // more than 7 (bf16: 8) powers of two.
-// 4001 rows, 32 heads over 8 KV heads, bf16: 125 us, 1050 TFLOP/s, 0.63 of the measured rate (136 us in sustained use).  The tensor pipe is active
-// in 58 % of active cycles, the exponential unit in 40 %; a softmax warp waits 1140 of some 3660 cycles a tile for scores.
+// 4001 rows, 32 heads over 8 KV heads, bf16: 126 us, 1040 TFLOP/s, 0.62 of the measured rate (137 us in sustained use).  The tensor pipe is active
+// in 57 % of active cycles, the exponential unit in 40 %; in an earlier build with timers a softmax warp waited 1140 of some 3660 cycles a tile for scores.
 // All waits are bounded, by a second and what 32 rows done again may take: over 250000 keys 1.1 s, and the block behind them waits for that.
 // After a wait that gives up the error word is set, the rows that the CTA has begun are written as NaN, blocks that no other CTA takes stay
 // as they were, and the CTA leaves when its copies and MMAs in flight are done.

@@ -11,7 +11,7 @@ namespace qw3 {
 // One cluster.  Every CTA sums the lengths of all requests for itself (two prefix sums, of new tokens and of new pages, kept in shared
 // memory) and checks its share of the pages that will get tokens, the cluster meets, so that outputs may be the inputs' own buffers and a call that
 // cannot be served changes nothing, and then its threads fill the lists: a thread takes
-// four tokens in a row and finds their request by bisection.  Bound by latency, two dependent rounds of global loads: 10.3 us
+// four tokens in a row and finds their request by bisection.  Bound by latency, two dependent rounds of global loads: 10.4 us
 // for 7 requests, 14.4 for 250 with 34 K new tokens (launch included, caches cold).
 constexpr int PS_THREADS = 512;
 constexpr int PS_CLUSTER = 8;   // one CTA instead: the same up to 2500 new tokens of 8 requests (10.2 us), 16.4 instead of 10.2 for 8000, 41 instead of 14.3 for 34000

@@ -249,7 +249,7 @@ def page_slots(ctx_len, new_len, page_size, block_table, free_pages, n_free, max
 
 def rope_kv4_append(qkv, cache, slots, pos, cos, sin, heads, ws, pairs=False):
     """Rotates q and k of the rows qkv = [tokens][(heads + 2 kv_heads) * 128] by the angles of cos, sin = fp32 [max_pos][rot_dim / 2] (None: not
-    at all) at pos, and stores k and v in 4 bits in their slots (below 0: not stored).  Returns the rotated q [tokens][heads][128] and
+    at all) at pos, and stores k and v in 4 bits in their slots, which differ (below 0: not stored).  Returns the rotated q [tokens][heads][128] and
     k [tokens][kv_heads][128].  pairs: dims 2i and 2i + 1 turn together, as in rope_kv_append; else i and i + rot_dim / 2."""
     dev, kv, dtype = qkv.device, cache.kv_heads, cache.dtype
     _want(cache.device == dev, "qkv and the cache's pages: one device expected")

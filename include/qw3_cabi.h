@@ -183,8 +183,8 @@ int qw3_attn_prefill_poll_once(const void* d_qkv, const void* d_k_cache, const v
  * for code * scale + minimum:
  *   minimum = T(min), scale = max(T((max - minimum) / 15), floor), code = clamp(rint((x - minimum) / scale), 0, 15)
  * in fp32, T() rounding to the rows' type; the floor is 2^-24 (fp16) or 2^-60 (bf16).  A row with Inf or NaN (bf16: or with a range
- * of more than 15 * 2^60; fp16: or with a minimum that fp16 does not have, as a rotation may give) reads back as NaN.  16 tokens of a KV head lie together in 2176 bytes: 16 rows of 64 bytes of K codes (byte i:
- * dim 2i in the low nibble), the same of V, 16 pairs (scale, minimum) of K, 16 of V; a page is [kv_heads][page_size / 16] of these.
+ * of more than 15 * 2^60; fp16: or with a minimum that fp16 does not have, as a rotation may give) reads back as NaN.  16 tokens of a
+ * KV head lie together in 2176 bytes: 16 rows of 64 bytes of K codes (byte i: dim 2i in the low nibble), the same of V, 16 pairs (scale, minimum) of K, 16 of V; a page is [kv_heads][page_size / 16] of these.
  * A row of zero bytes, which was never stored, stands for zeros; qw3_attn_kv4_decode takes a V scale below the floor for the floor.
  *
  * A slot is page * page_size + offset.  What the device finds out of range (slots, pages, positions, lengths) is left out, never read
@@ -271,7 +271,8 @@ typedef struct Qw3AttnKv4Args {
 } Qw3AttnKv4Args;
 
 /* Attention of one token a request over its cached tokens (attentionKernel, Inference.cu:182-266, intended math), read as codes: the rows
- * are never expanded.  Scores, probabilities' sums and outputs are fp32; probabilities times V scales enter the products as
+ * are never expanded, and read once for every eight heads of a group.  A length that the table does not hold counts up to its end.
+ * Scores, probabilities' sums and outputs are fp32; probabilities times V scales enter the products as
  * fp16 (fp16 rows, groups of four heads at most: as two fp16 terms). */
 int qw3_attn_kv4_decode(const Qw3Kv4Pool* pool, const Qw3AttnKv4Args* args, qw3_ws_t ws, void* stream);
 
@@ -299,7 +300,8 @@ typedef struct Qw3AttnPackedArgs {
  * many KV heads as heads).  The queries of a sequence are its last rows: row i of its nq sees its keys 0 .. nk - nq + i, so that a prompt whose
  * beginning is in the cache attends to all of it; a row that sees no key is zeros.  Rows of d_out that belong to no sequence are left as
  * they were, and a sequence whose rows are not inside the buffers is left out (QW3_ERR_RANGE from qw3_ws_check).  Nothing that a row does not
- * see reaches it, Inf and NaN included.  Scores and sums are fp32, probabilities are rounded to the rows' type. */
+ * see reaches it, Inf and NaN included.  Scores and sums are fp32, probabilities are rounded to the rows' type once, 11 or 8 bits, where
+ * qw3_attn_prefill holds them as two fp16 terms: errors are 1.1 to 1.4 times those of the result's own rounding. */
 int qw3_attn_packed(const Qw3AttnPackedArgs* args, qw3_ws_t ws, void* stream);
 
 /* Embedding column gather straight from the packed [hidden][vocab] matrix (gather lambda,
